@@ -216,6 +216,109 @@ int sepia_cuda_banded_attn_noalloc(int kv_f16, const float *q, const void *k, co
                                    int64_t Dh, int64_t rel_extent, int64_t q_pos_base, int64_t kv_dim,
                                    float inv_head_dim, int64_t max_kv, void *stream);
 
+/* ------------------------------------------ paged 8-bit K/V cache (serving)
+ * No counterpart in the reference (one sequence, fp32 K/V in one flat array
+ * per layer). K and V of many sequences are held in blocks of `block` tokens;
+ * a block of one KV head is block x head_dim e4m3 codes and one power-of-two
+ * scale s, for K and for V each: value = code * s, with s the smallest power
+ * of two for which the block's largest magnitude / s is at most 448 (1 for a
+ * block of zeros). A floating code gains no precision from a finer scale, and
+ * dividing by a power of two is exact. The newest, unfinished block of a
+ * sequence is held in fp16 in the sequence's row of the tail arrays
+ * (magnitudes above 65504 saturate) and is rounded to 8 bits once, when its
+ * last token arrives: what the cache holds is a function of the tokens
+ * alone, however they were cut into calls. */
+typedef struct {
+    int32_t n_blocks, n_slots;           /* blocks of the pool, rows of the tail arrays */
+    int32_t n_kv_heads, head_dim, block; /* head_dim a multiple of 16 up to 128; block 16, 32 or 64 */
+    void *k, *v;                         /* [n_blocks, n_kv_heads, block, head_dim] e4m3; 16-byte aligned */
+    float *k_scale, *v_scale;            /* [n_blocks, n_kv_heads] */
+    void *k_tail, *v_tail;               /* [n_slots, n_kv_heads, block, head_dim] fp16; 16-byte aligned */
+} SepiaKv8Cache;
+
+/* One step of a batch: which sequences get how many new tokens. The arrays
+ * are DEVICE memory and are read when the kernels run, so a captured graph
+ * can be replayed as they change; the host passes bounds. kv_len is not
+ * advanced by the calls: append writes positions kv_len[s] ..., attention
+ * (after append) sees kv_len[s] plus the new tokens. A sequence with
+ * kv_len < 0 is idle: nothing is appended and its outputs are zero. A
+ * sequence that breaks a bound (more than max_new new tokens, more than max_kv
+ * in all, a block or slot out of range) is skipped the same way and sets the
+ * device error word to 2. Two sequences of a step never share a block that
+ * the step writes, nor a slot. */
+typedef struct {
+    int32_t n_seqs, n_tokens;            /* n_tokens: new tokens of all sequences */
+    int32_t max_new, max_kv;             /* per sequence: new tokens, tokens held after the step */
+    int32_t table_cols;
+    const int32_t *table;                /* [n_seqs, table_cols]: block of positions [c*block, (c+1)*block) */
+    const int32_t *kv_len;               /* [n_seqs]: tokens held before the step */
+    const int32_t *start;                /* [n_seqs + 1]: first new token of each sequence; NULL: one each */
+    const int32_t *slot;                 /* [n_seqs]: tail row; NULL: the sequence's own number */
+} SepiaKv8Step;
+
+/* New keys and values on their way into the cache, and the queries beside
+ * them. Optional, in this order: RMS norm of each head (k_norm, q_norm:
+ * [head_dim] weights), rotation of the first rot_dim dims by the token's
+ * position, and a factor per token on the query (q_scale). Strides count
+ * elements from one token to the next, so q, k and v may be slices of one
+ * projection's rows. */
+typedef struct {
+    int32_t x_f16;                       /* q, k, v and q_out: 1 fp16, 0 fp32 (arithmetic in fp32 either way) */
+    int32_t n_heads;                     /* query heads; read only with q */
+    const void *k, *v;                   /* [n_tokens, n_kv_heads, head_dim] */
+    int64_t k_stride, v_stride;
+    const void *q;                       /* [n_tokens, n_heads, head_dim] or NULL */
+    int64_t q_stride;
+    void *q_out;                         /* [n_tokens, n_heads, head_dim], contiguous; may be q itself */
+    const float *k_norm, *q_norm, *q_scale;
+    float eps;
+    int32_t rot_dim, rot_positions, rot_adjacent; /* rot_dim a multiple of 8; pairs (2i, 2i+1) or (i, i + rot_dim/2) */
+    const float *rotation;               /* [rot_positions, rot_dim/2, 2] cosines and sines, or NULL */
+} SepiaKv8Append;
+int sepia_cuda_kv8_append(const SepiaKv8Cache *c, const SepiaKv8Step *b, const SepiaKv8Append *a, void *stream);
+
+/* Causal attention of the new tokens over the cache, grouped query heads
+ * (n_heads a multiple of n_kv_heads): with p the token's position,
+ *   s[j] = scale * q.K[j] + (p - j < rel_extent ? rel_logits[n, h, p - j] * tau[n] : 0)
+ *   out = sum_j softmax(s)[j] V[j],   j in (p - window, p] (window 0: j in [0, p]).
+ * A row whose scores are all -infinity gives zeros. tau NULL means 1.
+ * The workspace (16-byte aligned, zeroed once by the caller; every call
+ * leaves its counters zero) belongs to one call at a time. */
+typedef struct {
+    int32_t x_f16;                       /* q and out: 1 fp16, 0 fp32 */
+    int32_t n_heads;
+    const void *q;                       /* [n_tokens, n_heads, head_dim], token stride q_stride */
+    int64_t q_stride;
+    void *out;                           /* [n_tokens, n_heads, head_dim], contiguous */
+    float scale;
+    int32_t window;
+    int32_t rel_extent;
+    const float *rel_logits;             /* [n_tokens, n_heads, rel_extent], or NULL with rel_extent 0 */
+    const float *tau;                    /* [n_tokens] or NULL */
+} SepiaKv8Attn;
+size_t sepia_cuda_kv8_attn_ws_bytes(const SepiaKv8Cache *c, const SepiaKv8Step *b, const SepiaKv8Attn *a);
+int sepia_cuda_kv8_attn(const SepiaKv8Cache *c, const SepiaKv8Step *b, const SepiaKv8Attn *a, void *ws,
+                        size_t ws_bytes, void *stream);
+
+/* ----------------------------------------------------------------- sampling
+ * One token per row of logits [rows, vocab] (row stride in elements) from
+ * one given uniform number u[row] in [0, 1) each. No counterpart in the
+ * reference (greedy only). Per row, with arrays that may be NULL (off):
+ *   e_i = exp((l_i - max) * (1/temperature)), w_i = e_i * 2^31 rounded to an integer;
+ *   order: greater logit first, among equals the lower index;
+ *   top_k (0: off): the first k; top_p (>= 1: off): of those, each token with
+ *   less than top_p of their weight before it; min_p (<= 0: off): e_i >= min_p;
+ *   id: the lowest index at which the running sum, in index order, of the
+ *   weights still in exceeds floor(u * their sum).
+ * temperature <= 0 takes the best token. Weights are summed as integers, so
+ * the result does not depend on the order of summation. NaN logits count as
+ * -infinity; a row without any finite or +infinite logit gives id -1 and
+ * prob 0. prob (may be NULL): the drawn token's share of the weights in.
+ * vocab at most 2^22. */
+int sepia_cuda_sample(int x_f16, const void *logits, int64_t stride, int32_t rows, int32_t vocab, const float *u,
+                      const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                      int32_t *ids, float *prob, void *stream);
+
 /* ------------------------------------------------------ synthetic weights */
 /* Fills n_units units (unit u at dst + u*unit_stride, blocks_per_unit
  * blocks of ggml_type each) with seeded random blocks: bytes uniform, every

@@ -1,0 +1,191 @@
+"""The paged 8-bit K/V cache of a serving batch (include/sepia_cuda.h,
+SepiaKv8Cache; csrc/kv8_append.cu, csrc/kv8_attn.cu).
+
+  Kv8Cache      one layer's blocks: e4m3 codes, a power-of-two scale per block
+                and KV head, fp16 tails of the unfinished blocks
+  Kv8Step       one step of a batch, shared by all layers: the block table,
+                the tokens held, the new tokens of each sequence
+  append        norms, rotates and stores new keys and values (and the queries
+                beside them); attention reads them back
+
+Tensors only carry device memory here; every computation is one of the
+library's CUDA kernels. A step's lengths stay on the device: a caller that
+replays a CUDA graph changes them in place.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from .lib import SepiaKv8Append, SepiaKv8Attn, SepiaKv8Cache, SepiaKv8Step, last_error, load
+
+_F16 = {torch.float32: 0, torch.float16: 1}
+
+
+def _need(cond, what):
+    if not cond:
+        raise ValueError(f"sepia_b200: kv8: {what}")
+
+
+def _check(t, name, dtype, shape=None):
+    _need(t.is_cuda and t.is_contiguous() and t.dtype == dtype, f"{name} must be a contiguous CUDA tensor of {dtype}")
+    _need(shape is None or tuple(t.shape) == tuple(shape), f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    return t.data_ptr()
+
+
+def _rows(t, name, heads, dim, n):
+    """A [tokens, heads, dim] tensor whose heads lie side by side; returns (pointer, token stride)."""
+    _need(t.is_cuda and t.dtype in _F16, f"{name} must be a float32 or float16 CUDA tensor")
+    _need(tuple(t.shape) == (n, heads, dim), f"{name} has shape {tuple(t.shape)}, expected {(n, heads, dim)}")
+    st = t.stride()
+    _need(n == 0 or (st[2] == 1 and (heads == 1 or st[1] == dim)), f"the heads of {name} must lie side by side")
+    return t.data_ptr(), st[0] if n > 1 else heads * dim
+
+
+def rotation_table(n_positions: int, rot_dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
+    """Cosines and sines [n_positions, rot_dim/2, 2] of angle position * base^(-2i/rot_dim), from 64-bit angles."""
+    freq = float(base) ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device) / rot_dim)
+    ang = torch.arange(n_positions, dtype=torch.float64, device=device)[:, None] * freq
+    return torch.stack([ang.cos(), ang.sin()], dim=-1).float().contiguous()
+
+
+class Kv8Step:
+    """One step of a batch. table int32 [n_seqs, columns], kv_len int32
+    [n_seqs] (tokens held before the step; < 0: idle), start int32
+    [n_seqs + 1] (None: one new token each), slot int32 [n_seqs] (None: row s
+    of the tails). n_tokens, max_new and max_kv are host bounds; max_kv
+    defaults to what the table can hold."""
+
+    def __init__(self, table, kv_len, start=None, slot=None, n_tokens=None, max_new=1, max_kv=None):
+        n = kv_len.shape[0]
+        _need(table.dim() == 2, "table must have two dimensions")
+        st = SepiaKv8Step()
+        st.table = _check(table, "table", torch.int32, (n, table.shape[1]))
+        st.kv_len = _check(kv_len, "kv_len", torch.int32, (n,))
+        st.start = _check(start, "start", torch.int32, (n + 1,)) if start is not None else None
+        st.slot = _check(slot, "slot", torch.int32, (n,)) if slot is not None else None
+        st.n_seqs, st.table_cols, st.max_new = n, table.shape[1], int(max_new)
+        st.n_tokens = n if n_tokens is None else int(n_tokens)
+        st.max_kv = -1 if max_kv is None else int(max_kv)
+        self.struct, self._keep = st, (table, kv_len, start, slot)
+        self.device = kv_len.device
+        self._max_kv, self._bound, self._ws = max_kv, {}, {}
+
+    def _for(self, cache):
+        """The step as a struct for this cache's block size, by reference."""
+        b = cache.struct.block
+        r = self._bound.get(b)
+        if r is None:
+            st = SepiaKv8Step.from_buffer_copy(self.struct)
+            if self._max_kv is None:
+                st.max_kv = st.table_cols * b
+            r = self._bound[b] = C.byref(st)
+        return r
+
+    def workspace(self, cache, attn, key):
+        """The attention workspace for one shape, zeroed once. One per stream: a workspace serves one call at a time."""
+        ws = self._ws.get(key)
+        if ws is None:
+            nb = load().sepia_cuda_kv8_attn_ws_bytes(C.byref(cache.struct), self._for(cache), C.byref(attn))
+            if not nb:
+                raise RuntimeError(f"sepia_b200: kv8_attn: {last_error()}")
+            t = torch.zeros(nb, dtype=torch.uint8, device=self.device)
+            ws = self._ws[key] = (t.data_ptr(), nb, t)
+        return ws
+
+
+class Kv8Cache:
+    """One layer's cache over tensors of the caller: k, v float8_e4m3fn
+    [n_blocks, n_kv_heads, block, head_dim], k_scale, v_scale float32
+    [n_blocks, n_kv_heads], k_tail, v_tail float16 [n_slots, n_kv_heads,
+    block, head_dim]."""
+
+    def __init__(self, k, v, k_scale, v_scale, k_tail, v_tail):
+        _need(k.dim() == 4 and k_tail.dim() == 4, "k and k_tail must have four dimensions")
+        n, hk, b, d = k.shape
+        st = SepiaKv8Cache()
+        st.n_blocks, st.n_slots, st.n_kv_heads, st.head_dim, st.block = n, k_tail.shape[0], hk, d, b
+        for name, t in (("k", k), ("v", v)):
+            setattr(st, name, _check(t, name, torch.float8_e4m3fn, (n, hk, b, d)))
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            setattr(st, name, _check(t, name, torch.float32, (n, hk)))
+        for name, t in (("k_tail", k_tail), ("v_tail", v_tail)):
+            setattr(st, name, _check(t, name, torch.float16, (k_tail.shape[0], hk, b, d)))
+        self.struct = st
+        self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail = k, v, k_scale, v_scale, k_tail, v_tail
+        self._ref, self._lib = C.byref(st), load()
+
+    @classmethod
+    def allocate(cls, n_blocks, n_slots, n_kv_heads, head_dim, block=32, device="cuda"):
+        def codes():
+            return torch.zeros(n_blocks, n_kv_heads, block, head_dim, dtype=torch.uint8,
+                               device=device).view(torch.float8_e4m3fn)
+
+        def scales():
+            return torch.ones(n_blocks, n_kv_heads, device=device)
+
+        def tails():
+            return torch.zeros(n_slots, n_kv_heads, block, head_dim, dtype=torch.float16, device=device)
+        return cls(codes(), codes(), scales(), scales(), tails(), tails())
+
+    def append(self, step, k, v, q=None, k_norm=None, q_norm=None, eps=1e-6, q_scale=None, rotation=None,
+               adjacent=False, q_out=None, stream=None):
+        """Stores the new tokens' keys and values (float32 or float16
+        [n_tokens, heads, head_dim]; a token's heads side by side, any token
+        stride): norm of each head, rotation by position, 8 bits. With q, also
+        norms, rotates and scales (q_scale float32 [n_tokens]) the queries into
+        q_out, which is returned."""
+        c, n = self.struct, step.struct.n_tokens
+        a = SepiaKv8Append()
+        a.x_f16 = _F16.get(k.dtype, 0)
+        a.k, a.k_stride = _rows(k, "k", c.n_kv_heads, c.head_dim, n)
+        a.v, a.v_stride = _rows(v, "v", c.n_kv_heads, c.head_dim, n)
+        _need(v.dtype == k.dtype, "k and v must have one type")
+        a.eps = eps
+        if k_norm is not None:
+            a.k_norm = _check(k_norm, "k_norm", torch.float32, (c.head_dim,))
+        if q is not None:
+            _need(q.dtype == k.dtype, "q and k must have one type")
+            h = q.shape[1]
+            a.n_heads = h
+            a.q, a.q_stride = _rows(q, "q", h, c.head_dim, n)
+            if q_out is None:
+                q_out = torch.empty((n, h, c.head_dim), dtype=q.dtype, device=q.device)
+            a.q_out = _check(q_out, "q_out", q.dtype, (n, h, c.head_dim))
+            if q_norm is not None:
+                a.q_norm = _check(q_norm, "q_norm", torch.float32, (c.head_dim,))
+            if q_scale is not None:
+                a.q_scale = _check(q_scale, "q_scale", torch.float32, (n,))
+        if rotation is not None:
+            _need(rotation.dim() == 3 and rotation.shape[2] == 2, "rotation must be [positions, rot_dim/2, 2]")
+            a.rotation = _check(rotation, "rotation", torch.float32)
+            a.rot_positions, a.rot_dim, a.rot_adjacent = rotation.shape[0], 2 * rotation.shape[1], int(adjacent)
+        st = stream if stream is not None else torch.cuda.current_stream(step.device)
+        if not self._lib.sepia_cuda_kv8_append(self._ref, step._for(self), C.byref(a), st.cuda_stream):
+            raise RuntimeError(f"sepia_b200: kv8_append failed: {last_error()}")
+        return q_out
+
+    def attention(self, step, q, scale, window=0, rel_logits=None, tau=None, out=None, stream=None):
+        """Causal attention of the new tokens (after append) over what the
+        cache holds of their sequences. rel_logits float32 [n_tokens, heads,
+        extent] is added at distance 0 .. extent-1, times tau[token]."""
+        c, n = self.struct, step.struct.n_tokens
+        _need(q.dim() == 3, "q must be [tokens, heads, head_dim]")
+        h = q.shape[1]
+        a = SepiaKv8Attn()
+        a.x_f16, a.n_heads, a.scale, a.window = _F16.get(q.dtype, 0), h, scale, window
+        a.q, a.q_stride = _rows(q, "q", h, c.head_dim, n)
+        if out is None:
+            out = torch.empty((n, h, c.head_dim), dtype=q.dtype, device=q.device)
+        a.out = _check(out, "out", q.dtype, (n, h, c.head_dim))
+        if rel_logits is not None:
+            a.rel_extent = rel_logits.shape[-1]
+            a.rel_logits = _check(rel_logits, "rel_logits", torch.float32, (n, h, a.rel_extent))
+        if tau is not None:
+            a.tau = _check(tau, "tau", torch.float32, (n,))
+        st = (stream if stream is not None else torch.cuda.current_stream(step.device)).cuda_stream
+        ws = step.workspace(self, a, (st, a.x_f16, h, c.n_kv_heads, c.head_dim, c.block, window))
+        if not self._lib.sepia_cuda_kv8_attn(self._ref, step._for(self), C.byref(a), ws[0], ws[1], st):
+            raise RuntimeError(f"sepia_b200: kv8_attn failed: {last_error()}")
+        return out

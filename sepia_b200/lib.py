@@ -75,6 +75,28 @@ class SepiaModelDesc(C.Structure):
                 ("layers", C.POINTER(SepiaModelLayer)), ("rank", i32), ("world", i32)]
 
 
+class SepiaKv8Cache(C.Structure):
+    _fields_ = [("n_blocks", i32), ("n_slots", i32), ("n_kv_heads", i32), ("head_dim", i32), ("block", i32),
+                ("k", vp), ("v", vp), ("k_scale", vp), ("v_scale", vp), ("k_tail", vp), ("v_tail", vp)]
+
+
+class SepiaKv8Step(C.Structure):
+    _fields_ = [("n_seqs", i32), ("n_tokens", i32), ("max_new", i32), ("max_kv", i32), ("table_cols", i32),
+                ("table", vp), ("kv_len", vp), ("start", vp), ("slot", vp)]
+
+
+class SepiaKv8Append(C.Structure):
+    _fields_ = [("x_f16", i32), ("n_heads", i32), ("k", vp), ("v", vp), ("k_stride", i64), ("v_stride", i64),
+                ("q", vp), ("q_stride", i64), ("q_out", vp), ("k_norm", vp), ("q_norm", vp), ("q_scale", vp),
+                ("eps", C.c_float), ("rot_dim", i32), ("rot_positions", i32), ("rot_adjacent", i32),
+                ("rotation", vp)]
+
+
+class SepiaKv8Attn(C.Structure):
+    _fields_ = [("x_f16", i32), ("n_heads", i32), ("q", vp), ("q_stride", i64), ("out", vp), ("scale", C.c_float),
+                ("window", i32), ("rel_extent", i32), ("rel_logits", vp), ("tau", vp)]
+
+
 # name -> (restype, argtypes)
 _PROTOS = {
     # ---- sepia_gpu.h (reference ABI) ----
@@ -146,6 +168,13 @@ _PROTOS = {
     "sepia_cuda_exchange_connect": (C.c_int, [vp, vp]),
     "sepia_cuda_moe_exchange": (C.c_int, [vp, C.POINTER(SepiaMoeLayer), C.POINTER(SepiaMoeWork), vp, vp]),
     "sepia_cuda_moe_layer_sharded": (C.c_int, [vp, C.POINTER(SepiaMoeLayer), vp, C.POINTER(SepiaMoeWork), vp, vp]),
+    "sepia_cuda_kv8_append": (C.c_int, [C.POINTER(SepiaKv8Cache), C.POINTER(SepiaKv8Step),
+                                        C.POINTER(SepiaKv8Append), vp]),
+    "sepia_cuda_kv8_attn_ws_bytes": (C.c_size_t, [C.POINTER(SepiaKv8Cache), C.POINTER(SepiaKv8Step),
+                                                  C.POINTER(SepiaKv8Attn)]),
+    "sepia_cuda_kv8_attn": (C.c_int, [C.POINTER(SepiaKv8Cache), C.POINTER(SepiaKv8Step), C.POINTER(SepiaKv8Attn),
+                                      vp, C.c_size_t, vp]),
+    "sepia_cuda_sample": (C.c_int, [C.c_int, vp, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
     "sepia_cuda_fill_blocks": (C.c_int, [C.c_int, vp, i64, i64, i64, C.c_uint64, i64, i64, C.c_float, C.c_float, vp]),
     # ---- sepia_model.h (whole-token decode engine) ----
     "sepia_model_create": (C.c_int, [C.POINTER(SepiaModelDesc), C.POINTER(vp)]),
