@@ -460,3 +460,30 @@ def test_no_tokens(lib):
     k = torch.zeros(0, 2, 32, device="cuda")
     q = c.append(step, k, k, q=torch.zeros(0, 4, 32, device="cuda"))
     assert c.attention(step, q, 1.0).shape == (0, 4, 32)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("held,window", [(53, 20), (41, 0)])
+def test_attention_not_numbers_behind_a_mask(lib, dtype, held, window):
+    """Keys and values that are NaN at positions that a token does not see
+    (behind its window, or later new tokens) leave its output as it is; a
+    token that sees one gets NaN."""
+    hk, h, dim, new = 2, 6, 64, 4
+    outs = []
+    for spoil in (False, True):
+        B = Batch([0], hk, dim, 16, seed=6)
+        rng = np.random.default_rng(8)
+        k = torch.tensor(rng.standard_normal((held + new, hk, dim)), dtype=F32, device="cuda")
+        v = torch.tensor(rng.standard_normal((held + new, hk, dim)), dtype=F32, device="cuda")
+        if spoil:
+            v[held + new - 1, 1, 7] = k[held + new - 1, 0, 3] = float("nan")      # the last new token: seen by itself only
+            if window:
+                v[held + new - 1 - window - 3, 0, 5] = float("nan")              # behind every window, in a tile that is read
+                k[held + new - 1 - window - 3, 1, 2] = float("nan")
+        B.append([held], k=k[:held], v=v[:held])
+        step = B.step([new])
+        q = torch.tensor(rng.standard_normal((new, h, dim)), dtype=dtype, device="cuda")
+        B.cache.append(step, k[held:].contiguous(), v[held:].contiguous())
+        outs.append(B.cache.attention(step, q, 1.0 / dim, window=window))
+    assert torch.equal(outs[0][: new - 1], outs[1][: new - 1])
+    assert torch.isnan(outs[1][new - 1]).view(hk, -1).any(dim=1).all()
