@@ -282,8 +282,9 @@ int sepia_cuda_kv8_append(const SepiaKv8Cache *c, const SepiaKv8Step *b, const S
  *   s[j] = scale * q.K[j] + (p - j < rel_extent ? rel_logits[n, h, p - j] * tau[n] : 0)
  *   out = sum_j softmax(s)[j] V[j],   j in (p - window, p] (window 0: j in [0, p]).
  * A row whose scores are all -infinity gives zeros. tau NULL means 1.
- * The workspace (16-byte aligned, zeroed once by the caller; every call
- * leaves its counters zero) belongs to one call at a time. */
+ * The workspace (16-byte aligned, never read before it is written) belongs
+ * to one call at a time. A key or value that is not a number spoils the rows
+ * that see its position, and no other. */
 typedef struct {
     int32_t x_f16;                       /* q and out: 1 fp16, 0 fp32 */
     int32_t n_heads;

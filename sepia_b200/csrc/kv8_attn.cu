@@ -7,9 +7,10 @@
 //
 //   Work      grid (split, KV head x row tile, sequence); a CTA owns a chunk
 //             of positions, its warps take 16-key tiles of it in turn, each
-//             with its own maximum, sum and output, merged at the end. The
-//             chunks of a long context are merged by the CTA that finishes
-//             last, in chunk order.
+//             with its own maximum, sum and output, merged at the end. A
+//             second kernel merges the chunks of a long context, many rows
+//             at once (as the last step of the last CTA of each KV head the
+//             same sum took 65 us of 95 at 1 x 32768: 8 CTAs at work).
 //   Operands  mma m16n8k16 in fp16 with fp32 sums. e4m3 codes are fp16
 //             numbers exactly; block scales multiply the score and the
 //             weight. fp32 rows: q and the weight are split into two fp16
@@ -46,7 +47,6 @@ struct K8Params {
     SepiaKv8Step b;
     SepiaKv8Attn a;
     int G, row_tiles, splits, chunk;     // chunk: positions per split, a multiple of kK8Tile * kK8Warps
-    uint32_t *counter;                   // [n_seqs, n_kv_heads * row_tiles]
     float *part;                         // [n_seqs, n_kv_heads * row_tiles, splits, rows of a tile, Dh + 2]
     int *err;
 };
@@ -106,7 +106,6 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
     using F = K8Cfg<T, DP>;
     constexpr int RL = F::RL, RT = F::RT;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ int s_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
     const int split = blockIdx.x, s = blockIdx.z;
     const int hk = blockIdx.y / P.row_tiles, rt = blockIdx.y - hk * P.row_tiles;
@@ -511,36 +510,74 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
             to[2 + d] = A;
         }
     }
-    if (n_act == 1) return;
-    // ---- merge the chunks: the CTA that finishes last, in chunk order ----
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) {
-        const uint32_t done = atomicAdd(P.counter + group, 1u) + 1u;
-        s_last = done == (uint32_t)n_act;
-        if (s_last) P.counter[group] = 0;
-    }
-    __syncthreads();
-    if (!s_last) return;
-    __threadfence();
-    for (int i = tid; i < live * Dh; i += kK8Threads) {
-        const int r = i / Dh, d = i - r * Dh;
-        const float *o = part + r * (Dh + 2);
-        float M = -INFINITY, L = 0.0f, A = 0.0f;
-        for (int k = 0; k < n_act; k++) M = fmaxf(M, __ldcg(o + k * stride));
-        for (int k = 0; k < n_act; k++) {
-            const float mk = __ldcg(o + k * stride);
-            const float f = mk == -INFINITY ? 0.0f : exp2_fast((mk - M) * kLog2e);
-            L += f * __ldcg(o + k * stride + 1);
-            A += f * __ldcg(o + k * stride + 2 + d);
+}
+
+// Merges the chunks of a row, in chunk order within each of the W warps that
+// share the row, then across the warps. One CTA does kK8Warps / W rows.
+template <typename T, int W>
+__global__ void __launch_bounds__(kK8Threads) k_kv8_merge(const K8Params P) {
+    constexpr int RT = sizeof(T) == 4 ? 8 : 16;
+    __shared__ float s_part[W > 1 ? kK8Warps : 1][kKv8MaxDh + 2];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, d = 4 * lane;
+    const int Dh = P.c.head_dim, H = P.a.n_heads, G = P.G, s = blockIdx.y;
+    griddep_wait();
+    griddep_launch();
+    const int at = blockIdx.x * (kK8Warps / W) + warp / W, h = at % H, t = at / H;
+    const Kv8Seq sq = kv8_seq(P.c, P.b, s, nullptr);
+    if (sq.add < 0 || t >= sq.add) return;             // with W > 1 the whole CTA
+    // the row's tile, and the chunks that k_kv8_attn cut for it
+    const int hk = h / G, R = t * G + h - hk * G, rt = R / RT, r = R - rt * RT;
+    const int ta = rt * RT / G, tb = min(sq.add - 1, (rt * RT + RT - 1) / G);
+    const int lo = P.a.window ? max(0, sq.held + ta - P.a.window + 1) / kK8Tile * kK8Tile : 0;
+    const int n_act = (sq.held + tb + 1 - lo + P.chunk - 1) / P.chunk;
+    if (n_act <= 1) return;
+    const int group = s * P.c.n_kv_heads * P.row_tiles + hk * P.row_tiles + rt;
+    const int64_t stride = (int64_t)RT * (Dh + 2);
+    const float *part = P.part + (int64_t)group * P.splits * stride + (int64_t)r * (Dh + 2);
+    float M = -INFINITY, L = 0.0f, A[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = lane; k < n_act; k += 32) M = fmaxf(M, part[k * stride]);
+    M = warp_max(M);
+    const int per = (n_act + W - 1) / W, k0 = (warp % W) * per, k1 = min(n_act, k0 + per);
+    constexpr int kAhead = 8;                          // chunks in flight per warp
+    for (int k = k0; k < k1; k += kAhead) {
+        float2 x[kAhead][2], ml[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            const float2 *p = reinterpret_cast<const float2 *>(part + min(k + i, k1 - 1) * stride);
+            ml[i] = p[0];
+            x[i][0] = d < Dh ? p[1 + d / 2] : make_float2(0.0f, 0.0f);
+            x[i][1] = d < Dh ? p[2 + d / 2] : make_float2(0.0f, 0.0f);
         }
-        put(r, d, A, L);
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            if (k + i >= k1) break;
+            const float f = ml[i].x == -INFINITY ? 0.0f : exp2_fast((ml[i].x - M) * kLog2e);
+            L += f * ml[i].y;
+            A[0] += f * x[i][0].x, A[1] += f * x[i][0].y, A[2] += f * x[i][1].x, A[3] += f * x[i][1].y;
+        }
+    }
+    if constexpr (W > 1) {
+        if (d < Dh)
+            for (int e = 0; e < 4; e++) s_part[warp][2 + d + e] = A[e];
+        if (lane == 0) s_part[warp][0] = L;
+        __syncthreads();
+        if (warp) return;
+#pragma unroll
+        for (int w = 1; w < W; w++) {
+            L += s_part[w][0];
+            if (d < Dh)
+                for (int e = 0; e < 4; e++) A[e] += s_part[w][2 + d + e];
+        }
+    }
+    if (d < Dh) {
+        T *o = (T *)P.a.out + ((int64_t)(sq.n0 + t) * H + h) * Dh + d;
+        for (int e = 0; e < 4; e++) o[e] = (T)(L == 0.0f ? 0.0f : A[e] / L);
     }
 }
 
 struct K8Plan {
     int G, row_tiles, splits, chunk;
-    size_t counter_bytes, bytes;
+    size_t bytes;
 };
 
 // Chunks: one wave of equal chunks over all CTA slots while that leaves a
@@ -558,8 +595,7 @@ static K8Plan k8_plan(const SepiaKv8Cache &c, const SepiaKv8Step &b, const Sepia
     const int64_t one = (groups * span + slots - 1) / slots;
     p.chunk = (int)(std::min(kMaxChunk, std::max<int64_t>(one, 1)) + kUnit - 1) / kUnit * kUnit;
     p.splits = (int)std::max<int64_t>(1, (span + p.chunk - 1) / p.chunk);
-    p.counter_bytes = ((size_t)groups * 4 + 255) / 256 * 256;
-    p.bytes = p.counter_bytes + (p.splits > 1 ? (size_t)groups * p.splits * rt * (c.head_dim + 2) * 4 : 0);
+    p.bytes = p.splits > 1 ? (size_t)groups * p.splits * rt * (c.head_dim + 2) * 4 : 0;
     return p;
 }
 
@@ -568,7 +604,14 @@ static int k8_launch(const K8Params &P, cudaStream_t st) {
     constexpr int smem = K8Cfg<T, DP>::kSmem;
     if (!ensure_smem((const void *)k_kv8_attn<T, DP>, smem)) return 0;
     const dim3 grid((unsigned)P.splits, (unsigned)(P.c.n_kv_heads * P.row_tiles), (unsigned)P.b.n_seqs);
-    return check(launch_pdl(k_kv8_attn<T, DP>, grid, dim3(kK8Threads), smem, st, P), "kv8_attn launch");
+    if (!check(launch_pdl(k_kv8_attn<T, DP>, grid, dim3(kK8Threads), smem, st, P), "kv8_attn launch")) return 0;
+    if (P.splits == 1) return 1;
+    // one warp per row while a row has few chunks, four beyond
+    const int64_t rows = (int64_t)P.b.max_new * P.a.n_heads;
+    const dim3 g1((unsigned)((rows + kK8Warps - 1) / kK8Warps), (unsigned)P.b.n_seqs), g4((unsigned)rows, (unsigned)P.b.n_seqs);
+    const cudaError_t e = P.splits <= 8 ? launch_pdl(k_kv8_merge<T, 1>, g1, dim3(kK8Threads), 0, st, P)
+                                        : launch_pdl(k_kv8_merge<T, 4>, g4, dim3(kK8Threads), 0, st, P);
+    return check(e, "kv8_attn merge launch");
 }
 
 static int k8_check(const SepiaKv8Cache *c, const SepiaKv8Step *b, const SepiaKv8Attn *a) {
@@ -602,7 +645,7 @@ extern "C" int sepia_cuda_kv8_attn(const SepiaKv8Cache *c, const SepiaKv8Step *b
     if (a->rel_extent && !a->rel_logits) return fail("%s: rel_extent without rel_logits", what);
     const K8Plan p = k8_plan(*c, *b, *a);
     if ((int64_t)c->n_kv_heads * p.row_tiles > 65535) return fail("%s: step too large", what);
-    if (!ws || ws_bytes < p.bytes) return fail("%s: workspace of %zu bytes < %zu needed", what, ws_bytes, p.bytes);
+    if (!ws || ws_bytes < std::max<size_t>(16, p.bytes)) return fail("%s: workspace of %zu bytes < %zu needed", what, ws_bytes, p.bytes);
     if (reinterpret_cast<uintptr_t>(ws) & 15) return fail("%s: workspace must be 16-byte aligned", what);
     K8Params P;
     P.c = *c;
@@ -612,8 +655,7 @@ extern "C" int sepia_cuda_kv8_attn(const SepiaKv8Cache *c, const SepiaKv8Step *b
     P.row_tiles = p.row_tiles;
     P.splits = p.splits;
     P.chunk = p.chunk;
-    P.counter = (uint32_t *)ws;
-    P.part = (float *)((char *)ws + p.counter_bytes);
+    P.part = (float *)ws;
     P.err = dev_info().err;
     cudaStream_t st = as_stream(stream);
     if (c->head_dim <= 64) return a->x_f16 ? k8_launch<__half, 64>(P, st) : k8_launch<float, 64>(P, st);

@@ -84,13 +84,13 @@ class Kv8Step:
         return r
 
     def workspace(self, cache, attn, key):
-        """The attention workspace for one shape, zeroed once. One per stream: a workspace serves one call at a time."""
+        """The attention workspace for one shape. One per stream: a workspace serves one call at a time."""
         ws = self._ws.get(key)
         if ws is None:
             nb = load().sepia_cuda_kv8_attn_ws_bytes(C.byref(cache.struct), self._for(cache), C.byref(attn))
             if not nb:
                 raise RuntimeError(f"sepia_b200: kv8_attn: {last_error()}")
-            t = torch.zeros(nb, dtype=torch.uint8, device=self.device)
+            t = torch.empty(nb, dtype=torch.uint8, device=self.device)
             ws = self._ws[key] = (t.data_ptr(), nb, t)
         return ws
 
