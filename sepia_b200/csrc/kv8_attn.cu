@@ -26,44 +26,51 @@
 
 #include <cuda_fp16.h>
 #include <algorithm>
+#include <type_traits>
 
 namespace sepia {
 
 constexpr int kK8Warps = 4;
 constexpr int kK8Threads = 32 * kK8Warps;
-constexpr int kK8Tile = 16;              // keys per warp step
+constexpr int kK8Tile = 16;              // keys of one scale: a block is a multiple of it
+constexpr int kK8Unit = 2 * kK8Tile;     // keys per warp step
+constexpr int kK8Stages = 2;             // steps in a warp's ring
 constexpr int kK8CtasPerSm = 3;
 constexpr float kLog2e = 1.4426950408889634f;
-// A weight's exponent may pass the running maximum by this before the
-// maximum is moved (and the output rescaled): weights reach e^5.5 = 245,
-// times kPOne below 65504, the largest fp16.
-constexpr float kSlack = 5.5f;
-// Weights are handed to the tensor core times 2^7: with the slack that keeps
-// 22 bits of a weight down to 2^-20 of the largest.
-constexpr float kPOne = 128.0f;
+constexpr float kLowest = -3.402823466e38f;
+// Weights reach the tensor core as 2^(score - maximum + kPBits), in base 2.
+// The maximum is only moved (and the output rescaled) when a weight would
+// pass 2^15, so it may lag; kPBits leaves it 8 binary places to do so and
+// keeps 22 bits of a weight down to 2^-20 of the largest.
+constexpr float kPBits = 7.0f, kPMax = 15.0f;
 
 struct K8Params {
     SepiaKv8Cache c;
     SepiaKv8Step b;
     SepiaKv8Attn a;
-    int G, row_tiles, splits, chunk;     // chunk: positions per split, a multiple of kK8Tile * kK8Warps
+    int G, row_tiles, splits, chunk;     // chunk: positions per split, a multiple of kK8Unit * kK8Warps
+    int bias_rows;                       // rows of a lane that have a band: 0, 1 or 2
+    uint32_t two16;
     float *part;                         // [n_seqs, n_kv_heads * row_tiles, splits, rows of a tile, Dh + 2]
     int *err;
 };
 
-__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t two) {
+// The low two e4m3 codes of a word as fp16: one conversion. The high two
+// are first moved down by a multiplication (high half of x * 2^16), which
+// runs beside the conversions: shifts, permutes and conversions share one
+// pipe of half the rate (measured 64 lanes a clock and SM each).
+__device__ __forceinline__ uint32_t e4m3_lo(uint32_t x) {
     uint32_t r;
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(r) : "r"(two));
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(r) : "r"(x));
     return r;
 }
-__device__ __forceinline__ uint32_t e4m3x2_to_half2_hi(uint32_t two) {
-    uint32_t r;
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(two));
-    return r;
+__device__ __forceinline__ uint32_t e4m3_hi(uint32_t x, uint32_t two16) {
+    uint32_t y;
+    asm("mul.hi.u32 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(two16));
+    return e4m3_lo(y);
 }
 __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -72,7 +79,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// cp.async of `bytes` (16 or 8 or 4) or of zeros
+// cp.async of N (16, 8 or 4) bytes; of zeros where `on` is false
+template <int N>
+__device__ __forceinline__ void cp_async_bytes(uint32_t dst, const void *src) {
+    if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
+}
 template <int N>
 __device__ __forceinline__ void cp_async_or_zero(uint32_t dst, const void *src, bool on) {
     const int n = on ? N : 0;
@@ -94,14 +106,17 @@ struct K8Cfg {
     static constexpr int KW = DP / 64;                // 16-byte pieces of a key row per lane
     static constexpr int VB = DP / 8;                 // bytes of a value row per lane
     static constexpr int NT = DP / 8, KS = DP / 16;   // output columns of 8, k steps of 16
-    static constexpr int kStages = kTwo ? 4 : 3;
-    static constexpr int kKeyB = 2 * KW * 512, kValB = 4 * VB * 32, kBiasB = 4 * RL * 128;
-    static constexpr int kStageB = kKeyB + kValB + kBiasB + 16;   // the last 16: the block's scales
-    static constexpr int kMergeB = kK8Warps * RT * (DP + 2) * 4;
-    static constexpr int kSmem = kStages * kStageB * kK8Warps > kMergeB ? kStages * kStageB * kK8Warps : kMergeB;
+    static constexpr int kKeyB = 2 * KW * 512, kValB = 4 * VB * 32, kTileB = kKeyB + kValB;
+    static constexpr int kHeadB = 16;                 // a step's scales
+    static constexpr int kPitch = DP + 8;             // of a merge row: 8 rows of 8-byte stores meet no bank twice
+    static constexpr int kMergeB = kK8Warps * RT * kPitch * 4;
+    // bytes of a ring stage with the bias of `rows` rows a lane
+    static constexpr int stage(int rows) { return 2 * kTileB + kHeadB + rows * 8 * 128; }
 };
 
-template <typename T, int DP>
+// FULL: head_dim is DP (64 or 128), every offset a constant; otherwise the
+// dims past head_dim are read as zeros.
+template <typename T, int DP, bool FULL>
 __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8Params P) {
     using F = K8Cfg<T, DP>;
     constexpr int RL = F::RL, RT = F::RT;
@@ -109,7 +124,7 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
     const int split = blockIdx.x, s = blockIdx.z;
     const int hk = blockIdx.y / P.row_tiles, rt = blockIdx.y - hk * P.row_tiles;
-    const int Dh = P.c.head_dim, B = P.c.block, H = P.a.n_heads, Hkv = P.c.n_kv_heads, G = P.G;
+    const int Dh = FULL ? DP : P.c.head_dim, B = P.c.block, H = P.a.n_heads, Hkv = P.c.n_kv_heads, G = P.G;
     griddep_wait();
     griddep_launch();
     const Kv8Seq sq = kv8_seq(P.c, P.b, s, P.err);
@@ -133,19 +148,94 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
     if (split >= n_act) return;
     const int c0 = lo + split * P.chunk, c1 = min(pb + 1, c0 + P.chunk);
 
+    // ---- coded steps: this warp's share of [c0, min(c1, tail0)), through its ring ----
+    const int ce = min(c1, tail0);
+    const int n_units = ce > c0 ? (ce - c0 + kK8Unit - 1) / kK8Unit : 0;
+    const int mine = n_units > warp ? (n_units - warp + kK8Warps - 1) / kK8Warps : 0;
+    const int stage_b = F::stage(P.bias_rows);
+    uint8_t *ring = smem + warp * kK8Stages * stage_b;
+    const uint32_t ring_u = smem_u32(ring);
+    int pos[RL];
+    const float *rel[RL];
+#pragma unroll
+    for (int j = 0; j < RL; j++) {
+        const int R = min(rt * RT + gid + 8 * j, sq.add * G - 1), t = R / G;
+        pos[j] = sq.held + t;
+        rel[j] = P.a.rel_logits + ((int64_t)(sq.n0 + t) * H + hk * G + R - t * G) * E;
+    }
+    int id_l = 0;
+    float ks_l = -1.0f, ev_l = 0.0f;
+    auto issue = [&](int i) {
+        if (i < mine) {
+            if ((i & 15) == 0) {                       // lane: tile lane % 2 of step i + lane / 2
+                const int at = c0 + (warp + kK8Warps * (i + (lane >> 1))) * kK8Unit + (lane & 1) * kK8Tile;
+                ks_l = -1.0f;                          // a tile that is not there: all its keys hidden
+                ev_l = 0.0f;
+                id_l = 0;
+                if (at < ce) {
+                    const int id = kv8_block(P.c, P.b, s, at / B, P.err);
+                    if (id >= 0) {
+                        id_l = id;
+                        ks_l = P.c.k_scale[(int64_t)id * Hkv + hk];
+                        ev_l = (float)((int)(__float_as_uint(P.c.v_scale[(int64_t)id * Hkv + hk]) >> 23 & 255) - 127);
+                    }
+                }
+            }
+            const int t0 = c0 + (warp + kK8Warps * i) * kK8Unit;
+            const uint32_t st = ring_u + (i & (kK8Stages - 1)) * stage_b;
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int id = __shfl_sync(0xffffffffu, id_l, (2 * i + u) & 31);
+                const int64_t row0 = ((int64_t)id * Hkv + hk) * B + ((t0 + u * kK8Tile) & (B - 1));
+                const uint8_t *K = (const uint8_t *)P.c.k + row0 * Dh + gid * Dh + 16 * tig;
+                const uint8_t *V = (const uint8_t *)P.c.v + row0 * Dh + 2 * tig * Dh + gid * F::VB;
+                const uint32_t at = st + u * F::kTileB + lane * 16;
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int j = 0; j < F::KW; j++) {
+                        if constexpr (FULL) cp_async_bytes<16>(at + (n * F::KW + j) * 512, K + n * 8 * Dh + j * 64);
+                        else cp_async_or_zero<16>(at + (n * F::KW + j) * 512, K + n * 8 * Dh + j * 64, 64 * j + 16 * tig < Dh);
+                    }
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t to = st + u * F::kTileB + F::kKeyB + k * (32 * F::VB) + lane * F::VB;
+                    const uint8_t *src = V + ((k & 1) + 8 * (k >> 1)) * Dh;
+                    if constexpr (FULL) cp_async_bytes<F::VB>(to, src);
+                    else cp_async_or_zero<F::VB>(to, src, gid * F::VB < Dh);
+                }
+            }
+            if (E && pa - (t0 + kK8Unit - 1) < E) {
+#pragma unroll
+                for (int j = 0; j < RL; j++) {
+                    if (j >= P.bias_rows) break;
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const int far = pos[j] - (t0 + 2 * tig + (k & 1) + 8 * (k >> 1));
+                        const bool on = far >= 0 && far < E;
+                        cp_async_or_zero<4>(st + 2 * F::kTileB + F::kHeadB + (8 * j + k) * 128 + lane * 4,
+                                            rel[j] + (on ? far : 0), on);
+                    }
+                }
+            }
+            if ((lane >> 1) == (i & 15))
+                *reinterpret_cast<float2 *>(ring + (i & (kK8Stages - 1)) * stage_b + 2 * F::kTileB + 8 * (lane & 1)) =
+                    make_float2(ks_l, ev_l);
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < kK8Stages - 1; i++) issue(i);
+
     // ---- this lane's rows and their q operand ----
-    int pos[RL], n_row[RL], h_row[RL];
     float qmul[RL], tau[RL];
     uint32_t qa[F::KS][4];
 #pragma unroll
     for (int j = 0; j < RL; j++) {
         const int r = gid + 8 * j, R = min(rt * RT + r, sq.add * G - 1), t = R / G;
         const bool on = r < rows;
-        n_row[j] = sq.n0 + t;
-        pos[j] = sq.held + t;
-        h_row[j] = hk * G + R - t * G;
-        tau[j] = P.a.tau && on ? P.a.tau[n_row[j]] : 1.0f;
-        const T *q = (const T *)P.a.q + (int64_t)n_row[j] * P.a.q_stride + (int64_t)h_row[j] * Dh;
+        tau[j] = P.a.tau && on ? P.a.tau[sq.n0 + t] : 1.0f;
+        const T *q = (const T *)P.a.q + (int64_t)(sq.n0 + t) * P.a.q_stride + (int64_t)(hk * G + R - t * G) * Dh;
         float x[F::KS][4], amax = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < F::KS; ks++) {
@@ -162,7 +252,7 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
             const int ex = amax > 0.0f ? max((int)(__float_as_uint(amax) >> 23) - 127, -100) : 13;
             const float f = __uint_as_float((uint32_t)(127 + 13 - ex) << 23);
-            qmul[j] = P.a.scale * __uint_as_float((uint32_t)(127 - 13 + ex) << 23);
+            qmul[j] = P.a.scale * kLog2e * __uint_as_float((uint32_t)(127 - 13 + ex) << 23);
 #pragma unroll
             for (int ks = 0; ks < F::KS; ks++) {
 #pragma unroll
@@ -175,7 +265,7 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
                 }
             }
         } else {
-            qmul[j] = P.a.scale;
+            qmul[j] = P.a.scale * kLog2e;
 #pragma unroll
             for (int ks = 0; ks < F::KS; ks++) {
                 qa[ks][j] = pack_half2(x[ks][0], x[ks][1]);
@@ -184,78 +274,108 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
         }
     }
 
-    float O[F::NT][4], m[RL], l[RL], vref = 0.0f;
+    // Running maximum in base 2 (a lag is allowed), sum, and output / 2^eref.
+    float O[F::NT][4], m2[RL], l[RL], eref = -1000.0f;
 #pragma unroll
     for (int nt = 0; nt < F::NT; nt++) O[nt][0] = O[nt][1] = O[nt][2] = O[nt][3] = 0.0f;
 #pragma unroll
-    for (int j = 0; j < RL; j++) m[j] = -INFINITY, l[j] = 0.0f;
+    for (int j = 0; j < RL; j++) m2[j] = kLowest, l[j] = 0.0f;
 
-    // One 16-key tile at position t0. kf(n, ks, b0, b1): key fragment of keys
-    // t0 + 8n + gid; vf(nt, b0, b1): value fragment; bias(j, i): term i of
-    // this lane's row j, keys t0 + 2 tig + {0, 1, 8, 9}; clean(): values that
-    // are not numbers to 0, and which of those keys had any.
-    auto tile = [&](int t0, float ks_, float vs, auto kf, auto vf, auto bias, auto clean) {
-        float S[2][4];
+    // One step of U 16-key tiles from position t0; ksc, ev: each tile's key
+    // scale (negative: hidden) and the exponent of its value scale.
+    // kf(S): the key products, S[2 u + n] for keys 8 n .. of tile u; pv(u, w): the weights'
+    // products with tile u's values into O; bias(j, i): term i of this lane's
+    // row j, keys t0 + 2 tig + {0, 1, 8, 9, 16, ...}; clean(u): values that
+    // are not numbers to 0, and which of the lane's four keys had any.
+    auto step = [&](auto units, int t0, const float *ksc, const float *ev, auto kf, auto pv, auto bias, auto clean) {
+        constexpr int U = decltype(units)::value;
+        float x[RL][4 * U], f2[RL][U], lv[U], S[2 * U][4];
 #pragma unroll
-        for (int n = 0; n < 2; n++) {
-            S[n][0] = S[n][1] = S[n][2] = S[n][3] = 0.0f;
+        for (int n = 0; n < 2 * U; n++) S[n][0] = S[n][1] = S[n][2] = S[n][3] = 0.0f;
+        kf(S);
 #pragma unroll
-            for (int ks = 0; ks < F::KS; ks++) {
-                uint32_t b0, b1;
-                kf(n, ks, b0, b1);
-                mma16(S[n], qa[ks], b0, b1);
-            }
-        }
-        const bool biased = E && pa - (t0 + kK8Tile - 1) < E;
-        const bool masked = t0 + kK8Tile - 1 > pa || (window && t0 <= pb - window) || ks_ < 0.0f;
-        float p[RL][4];
-        bool grow = false;
-        uint32_t seen = 0;                             // bit 4j + i: row j sees key i
+        for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int j = 0; j < RL; j++) {
-            const float f = ks_ * qmul[j];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int n = i >> 1, e = i & 1;
-                const float x = F::kTwo ? S[n][e] + S[n][e + 2] : S[n][e + 2 * j];
-                p[j][i] = x * f;
-            }
-            if (biased) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) p[j][i] += bias(j, i) * tau[j];
-            }
-            if (masked) {
+            for (int j = 0; j < RL; j++) {
+                f2[j][u] = ksc[u] * qmul[j];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const int at = t0 + 2 * tig + (i & 1) + 8 * (i >> 1);
-                    if (at > pos[j] || (window && at <= pos[j] - window) || ks_ < 0.0f) p[j][i] = -INFINITY;
+                    const float *y = S[2 * u + (i >> 1)];
+                    x[j][4 * u + i] = F::kTwo ? y[i & 1] + y[(i & 1) + 2] : y[(i & 1) + 2 * j];
                 }
             }
-            const float top = fmaxf(fmaxf(p[j][0], p[j][1]), fmaxf(p[j][2], p[j][3]));
-#pragma unroll
-            for (int i = 0; i < 4; i++) seen |= p[j][i] == -INFINITY ? 0u : 1u << (4 * j + i);
-            grow |= top > m[j] + kSlack || (top > m[j] && m[j] < -1e30f);
-        }
-        float vmul = kPOne;
-        if (vs > vref) {                               // the whole warp: scales are powers of two
-            const float f = vref / vs;
+        const float top_ev = U == 2 ? fmaxf(ev[0], ev[U - 1]) : ev[0];
+        if (top_ev > eref) {                           // the whole warp
+            const float f = exp2_fast(eref - top_ev);
 #pragma unroll
             for (int nt = 0; nt < F::NT; nt++) O[nt][0] *= f, O[nt][1] *= f, O[nt][2] *= f, O[nt][3] *= f;
-            vref = vs;
-        } else {
-            vmul = kPOne * (vs / vref);
+            eref = top_ev;
         }
-        if (__any_sync(0xffffffffu, grow)) {
+        const bool biased = E && pa - (t0 + U * kK8Tile - 1) < E;
+        bool masked = t0 + U * kK8Tile - 1 > pa || (window && t0 <= pb - window) || ksc[0] < 0.0f || ksc[U - 1] < 0.0f;
+        if (biased || masked) {
+            uint32_t seen = 0;                         // bit 4 U j + i: row j sees key i
+#pragma unroll
+            for (int j = 0; j < RL; j++)
+#pragma unroll
+                for (int i = 0; i < 4 * U; i++) {
+                    const int at = t0 + 2 * tig + (i & 1) + 8 * (i >> 1);
+                    float y = x[j][i] * f2[j][i / 4];
+                    if (biased) {
+                        // a score of the type's lowest stays a number in base 2
+                        const float b = bias(j, i) * tau[j] * kLog2e;
+                        y = y + b;
+                        if (y < kLowest && bias(j, i) * tau[j] > -INFINITY) y = kLowest;
+                    }
+                    if (at > pos[j] || (window && at <= pos[j] - window) || ksc[i / 4] < 0.0f) y = -INFINITY;
+                    x[j][i] = y;
+                    seen |= y == -INFINITY ? 0u : 1u << (4 * U * j + i);
+                }
+#pragma unroll
+            for (int j = 0; j < RL; j++)
+#pragma unroll
+                for (int u = 0; u < U; u++) f2[j][u] = 1.0f;
+            // A value that is not a number must not reach a row that does not
+            // see its key (0 * NaN): in a step with hidden keys such values
+            // count as 0, and a row that does see one gets a sum of NaN.
+            if (__any_sync(0xffffffffu, seen != (1u << (4 * U * RL)) - 1u)) {
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    uint32_t nan = clean(u);
+                    nan |= __shfl_xor_sync(0xffffffffu, nan, 4);
+                    nan |= __shfl_xor_sync(0xffffffffu, nan, 8);
+                    nan |= __shfl_xor_sync(0xffffffffu, nan, 16);
+#pragma unroll
+                    for (int j = 0; j < RL; j++)
+                        if (seen >> (4 * U * j + 4 * u) & nan) l[j] = __int_as_float(0x7fffffff);
+                }
+            }
+        }
+        float p[RL][4 * U], top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; u++) lv[u] = ev[u] - eref + kPBits;
+#pragma unroll
+        for (int j = 0; j < RL; j++)
+#pragma unroll
+            for (int i = 0; i < 4 * U; i++) {
+                p[j][i] = fmaf(x[j][i], f2[j][i / 4], -m2[j]) + lv[i / 4];   // exact where both are the lowest
+                top = fmaxf(top, p[j][i]);
+            }
+        if (__any_sync(0xffffffffu, top > kPMax)) {
             float f[RL];
 #pragma unroll
             for (int j = 0; j < RL; j++) {
-                float top = fmaxf(fmaxf(p[j][0], p[j][1]), fmaxf(p[j][2], p[j][3]));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                top = fmaxf(top, m[j]);
-                f[j] = top == -INFINITY ? 1.0f : exp2_fast((m[j] - top) * kLog2e);
-                m[j] = top;
+                float t = kLowest;
+#pragma unroll
+                for (int i = 0; i < 4 * U; i++) t = fmaxf(t, x[j][i] * f2[j][i / 4]);
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+                t = fmaxf(t, m2[j]);
+                f[j] = exp2_fast(m2[j] - t);
+                m2[j] = t;
                 l[j] *= f[j];
+#pragma unroll
+                for (int i = 0; i < 4 * U; i++) p[j][i] = fmaf(x[j][i], f2[j][i / 4], -t) + lv[i / 4];
             }
 #pragma unroll
             for (int nt = 0; nt < F::NT; nt++) {
@@ -263,105 +383,31 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
                 O[nt][2] *= f[RL - 1], O[nt][3] *= f[RL - 1];
             }
         }
-        uint32_t w[4];
 #pragma unroll
-        for (int j = 0; j < RL; j++) {
-            const float mj = m[j] == -INFINITY ? 0.0f : m[j];
+        for (int u = 0; u < U; u++) {
+            uint32_t w[4];
+            const float il = exp2_fast(-lv[u]);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                p[j][i] = exp2_fast((p[j][i] - mj) * kLog2e);
-                l[j] += p[j][i];
-                p[j][i] *= vmul;
-            }
+            for (int j = 0; j < RL; j++) {
+                float *q = &p[j][4 * u];
 #pragma unroll
-            for (int n = 0; n < 2; n++) {
-                const __half2 hi = __floats2half2_rn(p[j][2 * n], p[j][2 * n + 1]);
-                w[2 * n + j] = *reinterpret_cast<const uint32_t *>(&hi);
-                if constexpr (F::kTwo) {
-                    const float2 b = __half22float2(hi);
-                    w[2 * n + 1] = pack_half2(p[j][2 * n] - b.x, p[j][2 * n + 1] - b.y);
-                }
-            }
-        }
-        if (biased || masked) {
-            // A value that is not a number must not reach a row that does not
-            // see its key (0 * NaN): in a tile with hidden keys such values
-            // count as 0, and a row that does see one gets a sum of NaN.
-            if (__any_sync(0xffffffffu, seen != (1u << (4 * RL)) - 1u)) {
-                uint32_t nan = clean();                // bit i: key i, among this lane's dims
-                nan |= __shfl_xor_sync(0xffffffffu, nan, 4);
-                nan |= __shfl_xor_sync(0xffffffffu, nan, 8);
-                nan |= __shfl_xor_sync(0xffffffffu, nan, 16);
+                for (int i = 0; i < 4; i++) q[i] = exp2_fast(q[i]);
+                l[j] = fmaf((q[0] + q[1]) + (q[2] + q[3]), il, l[j]);
 #pragma unroll
-                for (int j = 0; j < RL; j++)
-                    if (seen >> (4 * j) & nan) l[j] = __int_as_float(0x7fffffff);
-            }
-        }
-#pragma unroll
-        for (int nt = 0; nt < F::NT; nt++) {
-            uint32_t b0, b1;
-            vf(nt, b0, b1);
-            mma16(O[nt], w, b0, b1);
-        }
-    };
-
-    // ---- coded tiles: this warp's share of [c0, min(c1, tail0)), through its ring ----
-    const int ce = min(c1, tail0);
-    const int n_tiles = ce > c0 ? (ce - c0 + kK8Tile - 1) / kK8Tile : 0;
-    const int mine = n_tiles > warp ? (n_tiles - warp + kK8Warps - 1) / kK8Warps : 0;
-    uint8_t *ring = smem + warp * F::kStages * F::kStageB;
-    const uint32_t ring_u = smem_u32(ring);
-    int id_l = -1;
-    float ks_l = -1.0f, vs_l = 1.0f;
-    auto issue = [&](int i) {
-        if (i < mine) {
-            if ((i & 31) == 0) {                       // this lane's block of the next 32 tiles
-                const int k = i + lane;
-                if (k < mine) {
-                    id_l = kv8_block(P.c, P.b, s, (c0 + (warp + kK8Warps * k) * kK8Tile) / B, P.err);
-                    ks_l = id_l >= 0 ? P.c.k_scale[(int64_t)id_l * Hkv + hk] : -1.0f;
-                    vs_l = id_l >= 0 ? P.c.v_scale[(int64_t)id_l * Hkv + hk] : 1.0f;
-                }
-            }
-            const int id = __shfl_sync(0xffffffffu, id_l, i & 31);
-            const float ks = __shfl_sync(0xffffffffu, ks_l, i & 31), vs = __shfl_sync(0xffffffffu, vs_l, i & 31);
-            const int t0 = c0 + (warp + kK8Warps * i) * kK8Tile;
-            const uint32_t st = ring_u + (i % F::kStages) * F::kStageB;
-            const int64_t row0 = ((int64_t)max(id, 0) * Hkv + hk) * B + (t0 & (B - 1));
-            const uint8_t *K = (const uint8_t *)P.c.k + row0 * Dh, *V = (const uint8_t *)P.c.v + row0 * Dh;
-#pragma unroll
-            for (int n = 0; n < 2; n++)
-#pragma unroll
-                for (int j = 0; j < F::KW; j++) {
-                    const int d = 64 * j + 16 * tig;
-                    cp_async_or_zero<16>(st + (n * F::KW + j) * 512 + lane * 16, d < Dh ? K + (gid + 8 * n) * Dh + d : K,
-                                         d < Dh && id >= 0);
-                }
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int r = 2 * tig + (k & 1) + 8 * (k >> 1), d = gid * F::VB;
-                cp_async_or_zero<F::VB>(st + F::kKeyB + k * (32 * F::VB) + lane * F::VB, d < Dh ? V + r * Dh + d : V,
-                                        d < Dh && id >= 0);
-            }
-            if (E && pa - (t0 + kK8Tile - 1) < E) {
-#pragma unroll
-                for (int j = 0; j < RL; j++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const int far = pos[j] - (t0 + 2 * tig + (k & 1) + 8 * (k >> 1));
-                        const bool on = far >= 0 && far < E;
-                        const float *src = P.a.rel_logits + ((int64_t)n_row[j] * H + h_row[j]) * E;
-                        cp_async_or_zero<4>(st + F::kKeyB + F::kValB + (4 * j + k) * 128 + lane * 4, on ? src + far : src, on);
+                for (int n = 0; n < 2; n++) {
+                    const __half2 hi = __floats2half2_rn(q[2 * n], q[2 * n + 1]);
+                    w[2 * n + j] = *reinterpret_cast<const uint32_t *>(&hi);
+                    if constexpr (F::kTwo) {
+                        const float2 b = __half22float2(hi);
+                        w[2 * n + 1] = pack_half2(q[2 * n] - b.x, q[2 * n + 1] - b.y);
                     }
+                }
             }
-            if (lane == 0)
-                *reinterpret_cast<float2 *>(ring + (i % F::kStages) * F::kStageB + F::kKeyB + F::kValB + F::kBiasB) =
-                    make_float2(ks, vs);
+            pv(u, w);
         }
-        cp_async_commit();
     };
-#pragma unroll
-    for (int i = 0; i < F::kStages - 1; i++) issue(i);
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
 
     // ---- the tail's fp16 tiles, one a warp, while the ring fills ----
     {
@@ -370,155 +416,176 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
             const int64_t at = (((int64_t)sq.slot * Hkv + hk) * B + (t0 - tail0)) * Dh;
             const __half *K = (const __half *)P.c.k_tail + at, *V = (const __half *)P.c.v_tail + at;
             const int held = sq.held + sq.add - t0;    // keys of the tile that exist
-            uint4 v[4][F::VB / 8];
+            const float one = 1.0f, zero = 0.0f;
+            uint32_t v[4][F::VB / 2];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 const int r = 2 * tig + (k & 1) + 8 * (k >> 1), d = gid * F::VB;
 #pragma unroll
                 for (int j = 0; j < F::VB / 8; j++)
-                    v[k][j] = r < held && d + 8 * j < Dh ? *reinterpret_cast<const uint4 *>(V + r * Dh + d + 8 * j)
-                                                         : make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4 *>(&v[k][4 * j]) =
+                        r < held && d + 8 * j < Dh ? *reinterpret_cast<const uint4 *>(V + r * Dh + d + 8 * j)
+                                                   : make_uint4(0, 0, 0, 0);
             }
-            tile(
-                t0, 1.0f, 1.0f,
-                [&](int n, int ks, uint32_t &b0, uint32_t &b1) {
-                    const int d = 64 * (ks / 4) + 16 * tig + 4 * (ks % 4), r = gid + 8 * n;
-                    const uint2 x = r < held && d < Dh ? *reinterpret_cast<const uint2 *>(K + r * Dh + d) : make_uint2(0, 0);
-                    b0 = x.x;
-                    b1 = x.y;
+            step(
+                One(), t0, &one, &zero,
+                [&](float (&S)[2][4]) {
+#pragma unroll
+                    for (int ks = 0; ks < F::KS; ks++) {
+                        const int d = 64 * (ks / 4) + 16 * tig + 4 * (ks % 4);
+#pragma unroll
+                        for (int n = 0; n < 2; n++) {
+                            const int r = gid + 8 * n;
+                            const uint2 x = r < held && d < Dh ? *reinterpret_cast<const uint2 *>(K + r * Dh + d)
+                                                               : make_uint2(0, 0);
+                            mma16(S[n], qa[ks], x.x, x.y);
+                        }
+                    }
                 },
-                [&](int nt, uint32_t &b0, uint32_t &b1) {
-                    const uint32_t *a = reinterpret_cast<const uint32_t *>(v[0]), *b = reinterpret_cast<const uint32_t *>(v[1]);
-                    const uint32_t *c = reinterpret_cast<const uint32_t *>(v[2]), *d = reinterpret_cast<const uint32_t *>(v[3]);
-                    const uint32_t sel = nt & 1 ? 0x7632 : 0x5410;
-                    b0 = __byte_perm(a[nt / 2], b[nt / 2], sel);
-                    b1 = __byte_perm(c[nt / 2], d[nt / 2], sel);
+                [&](int, const uint32_t (&w)[4]) {
+#pragma unroll
+                    for (int nt = 0; nt < F::NT; nt++) {
+                        const uint32_t sel = nt & 1 ? 0x7632 : 0x5410;
+                        mma16(O[nt], w, __byte_perm(v[0][nt / 2], v[1][nt / 2], sel),
+                              __byte_perm(v[2][nt / 2], v[3][nt / 2], sel));
+                    }
                 },
                 [&](int j, int i) {
                     const int far = pos[j] - (t0 + 2 * tig + (i & 1) + 8 * (i >> 1));
-                    return far >= 0 && far < E ? P.a.rel_logits[((int64_t)n_row[j] * H + h_row[j]) * E + far] : 0.0f;
+                    return far >= 0 && far < E ? rel[j][far] : 0.0f;
                 },
-                [&]() {
+                [&](int) {
                     uint32_t nan = 0;
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        uint32_t *x = reinterpret_cast<uint32_t *>(v[k]);
+                    for (int k = 0; k < 4; k++)
 #pragma unroll
                         for (int e = 0; e < F::VB / 2; e++) {
-                            const uint32_t at = __vcmpgtu2(x[e] & 0x7fff7fffu, 0x7c007c00u);
-                            x[e] &= ~at;
+                            const uint32_t at = __vcmpgtu2(v[k][e] & 0x7fff7fffu, 0x7c007c00u);
+                            v[k][e] &= ~at;
                             nan |= at ? 1u << k : 0u;
                         }
-                    }
                     return nan;
                 });
         }
     }
 
+    const uint32_t two16 = P.two16;                    // 2^16, unknown to the compiler (see e4m3_hi)
     for (int i = 0; i < mine; i++) {
         __syncwarp();                                  // every lane is done with the stage that is filled next
-        issue(i + F::kStages - 1);
-        cp_async_wait<F::kStages - 1>();
+        issue(i + kK8Stages - 1);
+        cp_async_wait<kK8Stages - 1>();
         __syncwarp();
-        const uint8_t *st = ring + (i % F::kStages) * F::kStageB;
-        const float2 sc = *reinterpret_cast<const float2 *>(st + F::kKeyB + F::kValB + F::kBiasB);
-        uint32_t kw[2][F::KW * 4], vw[4][F::VB / 4];
+        uint8_t *st = ring + (i & (kK8Stages - 1)) * stage_b;
+        const float4 sc = *reinterpret_cast<const float4 *>(st + 2 * F::kTileB);
+        const float ksc[2] = {sc.x, sc.z}, ev[2] = {sc.y, sc.w};
+        step(
+            Two(), c0 + (warp + kK8Warps * i) * kK8Unit, ksc, ev,
+            [&](float (&S)[4][4]) {
 #pragma unroll
-        for (int n = 0; n < 2; n++)
+                for (int j = 0; j < F::KW; j++) {
+                    uint4 k[4];
 #pragma unroll
-            for (int j = 0; j < F::KW; j++)
-                *reinterpret_cast<uint4 *>(&kw[n][4 * j]) = *reinterpret_cast<const uint4 *>(st + (n * F::KW + j) * 512 + lane * 16);
+                    for (int n = 0; n < 4; n++)
+                        k[n] = *reinterpret_cast<const uint4 *>(st + (n >> 1) * F::kTileB + ((n & 1) * F::KW + j) * 512 + lane * 16);
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const uint8_t *src = st + F::kKeyB + k * (32 * F::VB) + lane * F::VB;
-            if constexpr (F::VB == 16) *reinterpret_cast<uint4 *>(vw[k]) = *reinterpret_cast<const uint4 *>(src);
-            else *reinterpret_cast<uint2 *>(vw[k]) = *reinterpret_cast<const uint2 *>(src);
-        }
-        tile(
-            c0 + (warp + kK8Warps * i) * kK8Tile, sc.x, sc.y,
-            [&](int n, int ks, uint32_t &b0, uint32_t &b1) {
-                b0 = e4m3x2_to_half2(kw[n][ks]);
-                b1 = e4m3x2_to_half2_hi(kw[n][ks]);
+                    for (int e = 0; e < 4; e++)
+#pragma unroll
+                        for (int n = 0; n < 4; n++) {  // four independent chains
+                            const uint32_t kw = e == 0 ? k[n].x : e == 1 ? k[n].y : e == 2 ? k[n].z : k[n].w;
+                            mma16(S[n], qa[4 * j + e], e4m3_lo(kw), e4m3_hi(kw, two16));
+                        }
+                }
             },
-            [&](int nt, uint32_t &b0, uint32_t &b1) {
-                const uint32_t sel = nt & 2 ? 0x7362 : 0x5140;
-                const uint32_t x = __byte_perm(vw[0][nt / 4], vw[1][nt / 4], sel);
-                const uint32_t y = __byte_perm(vw[2][nt / 4], vw[3][nt / 4], sel);
-                b0 = nt & 1 ? e4m3x2_to_half2_hi(x) : e4m3x2_to_half2(x);
-                b1 = nt & 1 ? e4m3x2_to_half2_hi(y) : e4m3x2_to_half2(y);
+            [&](int u, const uint32_t (&w)[4]) {
+                uint32_t v[4][F::VB / 4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint8_t *src = st + u * F::kTileB + F::kKeyB + k * (32 * F::VB) + lane * F::VB;
+                    if constexpr (F::VB == 16) *reinterpret_cast<uint4 *>(v[k]) = *reinterpret_cast<const uint4 *>(src);
+                    else *reinterpret_cast<uint2 *>(v[k]) = *reinterpret_cast<const uint2 *>(src);
+                }
+#pragma unroll
+                for (int nt = 0; nt < F::NT; nt += 2) {
+                    const uint32_t sel = nt & 2 ? 0x7362 : 0x5140;
+                    const uint32_t x = __byte_perm(v[0][nt / 4], v[1][nt / 4], sel);
+                    const uint32_t y = __byte_perm(v[2][nt / 4], v[3][nt / 4], sel);
+                    mma16(O[nt], w, e4m3_lo(x), e4m3_lo(y));
+                    mma16(O[nt + 1], w, e4m3_hi(x, two16), e4m3_hi(y, two16));
+                }
             },
             [&](int j, int k) {
-                return *reinterpret_cast<const float *>(st + F::kKeyB + F::kValB + (4 * j + k) * 128 + lane * 4);
+                if (j >= P.bias_rows) return 0.0f;     // rows that do not exist have no room in the ring
+                return *reinterpret_cast<const float *>(st + 2 * F::kTileB + F::kHeadB + (8 * j + k) * 128 + lane * 4);
             },
-            [&]() {
+            [&](int u) {                               // the lane's own copies, in its ring
                 uint32_t nan = 0;
 #pragma unroll
-                for (int k = 0; k < 4; k++)
+                for (int k = 0; k < 4; k++) {
+                    uint32_t *v = reinterpret_cast<uint32_t *>(st + u * F::kTileB + F::kKeyB + k * (32 * F::VB) + lane * F::VB);
 #pragma unroll
                     for (int e = 0; e < F::VB / 4; e++) {
-                        const uint32_t at = __vcmpeq4(vw[k][e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                        vw[k][e] &= ~at;
+                        const uint32_t at = __vcmpeq4(v[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                        if (at) v[e] &= ~at;
                         nan |= at ? 1u << k : 0u;
                     }
+                }
                 return nan;
             });
     }
     cp_async_wait<0>();
     __syncthreads();
 
-    // ---- merge the warps: rows of m, l and the output, in warp order ----
-    float *mg = reinterpret_cast<float *>(smem) + warp * RT * (DP + 2);
+    // ---- merge the warps, in warp order. A row's output lies in the order
+    // of the lanes' columns: entry 8 nt + c is dim c * VB + nt ----
+    float *mg = reinterpret_cast<float *>(smem) + warp * RT * F::kPitch;
 #pragma unroll
     for (int j = 0; j < RL; j++) {
         l[j] += __shfl_xor_sync(0xffffffffu, l[j], 1);
         l[j] += __shfl_xor_sync(0xffffffffu, l[j], 2);
-        float *o = mg + (gid + 8 * j) * (DP + 2);
-        if (tig == 0) o[0] = m[j], o[1] = l[j];
-        const float f = vref / kPOne;
+        float *o = mg + (gid + 8 * j) * F::kPitch;
+        if (tig == 0) *reinterpret_cast<float2 *>(o + DP) = make_float2(m2[j], l[j]);
+        const float f = exp2_fast(eref - kPBits);
 #pragma unroll
         for (int nt = 0; nt < F::NT; nt++)
-#pragma unroll
-            for (int e = 0; e < 2; e++)
-                o[2 + (2 * tig + e) * F::VB + nt] = f * (F::kTwo ? O[nt][e] + O[nt][e + 2] : O[nt][e + 2 * j]);
+            *reinterpret_cast<float2 *>(o + 8 * nt + 2 * tig) =
+                make_float2(f * (F::kTwo ? O[nt][0] + O[nt][2] : O[nt][2 * j]),
+                            f * (F::kTwo ? O[nt][1] + O[nt][3] : O[nt][1 + 2 * j]));
     }
     __syncthreads();
     const int live = min(rows, RT), group = blockIdx.z * gridDim.y + blockIdx.y;
-    const int64_t stride = (int64_t)RT * (Dh + 2);
-    float *part = P.part + (int64_t)group * P.splits * stride;
-    auto put = [&](int r, int d, float o, float sum) {
-        const int R = rt * RT + r, t = R / G;
-        ((T *)P.a.out)[((int64_t)(sq.n0 + t) * H + hk * G + (R - t * G)) * Dh + d] = (T)(sum == 0.0f ? 0.0f : o / sum);
-    };
-    for (int i = tid; i < live * Dh; i += kK8Threads) {
-        const int r = i / Dh, d = i - r * Dh;
-        const float *o = reinterpret_cast<const float *>(smem) + r * (DP + 2);
-        float M = -INFINITY, L = 0.0f, A = 0.0f;
+    float *part = P.part + ((int64_t)group * P.splits + split) * RT * (DP + 2);
+    for (int i = tid; i < live * DP; i += kK8Threads) {
+        const int r = i / DP, c = i - r * DP, d = (c & 7) * F::VB + (c >> 3);
+        const float *o = reinterpret_cast<const float *>(smem) + r * F::kPitch;
+        float M = kLowest, L = 0.0f, A = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kK8Warps; w++) M = fmaxf(M, o[w * RT * (DP + 2)]);
+        for (int w = 0; w < kK8Warps; w++) M = fmaxf(M, o[w * RT * F::kPitch + DP]);
 #pragma unroll
         for (int w = 0; w < kK8Warps; w++) {
-            const float *ow = o + w * RT * (DP + 2);
-            const float f = ow[0] == -INFINITY ? 0.0f : exp2_fast((ow[0] - M) * kLog2e);
-            L += f * ow[1];
-            A += f * ow[2 + d];
+            const float *ow = o + w * RT * F::kPitch;
+            const float f = exp2_fast(ow[DP] - M);
+            L += f * ow[DP + 1];
+            A += f * ow[c];
         }
         if (n_act == 1) {
-            put(r, d, A, L);
+            const int R = rt * RT + r, t = R / G;
+            if (d < Dh)
+                ((T *)P.a.out)[((int64_t)(sq.n0 + t) * H + hk * G + (R - t * G)) * Dh + d] = (T)(L == 0.0f ? 0.0f : A / L);
         } else {
-            float *to = part + split * stride + r * (Dh + 2);
-            if (d == 0) to[0] = M, to[1] = L;
-            to[2 + d] = A;
+            float *to = part + r * (DP + 2);
+            if (c == 0) *reinterpret_cast<float2 *>(to) = make_float2(M, L);
+            to[2 + c] = A;
         }
     }
 }
 
 // Merges the chunks of a row, in chunk order within each of the W warps that
 // share the row, then across the warps. One CTA does kK8Warps / W rows.
-template <typename T, int W>
+template <typename T, int DP, int W>
 __global__ void __launch_bounds__(kK8Threads) k_kv8_merge(const K8Params P) {
-    constexpr int RT = sizeof(T) == 4 ? 8 : 16;
-    __shared__ float s_part[W > 1 ? kK8Warps : 1][kKv8MaxDh + 2];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, d = 4 * lane;
+    constexpr int RT = K8Cfg<T, DP>::RT;
+    __shared__ float s_part[W > 1 ? kK8Warps : 1][DP + 2];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c = 4 * lane;
     const int Dh = P.c.head_dim, H = P.a.n_heads, G = P.G, s = blockIdx.y;
     griddep_wait();
     griddep_launch();
@@ -532,9 +599,9 @@ __global__ void __launch_bounds__(kK8Threads) k_kv8_merge(const K8Params P) {
     const int n_act = (sq.held + tb + 1 - lo + P.chunk - 1) / P.chunk;
     if (n_act <= 1) return;
     const int group = s * P.c.n_kv_heads * P.row_tiles + hk * P.row_tiles + rt;
-    const int64_t stride = (int64_t)RT * (Dh + 2);
-    const float *part = P.part + (int64_t)group * P.splits * stride + (int64_t)r * (Dh + 2);
-    float M = -INFINITY, L = 0.0f, A[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int64_t stride = (int64_t)RT * (DP + 2);
+    const float *part = P.part + (int64_t)group * P.splits * stride + r * (DP + 2);
+    float M = kLowest, L = 0.0f, A[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int k = lane; k < n_act; k += 32) M = fmaxf(M, part[k * stride]);
     M = warp_max(M);
     const int per = (n_act + W - 1) / W, k0 = (warp % W) * per, k1 = min(n_act, k0 + per);
@@ -545,33 +612,34 @@ __global__ void __launch_bounds__(kK8Threads) k_kv8_merge(const K8Params P) {
         for (int i = 0; i < kAhead; i++) {
             const float2 *p = reinterpret_cast<const float2 *>(part + min(k + i, k1 - 1) * stride);
             ml[i] = p[0];
-            x[i][0] = d < Dh ? p[1 + d / 2] : make_float2(0.0f, 0.0f);
-            x[i][1] = d < Dh ? p[2 + d / 2] : make_float2(0.0f, 0.0f);
+            x[i][0] = c < DP ? p[1 + c / 2] : make_float2(0.0f, 0.0f);
+            x[i][1] = c < DP ? p[2 + c / 2] : make_float2(0.0f, 0.0f);
         }
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
-            if (k + i >= k1) break;
-            const float f = ml[i].x == -INFINITY ? 0.0f : exp2_fast((ml[i].x - M) * kLog2e);
+            const float f = k + i < k1 ? exp2_fast(ml[i].x - M) : 0.0f;
             L += f * ml[i].y;
             A[0] += f * x[i][0].x, A[1] += f * x[i][0].y, A[2] += f * x[i][1].x, A[3] += f * x[i][1].y;
         }
     }
     if constexpr (W > 1) {
-        if (d < Dh)
-            for (int e = 0; e < 4; e++) s_part[warp][2 + d + e] = A[e];
+        if (c < DP)
+            for (int e = 0; e < 4; e++) s_part[warp][2 + c + e] = A[e];
         if (lane == 0) s_part[warp][0] = L;
         __syncthreads();
         if (warp) return;
 #pragma unroll
         for (int w = 1; w < W; w++) {
             L += s_part[w][0];
-            if (d < Dh)
-                for (int e = 0; e < 4; e++) A[e] += s_part[w][2 + d + e];
+            if (c < DP)
+                for (int e = 0; e < 4; e++) A[e] += s_part[w][2 + c + e];
         }
     }
-    if (d < Dh) {
-        T *o = (T *)P.a.out + ((int64_t)(sq.n0 + t) * H + h) * Dh + d;
-        for (int e = 0; e < 4; e++) o[e] = (T)(L == 0.0f ? 0.0f : A[e] / L);
+    T *o = (T *)P.a.out + ((int64_t)(sq.n0 + t) * H + h) * Dh;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const int d = ((c + e) & 7) * (DP / 8) + ((c + e) >> 3);
+        if (c < DP && d < Dh) o[d] = (T)(L == 0.0f ? 0.0f : A[e] / L);
     }
 }
 
@@ -584,7 +652,7 @@ struct K8Plan {
 // chunk at most kMaxChunk positions; longer work runs in several waves of
 // kMaxChunk, so that ragged sequences even out.
 static K8Plan k8_plan(const SepiaKv8Cache &c, const SepiaKv8Step &b, const SepiaKv8Attn &a) {
-    constexpr int64_t kUnit = kK8Tile * kK8Warps, kMaxChunk = 1024;
+    constexpr int64_t kUnit = kK8Unit * kK8Warps, kMaxChunk = 1024;
     K8Plan p;
     const int rt = a.x_f16 ? 16 : 8;
     p.G = a.n_heads / c.n_kv_heads;
@@ -595,23 +663,32 @@ static K8Plan k8_plan(const SepiaKv8Cache &c, const SepiaKv8Step &b, const Sepia
     const int64_t one = (groups * span + slots - 1) / slots;
     p.chunk = (int)(std::min(kMaxChunk, std::max<int64_t>(one, 1)) + kUnit - 1) / kUnit * kUnit;
     p.splits = (int)std::max<int64_t>(1, (span + p.chunk - 1) / p.chunk);
-    p.bytes = p.splits > 1 ? (size_t)groups * p.splits * rt * (c.head_dim + 2) * 4 : 0;
+    p.bytes = p.splits > 1 ? (size_t)groups * p.splits * rt * ((c.head_dim <= 64 ? 64 : 128) + 2) * 4 : 0;
     return p;
 }
 
-template <typename T, int DP>
-static int k8_launch(const K8Params &P, cudaStream_t st) {
-    constexpr int smem = K8Cfg<T, DP>::kSmem;
-    if (!ensure_smem((const void *)k_kv8_attn<T, DP>, smem)) return 0;
+template <typename T, int DP, bool FULL>
+static int k8_launch(K8Params &P, cudaStream_t st) {
+    using F = K8Cfg<T, DP>;
+    const int64_t rows = (int64_t)P.b.max_new * P.a.n_heads;
+    P.bias_rows = P.a.rel_extent == 0 ? 0 : (int64_t)P.b.max_new * P.G <= 8 ? 1 : F::RL;
+    const int smem = std::max(kK8Warps * kK8Stages * F::stage(P.bias_rows), F::kMergeB);
+    if (!ensure_smem((const void *)k_kv8_attn<T, DP, FULL>, smem)) return 0;
     const dim3 grid((unsigned)P.splits, (unsigned)(P.c.n_kv_heads * P.row_tiles), (unsigned)P.b.n_seqs);
-    if (!check(launch_pdl(k_kv8_attn<T, DP>, grid, dim3(kK8Threads), smem, st, P), "kv8_attn launch")) return 0;
+    if (!check(launch_pdl(k_kv8_attn<T, DP, FULL>, grid, dim3(kK8Threads), smem, st, P), "kv8_attn launch")) return 0;
     if (P.splits == 1) return 1;
     // one warp per row while a row has few chunks, four beyond
-    const int64_t rows = (int64_t)P.b.max_new * P.a.n_heads;
     const dim3 g1((unsigned)((rows + kK8Warps - 1) / kK8Warps), (unsigned)P.b.n_seqs), g4((unsigned)rows, (unsigned)P.b.n_seqs);
-    const cudaError_t e = P.splits <= 8 ? launch_pdl(k_kv8_merge<T, 1>, g1, dim3(kK8Threads), 0, st, P)
-                                        : launch_pdl(k_kv8_merge<T, 4>, g4, dim3(kK8Threads), 0, st, P);
+    const cudaError_t e = P.splits <= 8 ? launch_pdl(k_kv8_merge<T, DP, 1>, g1, dim3(kK8Threads), 0, st, P)
+                                        : launch_pdl(k_kv8_merge<T, DP, 4>, g4, dim3(kK8Threads), 0, st, P);
     return check(e, "kv8_attn merge launch");
+}
+
+template <typename T>
+static int k8_launch_dim(K8Params &P, cudaStream_t st) {
+    const int Dh = P.c.head_dim;
+    if (Dh <= 64) return Dh == 64 ? k8_launch<T, 64, true>(P, st) : k8_launch<T, 64, false>(P, st);
+    return Dh == 128 ? k8_launch<T, 128, true>(P, st) : k8_launch<T, 128, false>(P, st);
 }
 
 static int k8_check(const SepiaKv8Cache *c, const SepiaKv8Step *b, const SepiaKv8Attn *a) {
@@ -655,9 +732,9 @@ extern "C" int sepia_cuda_kv8_attn(const SepiaKv8Cache *c, const SepiaKv8Step *b
     P.row_tiles = p.row_tiles;
     P.splits = p.splits;
     P.chunk = p.chunk;
+    P.two16 = 65536u;
     P.part = (float *)ws;
     P.err = dev_info().err;
     cudaStream_t st = as_stream(stream);
-    if (c->head_dim <= 64) return a->x_f16 ? k8_launch<__half, 64>(P, st) : k8_launch<float, 64>(P, st);
-    return a->x_f16 ? k8_launch<__half, 128>(P, st) : k8_launch<float, 128>(P, st);
+    return a->x_f16 ? k8_launch_dim<__half>(P, st) : k8_launch_dim<float>(P, st);
 }
