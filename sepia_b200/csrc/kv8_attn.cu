@@ -11,16 +11,16 @@
 //             second kernel merges the chunks of a long context, many rows
 //             at once (as the last step of the last CTA of each KV head the
 //             same sum took 65 us of 95 at 1 x 32768: 8 CTAs at work).
-//   Operands  mma m16n8k16 in fp16 with fp32 sums. e4m3 codes are fp16
-//             numbers exactly; block scales multiply the score and the
-//             weight. fp32 rows: q and the weight are split into two fp16
-//             terms (22 bits) that sit in the two halves of the 16-row
-//             operand, 8 rows a tile; fp16 rows: 16 rows a tile.
-//   Layout    the dims of a k step and of an output column are permuted so
-//             that a lane's codes are 16 consecutive bytes of a key row (K)
-//             or of four key rows (V). Each lane copies just the bytes that it
-//             will use into a ring of its own in shared memory (cp.async), so
-//             no lane waits for another and nothing conflicts.
+//   Operands  mma m16n8k16 in fp16 with fp32 sums, the codes as the 16-row
+//             operand (scores: 16 keys x 8 rows; output: 16 dims x 8 rows),
+//             so that 8 rows fill it. e4m3 codes are fp16 numbers exactly;
+//             block scales multiply the score and the weight. fp32 rows: q and
+//             the weight are two fp16 terms (22 bits), summed in one result.
+//   Layout    the dims of a k step and of an output tile are permuted so that
+//             a lane's codes are 16 consecutive bytes of a key row (K) or of
+//             four key rows (V). Each lane copies just the bytes that it will
+//             use into a ring of its own in shared memory (cp.async), so no
+//             lane waits for another and nothing conflicts.
 #include "kv8.cuh"
 #include "runtime.h"
 
@@ -49,25 +49,27 @@ struct K8Params {
     SepiaKv8Step b;
     SepiaKv8Attn a;
     int G, row_tiles, splits, chunk;     // chunk: positions per split, a multiple of kK8Unit * kK8Warps
-    int bias_rows;                       // rows of a lane that have a band: 0, 1 or 2
-    uint32_t two16;
+    int q_vec;                           // four elements of q in one load
     float *part;                         // [n_seqs, n_kv_heads * row_tiles, splits, rows of a tile, Dh + 2]
     int *err;
 };
 
-// The low two e4m3 codes of a word as fp16: one conversion. The high two
-// are first moved down by a multiplication (high half of x * 2^16), which
-// runs beside the conversions: shifts, permutes and conversions share one
-// pipe of half the rate (measured 64 lanes a clock and SM each).
+// The low and the high two e4m3 codes of a word as fp16
 __device__ __forceinline__ uint32_t e4m3_lo(uint32_t x) {
     uint32_t r;
     asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(r) : "r"(x));
     return r;
 }
-__device__ __forceinline__ uint32_t e4m3_hi(uint32_t x, uint32_t two16) {
-    uint32_t y;
-    asm("mul.hi.u32 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(two16));
-    return e4m3_lo(y);
+__device__ __forceinline__ uint32_t e4m3_hi(uint32_t x) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(x));
+    return r;
+}
+// The warp's 8 x 8 matrix of halves (row: lane / 4, columns 2 (lane % 4) and the next) transposed
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
 }
 __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -98,28 +100,29 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-template <typename T, int DP>
+// NB groups of 8 rows share a warp's converted codes.
+template <typename T, int DP, int NB>
 struct K8Cfg {
-    static constexpr bool kTwo = sizeof(T) == 4;      // two fp16 terms per row
-    static constexpr int RT = kTwo ? 8 : 16;          // rows of a tile
-    static constexpr int RL = kTwo ? 1 : 2;           // rows of a lane
+    static constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;   // fp16 terms of a row
+    static constexpr int RT = 8 * NB;                 // rows of a tile
     static constexpr int KW = DP / 64;                // 16-byte pieces of a key row per lane
     static constexpr int VB = DP / 8;                 // bytes of a value row per lane
-    static constexpr int NT = DP / 8, KS = DP / 16;   // output columns of 8, k steps of 16
+    static constexpr int MT = DP / 16, KS = DP / 16;  // output tiles of 16 dims, k steps of 16
     static constexpr int kKeyB = 2 * KW * 512, kValB = 4 * VB * 32, kTileB = kKeyB + kValB;
     static constexpr int kHeadB = 16;                 // a step's scales
-    static constexpr int kPitch = DP + 8;             // of a merge row: 8 rows of 8-byte stores meet no bank twice
-    static constexpr int kMergeB = kK8Warps * RT * kPitch * 4;
-    // bytes of a ring stage with the bias of `rows` rows a lane
-    static constexpr int stage(int rows) { return 2 * kTileB + kHeadB + rows * 8 * 128; }
+    static constexpr int kPitch = DP + 4;             // of a merge row: the lanes' stores meet no bank twice
+    static constexpr int kMergeB = kK8Warps * RT * (kPitch + 2) * 4;
+    static constexpr int kQB = NB > 1 ? NB * KS * 32 * 8 * TERMS : 0;   // q operands, kept in registers with one group
+    // bytes of a ring stage, with room for a band where there is one
+    static constexpr int stage(bool band) { return 2 * kTileB + kHeadB + (band ? NB * 8 * 128 : 0); }
 };
 
 // FULL: head_dim is DP (64 or 128), every offset a constant; otherwise the
 // dims past head_dim are read as zeros.
-template <typename T, int DP, bool FULL>
+template <typename T, int DP, int NB, bool FULL>
 __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8Params P) {
-    using F = K8Cfg<T, DP>;
-    constexpr int RL = F::RL, RT = F::RT;
+    using F = K8Cfg<T, DP, NB>;
+    constexpr int RT = F::RT, TERMS = F::TERMS;
     extern __shared__ __align__(16) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
     const int split = blockIdx.x, s = blockIdx.z;
@@ -152,40 +155,128 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
     const int ce = min(c1, tail0);
     const int n_units = ce > c0 ? (ce - c0 + kK8Unit - 1) / kK8Unit : 0;
     const int mine = n_units > warp ? (n_units - warp + kK8Warps - 1) / kK8Warps : 0;
-    const int stage_b = F::stage(P.bias_rows);
-    uint8_t *ring = smem + warp * kK8Stages * stage_b;
+    const int stage_b = F::stage(E > 0);
+    uint8_t *ring = smem + F::kQB + warp * kK8Stages * stage_b;
     const uint32_t ring_u = smem_u32(ring);
-    int pos[RL];
-    const float *rel[RL];
+    // the pool's block of this lane's tile: tile lane % 2 of step i + lane / 2
+    int id_l = -1;
+    auto look_up = [&](int i) {
+        const int at = c0 + (warp + kK8Warps * (i + (lane >> 1))) * kK8Unit + (lane & 1) * kK8Tile;
+        id_l = at < ce ? kv8_block(P.c, P.b, s, at / B, P.err) : -1;
+    };
+    look_up(0);
+
+    // ---- q: lane (gid, tig) holds 16 dims of row gid of each group ----
+    auto row_of = [&](int r, int &t, int &h) {         // of a row of the tile, or of the last one that exists
+        const int R = min(rt * RT + r, sq.add * G - 1);
+        t = R / G;
+        h = hk * G + R - t * G;
+    };
+    constexpr int NQ = NB == 1 ? F::KS : 1;
+    uint32_t qb[NQ][2 * TERMS];                        // [k step][term][half]
+    float qx[NB];                                      // row gid's factor on its products
 #pragma unroll
-    for (int j = 0; j < RL; j++) {
-        const int R = min(rt * RT + gid + 8 * j, sq.add * G - 1), t = R / G;
-        pos[j] = sq.held + t;
-        rel[j] = P.a.rel_logits + ((int64_t)(sq.n0 + t) * H + hk * G + R - t * G) * E;
-    }
-    int id_l = 0;
-    float ks_l = -1.0f, ev_l = 0.0f;
-    auto issue = [&](int i) {
-        if (i < mine) {
-            if ((i & 15) == 0) {                       // lane: tile lane % 2 of step i + lane / 2
-                const int at = c0 + (warp + kK8Warps * (i + (lane >> 1))) * kK8Unit + (lane & 1) * kK8Tile;
-                ks_l = -1.0f;                          // a tile that is not there: all its keys hidden
-                ev_l = 0.0f;
-                id_l = 0;
-                if (at < ce) {
-                    const int id = kv8_block(P.c, P.b, s, at / B, P.err);
-                    if (id >= 0) {
-                        id_l = id;
-                        ks_l = P.c.k_scale[(int64_t)id * Hkv + hk];
-                        ev_l = (float)((int)(__float_as_uint(P.c.v_scale[(int64_t)id * Hkv + hk]) >> 23 & 255) - 127);
-                    }
+    for (int g = 0; g < NB; g++) {
+        if (NB > 1 && (g & (kK8Warps - 1)) != warp) continue;   // one warp writes a group's operands
+        int t, h;
+        row_of(8 * g + gid, t, h);
+        const bool on = 8 * g + gid < rows;
+        const T *q = (const T *)P.a.q + (int64_t)(sq.n0 + t) * P.a.q_stride + (int64_t)h * Dh;
+        float x[F::KS][4], amax = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < F::KS; ks++) {
+            const int d = 64 * (ks / 4) + 16 * tig + 4 * (ks % 4);
+            T v[4] = {};
+            if (on && d < Dh) {
+                if (P.q_vec) {
+                    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(q + d);
+                    else *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(q + d);
+                } else {
+                    for (int e = 0; e < 4; e++) v[e] = q[d + e];
                 }
             }
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x[ks][e] = (float)v[e];
+                amax = fmaxf(amax, fabsf(x[ks][e]));
+            }
+        }
+        float f = 1.0f;
+        if constexpr (TERMS == 2) {
+            // the row times a power of two that puts its largest in [2^13, 2^14): both terms stay normal fp16
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            const int ex = amax > 0.0f ? max((int)(__float_as_uint(amax) >> 23) - 127, -100) : 13;
+            f = __uint_as_float((uint32_t)(127 + 13 - ex) << 23);
+            qx[g] = __uint_as_float((uint32_t)(127 - 13 + ex) << 23);
+        } else {
+            qx[g] = 1.0f;
+        }
+#pragma unroll
+        for (int ks = 0; ks < F::KS; ks++) {
+            uint32_t w[2 * TERMS];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const float u = x[ks][2 * e] * f, v = x[ks][2 * e + 1] * f;
+                const __half2 hi = __floats2half2_rn(u, v);
+                w[e] = *reinterpret_cast<const uint32_t *>(&hi);
+                if constexpr (TERMS == 2) {
+                    const float2 b = __half22float2(hi);
+                    w[2 + e] = pack_half2(u - b.x, v - b.y);
+                }
+            }
+            if constexpr (NB == 1) {
+#pragma unroll
+                for (int e = 0; e < 2 * TERMS; e++) qb[ks][e] = w[e];
+            } else {
+                uint32_t *to = reinterpret_cast<uint32_t *>(smem) + ((g * F::KS + ks) * 32 + lane) * (2 * TERMS);
+#pragma unroll
+                for (int e = 0; e < 2 * TERMS; e++) to[e] = w[e];
+            }
+        }
+    }
+    auto q_op = [&](int g, int ks, uint32_t (&w)[2 * TERMS]) {
+        if constexpr (NB == 1) {
+#pragma unroll
+            for (int e = 0; e < 2 * TERMS; e++) w[e] = qb[ks][e];
+        } else {
+            const uint32_t *from = reinterpret_cast<const uint32_t *>(smem) + ((g * F::KS + ks) * 32 + lane) * (2 * TERMS);
+            if constexpr (TERMS == 2) *reinterpret_cast<uint4 *>(w) = *reinterpret_cast<const uint4 *>(from);
+            else *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(from);
+        }
+    };
+
+    // this lane's rows of each group as columns of a product: 2 tig and 2 tig + 1
+    int pos[NB][2];
+    const float *rel[NB][2];
+#pragma unroll
+    for (int g = 0; g < NB; g++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            int t, h;
+            row_of(8 * g + 2 * tig + e, t, h);
+            pos[g][e] = sq.held + t;
+            rel[g][e] = P.a.rel_logits + ((int64_t)(sq.n0 + t) * H + h) * E;
+        }
+
+    auto issue = [&](int i) {
+        if (i < mine) {
+            if (i && (i & 15) == 0) look_up(i);
             const int t0 = c0 + (warp + kK8Warps * i) * kK8Unit;
             const uint32_t st = ring_u + (i & (kK8Stages - 1)) * stage_b;
+            if ((lane >> 1) == (i & 15)) {             // the tile's scales; a tile that is not there: hidden
+                const uint32_t to = st + 2 * F::kTileB + 8 * (lane & 1);
+                if (id_l >= 0) {
+                    cp_async_bytes<4>(to, P.c.k_scale + (int64_t)id_l * Hkv + hk);
+                    cp_async_bytes<4>(to + 4, P.c.v_scale + (int64_t)id_l * Hkv + hk);
+                } else {
+                    *reinterpret_cast<float2 *>(ring + (i & (kK8Stages - 1)) * stage_b + 2 * F::kTileB + 8 * (lane & 1)) =
+                        make_float2(-1.0f, 1.0f);
+                }
+            }
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const int id = __shfl_sync(0xffffffffu, id_l, (2 * i + u) & 31);
+                const int id = max(0, __shfl_sync(0xffffffffu, id_l, (2 * i + u) & 31));
                 const int64_t row0 = ((int64_t)id * Hkv + hk) * B + ((t0 + u * kK8Tile) & (B - 1));
                 const uint8_t *K = (const uint8_t *)P.c.k + row0 * Dh + gid * Dh + 16 * tig;
                 const uint8_t *V = (const uint8_t *)P.c.v + row0 * Dh + 2 * tig * Dh + gid * F::VB;
@@ -195,215 +286,203 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
 #pragma unroll
                     for (int j = 0; j < F::KW; j++) {
                         if constexpr (FULL) cp_async_bytes<16>(at + (n * F::KW + j) * 512, K + n * 8 * Dh + j * 64);
-                        else cp_async_or_zero<16>(at + (n * F::KW + j) * 512, K + n * 8 * Dh + j * 64, 64 * j + 16 * tig < Dh);
+                        else cp_async_or_zero<16>(at + (n * F::KW + j) * 512, 64 * j + 16 * tig < Dh ? K + n * 8 * Dh + j * 64 : K,
+                                                  64 * j + 16 * tig < Dh);
                     }
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     const uint32_t to = st + u * F::kTileB + F::kKeyB + k * (32 * F::VB) + lane * F::VB;
                     const uint8_t *src = V + ((k & 1) + 8 * (k >> 1)) * Dh;
                     if constexpr (FULL) cp_async_bytes<F::VB>(to, src);
-                    else cp_async_or_zero<F::VB>(to, src, gid * F::VB < Dh);
+                    else cp_async_or_zero<F::VB>(to, gid * F::VB < Dh ? src : (const uint8_t *)P.c.v, gid * F::VB < Dh);
                 }
             }
             if (E && pa - (t0 + kK8Unit - 1) < E) {
 #pragma unroll
-                for (int j = 0; j < RL; j++) {
-                    if (j >= P.bias_rows) break;
+                for (int g = 0; g < NB; g++)
 #pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        const int far = pos[j] - (t0 + 2 * tig + (k & 1) + 8 * (k >> 1));
+                    for (int k = 0; k < 8; k++) {      // key gid + 8 (k / 2), row 2 tig + k % 2
+                        const int far = pos[g][k & 1] - (t0 + gid + 8 * (k >> 1));
                         const bool on = far >= 0 && far < E;
-                        cp_async_or_zero<4>(st + 2 * F::kTileB + F::kHeadB + (8 * j + k) * 128 + lane * 4,
-                                            rel[j] + (on ? far : 0), on);
+                        cp_async_or_zero<4>(st + 2 * F::kTileB + F::kHeadB + (8 * g + k) * 128 + lane * 4,
+                                            rel[g][k & 1] + (on ? far : 0), on);
                     }
-                }
             }
-            if ((lane >> 1) == (i & 15))
-                *reinterpret_cast<float2 *>(ring + (i & (kK8Stages - 1)) * stage_b + 2 * F::kTileB + 8 * (lane & 1)) =
-                    make_float2(ks_l, ev_l);
         }
         cp_async_commit();
     };
 #pragma unroll
     for (int i = 0; i < kK8Stages - 1; i++) issue(i);
 
-    // ---- this lane's rows and their q operand ----
-    float qmul[RL], tau[RL];
-    uint32_t qa[F::KS][4];
+    float qmul[NB][2], tau[NB][2];                     // of the lane's rows as columns
 #pragma unroll
-    for (int j = 0; j < RL; j++) {
-        const int r = gid + 8 * j, R = min(rt * RT + r, sq.add * G - 1), t = R / G;
-        const bool on = r < rows;
-        tau[j] = P.a.tau && on ? P.a.tau[sq.n0 + t] : 1.0f;
-        const T *q = (const T *)P.a.q + (int64_t)(sq.n0 + t) * P.a.q_stride + (int64_t)(hk * G + R - t * G) * Dh;
-        float x[F::KS][4], amax = 0.0f;
+    for (int g = 0; g < NB; g++)
 #pragma unroll
-        for (int ks = 0; ks < F::KS; ks++) {
-            const int d = 64 * (ks / 4) + 16 * tig + 4 * (ks % 4);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                x[ks][e] = on && d < Dh ? (float)q[d + e] : 0.0f;
-                amax = fmaxf(amax, fabsf(x[ks][e]));
-            }
+        for (int e = 0; e < 2; e++) {
+            int t, h;
+            row_of(8 * g + 2 * tig + e, t, h);
+            tau[g][e] = P.a.tau ? P.a.tau[sq.n0 + t] : 1.0f;
+            qmul[g][e] = P.a.scale * kLog2e;
+            if constexpr (NB == 1) qmul[g][e] *= __shfl_sync(0xffffffffu, qx[g], 8 * tig + 4 * e);
         }
-        if constexpr (F::kTwo) {
-            // the row times a power of two that puts its largest in [2^13, 2^14): both terms stay normal fp16
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            const int ex = amax > 0.0f ? max((int)(__float_as_uint(amax) >> 23) - 127, -100) : 13;
-            const float f = __uint_as_float((uint32_t)(127 + 13 - ex) << 23);
-            qmul[j] = P.a.scale * kLog2e * __uint_as_float((uint32_t)(127 - 13 + ex) << 23);
+    if constexpr (NB > 1) {
+        __shared__ float s_qx[RT];
 #pragma unroll
-            for (int ks = 0; ks < F::KS; ks++) {
+        for (int g = 0; g < NB; g++)
+            if ((g & (kK8Warps - 1)) == warp && tig == 0) s_qx[8 * g + gid] = qx[g];
+        __syncthreads();
 #pragma unroll
-                for (int e = 0; e < 4; e += 2) {
-                    const float u = x[ks][e] * f, v = x[ks][e + 1] * f;
-                    const __half2 hi = __floats2half2_rn(u, v);
-                    const float2 b = __half22float2(hi);
-                    qa[ks][e] = *reinterpret_cast<const uint32_t *>(&hi);        // a0 / a2: rows 0-7
-                    qa[ks][e + 1] = pack_half2(u - b.x, v - b.y);                // a1 / a3: rows 8-15
-                }
-            }
-        } else {
-            qmul[j] = P.a.scale * kLog2e;
+        for (int g = 0; g < NB; g++)
 #pragma unroll
-            for (int ks = 0; ks < F::KS; ks++) {
-                qa[ks][j] = pack_half2(x[ks][0], x[ks][1]);
-                qa[ks][2 + j] = pack_half2(x[ks][2], x[ks][3]);
-            }
-        }
+            for (int e = 0; e < 2; e++) qmul[g][e] *= s_qx[8 * g + 2 * tig + e];
     }
 
-    // Running maximum in base 2 (a lag is allowed), sum, and output / 2^eref.
-    float O[F::NT][4], m2[RL], l[RL], eref = -1000.0f;
+    // Running maximum in base 2 (a lag is allowed), sum, and output / 2^eref;
+    // O[g][mt]: dims gid * VB + 2 mt (+ 1 in entries 2, 3), rows 2 tig (+ 1 in entries 1, 3).
+    float O[NB][F::MT][4], m2[NB][2], l[NB][2], eref = -1000.0f;
 #pragma unroll
-    for (int nt = 0; nt < F::NT; nt++) O[nt][0] = O[nt][1] = O[nt][2] = O[nt][3] = 0.0f;
+    for (int g = 0; g < NB; g++) {
+        m2[g][0] = m2[g][1] = kLowest;
+        l[g][0] = l[g][1] = 0.0f;
 #pragma unroll
-    for (int j = 0; j < RL; j++) m2[j] = kLowest, l[j] = 0.0f;
+        for (int mt = 0; mt < F::MT; mt++) O[g][mt][0] = O[g][mt][1] = O[g][mt][2] = O[g][mt][3] = 0.0f;
+    }
 
     // One step of U 16-key tiles from position t0; ksc, ev: each tile's key
-    // scale (negative: hidden) and the exponent of its value scale.
-    // kf(S): the key products, S[2 u + n] for keys 8 n .. of tile u; pv(u, w): the weights'
-    // products with tile u's values into O; bias(j, i): term i of this lane's
-    // row j, keys t0 + 2 tig + {0, 1, 8, 9, 16, ...}; clean(u): values that
-    // are not numbers to 0, and which of the lane's four keys had any.
-    auto step = [&](auto units, int t0, const float *ksc, const float *ev, auto kf, auto pv, auto bias, auto clean) {
+    // scale (negative: hidden) and the exponent of its value scale. kf(S):
+    // the key products; entry i of S[g][u]: key gid + 8 (i / 2), row
+    // 2 tig + i % 2. vf(u, mt, a): the values' operand. bias(g, i): the band's
+    // entry for key gid + 8 (i / 2), row i % 2. clean(u): values that are not
+    // numbers to 0, and which of the tile's 16 keys had any among this lane's.
+    auto step = [&](auto units, int t0, const float *ksc, const float *ev, auto kf, auto vf, auto bias, auto clean) {
         constexpr int U = decltype(units)::value;
-        float x[RL][4 * U], f2[RL][U], lv[U], S[2 * U][4];
-#pragma unroll
-        for (int n = 0; n < 2 * U; n++) S[n][0] = S[n][1] = S[n][2] = S[n][3] = 0.0f;
+        float S[NB][U][4], f2[U], lv[U];
         kf(S);
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int j = 0; j < RL; j++) {
-                f2[j][u] = ksc[u] * qmul[j];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float *y = S[2 * u + (i >> 1)];
-                    x[j][4 * u + i] = F::kTwo ? y[i & 1] + y[(i & 1) + 2] : y[(i & 1) + 2 * j];
-                }
-            }
         const float top_ev = U == 2 ? fmaxf(ev[0], ev[U - 1]) : ev[0];
         if (top_ev > eref) {                           // the whole warp
             const float f = exp2_fast(eref - top_ev);
 #pragma unroll
-            for (int nt = 0; nt < F::NT; nt++) O[nt][0] *= f, O[nt][1] *= f, O[nt][2] *= f, O[nt][3] *= f;
+            for (int g = 0; g < NB; g++)
+#pragma unroll
+                for (int mt = 0; mt < F::MT; mt++)
+                    O[g][mt][0] *= f, O[g][mt][1] *= f, O[g][mt][2] *= f, O[g][mt][3] *= f;
             eref = top_ev;
         }
+#pragma unroll
+        for (int u = 0; u < U; u++) f2[u] = ksc[u], lv[u] = ev[u] - eref + kPBits;
         const bool biased = E && pa - (t0 + U * kK8Tile - 1) < E;
-        bool masked = t0 + U * kK8Tile - 1 > pa || (window && t0 <= pb - window) || ksc[0] < 0.0f || ksc[U - 1] < 0.0f;
+        const bool masked =
+            t0 + U * kK8Tile - 1 > pa || (window && t0 <= pb - window) || ksc[0] < 0.0f || ksc[U - 1] < 0.0f;
+        // Scores, in base 2: S * (f2 * qmul). In a step with a band or hidden keys
+        // they are worked out here and the factor left is 1.
+        bool scored = false;
         if (biased || masked) {
-            uint32_t seen = 0;                         // bit 4 U j + i: row j sees key i
+            scored = true;
+            bool all = true;
+            uint32_t nan[U];
 #pragma unroll
-            for (int j = 0; j < RL; j++)
+            for (int g = 0; g < NB; g++)
 #pragma unroll
-                for (int i = 0; i < 4 * U; i++) {
-                    const int at = t0 + 2 * tig + (i & 1) + 8 * (i >> 1);
-                    float y = x[j][i] * f2[j][i / 4];
-                    if (biased) {
-                        // a score of the type's lowest stays a number in base 2
-                        const float b = bias(j, i) * tau[j] * kLog2e;
-                        y = y + b;
-                        if (y < kLowest && bias(j, i) * tau[j] > -INFINITY) y = kLowest;
+                for (int u = 0; u < U; u++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int at = t0 + u * kK8Tile + gid + 8 * (i >> 1), e = i & 1;
+                        float y = S[g][u][i] * (f2[u] * qmul[g][e]);
+                        if (biased) {
+                            // a score of the type's lowest stays a number in base 2
+                            const float b = bias(g, 4 * u + i) * tau[g][e];
+                            y = fmaf(b, kLog2e, y);
+                            if (y < kLowest && b > -INFINITY) y = kLowest;
+                        }
+                        if (at > pos[g][e] || (window && at <= pos[g][e] - window) || ksc[u] < 0.0f) y = -INFINITY;
+                        S[g][u][i] = y;
+                        all = all && y != -INFINITY;
                     }
-                    if (at > pos[j] || (window && at <= pos[j] - window) || ksc[i / 4] < 0.0f) y = -INFINITY;
-                    x[j][i] = y;
-                    seen |= y == -INFINITY ? 0u : 1u << (4 * U * j + i);
-                }
-#pragma unroll
-            for (int j = 0; j < RL; j++)
-#pragma unroll
-                for (int u = 0; u < U; u++) f2[j][u] = 1.0f;
             // A value that is not a number must not reach a row that does not
             // see its key (0 * NaN): in a step with hidden keys such values
             // count as 0, and a row that does see one gets a sum of NaN.
-            if (__any_sync(0xffffffffu, seen != (1u << (4 * U * RL)) - 1u)) {
+            if (__any_sync(0xffffffffu, !all)) {
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    uint32_t nan = clean(u);
-                    nan |= __shfl_xor_sync(0xffffffffu, nan, 4);
-                    nan |= __shfl_xor_sync(0xffffffffu, nan, 8);
-                    nan |= __shfl_xor_sync(0xffffffffu, nan, 16);
+                    nan[u] = __reduce_or_sync(0xffffffffu, clean(u));
 #pragma unroll
-                    for (int j = 0; j < RL; j++)
-                        if (seen >> (4 * U * j + 4 * u) & nan) l[j] = __int_as_float(0x7fffffff);
+                    for (int g = 0; g < NB; g++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (S[g][u][i] != -INFINITY && (nan[u] >> (gid + 8 * (i >> 1)) & 1))
+                                l[g][i & 1] = __int_as_float(0x7fffffff);
                 }
             }
         }
-        float p[RL][4 * U], top = -INFINITY;
+        float p[NB][U][4], top = -INFINITY;
+        auto weigh = [&]() {
 #pragma unroll
-        for (int u = 0; u < U; u++) lv[u] = ev[u] - eref + kPBits;
+            for (int g = 0; g < NB; g++)
 #pragma unroll
-        for (int j = 0; j < RL; j++)
+                for (int u = 0; u < U; u++)
 #pragma unroll
-            for (int i = 0; i < 4 * U; i++) {
-                p[j][i] = fmaf(x[j][i], f2[j][i / 4], -m2[j]) + lv[i / 4];   // exact where both are the lowest
-                top = fmaxf(top, p[j][i]);
-            }
+                    for (int i = 0; i < 4; i++)        // exact where score and maximum are both the lowest
+                        p[g][u][i] = fmaf(S[g][u][i], scored ? 1.0f : f2[u] * qmul[g][i & 1], -m2[g][i & 1]) + lv[u];
+        };
+        weigh();
+#pragma unroll
+        for (int g = 0; g < NB; g++)
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) top = fmaxf(top, p[g][u][i]);
         if (__any_sync(0xffffffffu, top > kPMax)) {
-            float f[RL];
 #pragma unroll
-            for (int j = 0; j < RL; j++) {
-                float t = kLowest;
+            for (int g = 0; g < NB; g++)
 #pragma unroll
-                for (int i = 0; i < 4 * U; i++) t = fmaxf(t, x[j][i] * f2[j][i / 4]);
-                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
-                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-                t = fmaxf(t, m2[j]);
-                f[j] = exp2_fast(m2[j] - t);
-                m2[j] = t;
-                l[j] *= f[j];
+                for (int e = 0; e < 2; e++) {
+                    float t = m2[g][e];
 #pragma unroll
-                for (int i = 0; i < 4 * U; i++) p[j][i] = fmaf(x[j][i], f2[j][i / 4], -t) + lv[i / 4];
-            }
+                    for (int u = 0; u < U; u++) {
+                        const float f = scored ? 1.0f : f2[u] * qmul[g][e];
+                        t = fmaxf(t, fmaxf(S[g][u][e] * f, S[g][u][2 + e] * f));
+                    }
+                    t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+                    t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+                    t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+                    const float f = exp2_fast(m2[g][e] - t);
+                    m2[g][e] = t;
+                    l[g][e] *= f;
 #pragma unroll
-            for (int nt = 0; nt < F::NT; nt++) {
-                O[nt][0] *= f[0], O[nt][1] *= f[0];
-                O[nt][2] *= f[RL - 1], O[nt][3] *= f[RL - 1];
-            }
+                    for (int mt = 0; mt < F::MT; mt++) O[g][mt][e] *= f, O[g][mt][2 + e] *= f;
+                }
+            weigh();
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            uint32_t w[4];
             const float il = exp2_fast(-lv[u]);
+            uint32_t w[NB][TERMS][2];
 #pragma unroll
-            for (int j = 0; j < RL; j++) {
-                float *q = &p[j][4 * u];
+            for (int g = 0; g < NB; g++) {
+                float *q = p[g][u];
 #pragma unroll
                 for (int i = 0; i < 4; i++) q[i] = exp2_fast(q[i]);
-                l[j] = fmaf((q[0] + q[1]) + (q[2] + q[3]), il, l[j]);
 #pragma unroll
-                for (int n = 0; n < 2; n++) {
+                for (int e = 0; e < 2; e++) l[g][e] = fmaf(q[e] + q[2 + e], il, l[g][e]);
+#pragma unroll
+                for (int n = 0; n < 2; n++) {          // keys gid + 8 n: 8 x 8 weights, turned
                     const __half2 hi = __floats2half2_rn(q[2 * n], q[2 * n + 1]);
-                    w[2 * n + j] = *reinterpret_cast<const uint32_t *>(&hi);
-                    if constexpr (F::kTwo) {
+                    w[g][0][n] = transpose8(*reinterpret_cast<const uint32_t *>(&hi));
+                    if constexpr (TERMS == 2) {
                         const float2 b = __half22float2(hi);
-                        w[2 * n + 1] = pack_half2(q[2 * n] - b.x, q[2 * n + 1] - b.y);
+                        w[g][TERMS - 1][n] = transpose8(pack_half2(q[2 * n] - b.x, q[2 * n + 1] - b.y));
                     }
                 }
             }
-            pv(u, w);
+#pragma unroll
+            for (int mt = 0; mt < F::MT; mt++) {
+                uint32_t a[4];
+                vf(u, mt, a);
+#pragma unroll
+                for (int g = 0; g < NB; g++)
+#pragma unroll
+                    for (int k = 0; k < TERMS; k++) mma16(O[g][mt], a, w[g][k][0], w[g][k][1]);
+            }
         }
     };
     using One = std::integral_constant<int, 1>;
@@ -429,30 +508,36 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
             }
             step(
                 One(), t0, &one, &zero,
-                [&](float (&S)[2][4]) {
+                [&](float (&S)[NB][1][4]) {
+#pragma unroll
+                    for (int g = 0; g < NB; g++) S[g][0][0] = S[g][0][1] = S[g][0][2] = S[g][0][3] = 0.0f;
 #pragma unroll
                     for (int ks = 0; ks < F::KS; ks++) {
                         const int d = 64 * (ks / 4) + 16 * tig + 4 * (ks % 4);
+                        uint2 x[2];
 #pragma unroll
-                        for (int n = 0; n < 2; n++) {
-                            const int r = gid + 8 * n;
-                            const uint2 x = r < held && d < Dh ? *reinterpret_cast<const uint2 *>(K + r * Dh + d)
+                        for (int n = 0; n < 2; n++)
+                            x[n] = gid + 8 * n < held && d < Dh ? *reinterpret_cast<const uint2 *>(K + (gid + 8 * n) * Dh + d)
                                                                : make_uint2(0, 0);
-                            mma16(S[n], qa[ks], x.x, x.y);
+                        const uint32_t a[4] = {x[0].x, x[1].x, x[0].y, x[1].y};
+#pragma unroll
+                        for (int g = 0; g < NB; g++) {
+                            uint32_t w[2 * TERMS];
+                            q_op(g, ks, w);
+#pragma unroll
+                            for (int k = 0; k < TERMS; k++) mma16(S[g][0], a, w[2 * k], w[2 * k + 1]);
                         }
                     }
                 },
-                [&](int, const uint32_t (&w)[4]) {
-#pragma unroll
-                    for (int nt = 0; nt < F::NT; nt++) {
-                        const uint32_t sel = nt & 1 ? 0x7632 : 0x5410;
-                        mma16(O[nt], w, __byte_perm(v[0][nt / 2], v[1][nt / 2], sel),
-                              __byte_perm(v[2][nt / 2], v[3][nt / 2], sel));
-                    }
+                [&](int, int mt, uint32_t (&a)[4]) {   // dims 2 mt and 2 mt + 1 of the lane's: the two halves of word mt
+                    a[0] = __byte_perm(v[0][mt], v[1][mt], 0x5410);
+                    a[1] = __byte_perm(v[0][mt], v[1][mt], 0x7632);
+                    a[2] = __byte_perm(v[2][mt], v[3][mt], 0x5410);
+                    a[3] = __byte_perm(v[2][mt], v[3][mt], 0x7632);
                 },
-                [&](int j, int i) {
-                    const int far = pos[j] - (t0 + 2 * tig + (i & 1) + 8 * (i >> 1));
-                    return far >= 0 && far < E ? rel[j][far] : 0.0f;
+                [&](int g, int i) {
+                    const int far = pos[g][i & 1] - (t0 + gid + 8 * (i >> 1));
+                    return far >= 0 && far < E ? rel[g][i & 1][far] : 0.0f;
                 },
                 [&](int) {
                     uint32_t nan = 0;
@@ -462,14 +547,13 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
                         for (int e = 0; e < F::VB / 2; e++) {
                             const uint32_t at = __vcmpgtu2(v[k][e] & 0x7fff7fffu, 0x7c007c00u);
                             v[k][e] &= ~at;
-                            nan |= at ? 1u << k : 0u;
+                            nan |= at ? 1u << (2 * tig + (k & 1) + 8 * (k >> 1)) : 0u;
                         }
                     return nan;
                 });
         }
     }
 
-    const uint32_t two16 = P.two16;                    // 2^16, unknown to the compiler (see e4m3_hi)
     for (int i = 0; i < mine; i++) {
         __syncwarp();                                  // every lane is done with the stage that is filled next
         issue(i + kK8Stages - 1);
@@ -477,56 +561,87 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
         __syncwarp();
         uint8_t *st = ring + (i & (kK8Stages - 1)) * stage_b;
         const float4 sc = *reinterpret_cast<const float4 *>(st + 2 * F::kTileB);
-        const float ksc[2] = {sc.x, sc.z}, ev[2] = {sc.y, sc.w};
+        const float ksc[2] = {sc.x, sc.z};
+        const float ev[2] = {(float)((int)(__float_as_uint(sc.y) >> 23 & 255) - 127),
+                             (float)((int)(__float_as_uint(sc.w) >> 23 & 255) - 127)};
+        uint32_t v[4][F::VB / 4];
         step(
             Two(), c0 + (warp + kK8Warps * i) * kK8Unit, ksc, ev,
-            [&](float (&S)[4][4]) {
+            [&](float (&S)[NB][2][4]) {
+                float R[NB][2][4];                     // the second term's sums, or the odd k steps'
+#pragma unroll
+                for (int g = 0; g < NB; g++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) S[g][u][e] = R[g][u][e] = 0.0f;
 #pragma unroll
                 for (int j = 0; j < F::KW; j++) {
-                    uint4 k[4];
+                    uint4 k[2][2];
 #pragma unroll
-                    for (int n = 0; n < 4; n++)
-                        k[n] = *reinterpret_cast<const uint4 *>(st + (n >> 1) * F::kTileB + ((n & 1) * F::KW + j) * 512 + lane * 16);
+                    for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
+                        for (int n = 0; n < 2; n++)
+                            k[u][n] = *reinterpret_cast<const uint4 *>(st + u * F::kTileB + (n * F::KW + j) * 512 + lane * 16);
 #pragma unroll
-                        for (int n = 0; n < 4; n++) {  // four independent chains
-                            const uint32_t kw = e == 0 ? k[n].x : e == 1 ? k[n].y : e == 2 ? k[n].z : k[n].w;
-                            mma16(S[n], qa[4 * j + e], e4m3_lo(kw), e4m3_hi(kw, two16));
+                    for (int e = 0; e < 4; e++) {
+                        uint32_t a[2][4];
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const uint32_t x = e == 0 ? k[u][0].x : e == 1 ? k[u][0].y : e == 2 ? k[u][0].z : k[u][0].w;
+                            const uint32_t y = e == 0 ? k[u][1].x : e == 1 ? k[u][1].y : e == 2 ? k[u][1].z : k[u][1].w;
+                            a[u][0] = e4m3_lo(x), a[u][1] = e4m3_lo(y), a[u][2] = e4m3_hi(x), a[u][3] = e4m3_hi(y);
                         }
-                }
-            },
-            [&](int u, const uint32_t (&w)[4]) {
-                uint32_t v[4][F::VB / 4];
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const uint8_t *src = st + u * F::kTileB + F::kKeyB + k * (32 * F::VB) + lane * F::VB;
-                    if constexpr (F::VB == 16) *reinterpret_cast<uint4 *>(v[k]) = *reinterpret_cast<const uint4 *>(src);
-                    else *reinterpret_cast<uint2 *>(v[k]) = *reinterpret_cast<const uint2 *>(src);
+                        for (int g = 0; g < NB; g++) {
+                            uint32_t w[2 * TERMS];
+                            q_op(g, 4 * j + e, w);
+#pragma unroll
+                            for (int u = 0; u < 2; u++) {
+                                if constexpr (TERMS == 2) {
+                                    mma16(S[g][u], a[u], w[0], w[1]);
+                                    mma16(R[g][u], a[u], w[2 * TERMS - 2], w[2 * TERMS - 1]);
+                                } else {
+                                    mma16(e & 1 ? R[g][u] : S[g][u], a[u], w[0], w[1]);
+                                }
+                            }
+                        }
+                    }
                 }
 #pragma unroll
-                for (int nt = 0; nt < F::NT; nt += 2) {
-                    const uint32_t sel = nt & 2 ? 0x7362 : 0x5140;
-                    const uint32_t x = __byte_perm(v[0][nt / 4], v[1][nt / 4], sel);
-                    const uint32_t y = __byte_perm(v[2][nt / 4], v[3][nt / 4], sel);
-                    mma16(O[nt], w, e4m3_lo(x), e4m3_lo(y));
-                    mma16(O[nt + 1], w, e4m3_hi(x, two16), e4m3_hi(y, two16));
-                }
+                for (int g = 0; g < NB; g++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) S[g][u][e] += R[g][u][e];
             },
-            [&](int j, int k) {
-                if (j >= P.bias_rows) return 0.0f;     // rows that do not exist have no room in the ring
-                return *reinterpret_cast<const float *>(st + 2 * F::kTileB + F::kHeadB + (8 * j + k) * 128 + lane * 4);
+            [&](int u, int mt, uint32_t (&a)[4]) {
+                if (mt == 0) {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint8_t *src = st + u * F::kTileB + F::kKeyB + k * (32 * F::VB) + lane * F::VB;
+                        if constexpr (F::VB == 16) *reinterpret_cast<uint4 *>(v[k]) = *reinterpret_cast<const uint4 *>(src);
+                        else *reinterpret_cast<uint2 *>(v[k]) = *reinterpret_cast<const uint2 *>(src);
+                    }
+                }
+                const uint32_t sel = mt & 1 ? 0x7362 : 0x5140;   // two dims of two keys
+                const uint32_t x = __byte_perm(v[0][mt / 2], v[1][mt / 2], sel);
+                const uint32_t y = __byte_perm(v[2][mt / 2], v[3][mt / 2], sel);
+                a[0] = e4m3_lo(x), a[1] = e4m3_hi(x), a[2] = e4m3_lo(y), a[3] = e4m3_hi(y);
+            },
+            [&](int g, int k) {
+                return *reinterpret_cast<const float *>(st + 2 * F::kTileB + F::kHeadB + (8 * g + k) * 128 + lane * 4);
             },
             [&](int u) {                               // the lane's own copies, in its ring
                 uint32_t nan = 0;
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    uint32_t *v = reinterpret_cast<uint32_t *>(st + u * F::kTileB + F::kKeyB + k * (32 * F::VB) + lane * F::VB);
+                    uint32_t *x = reinterpret_cast<uint32_t *>(st + u * F::kTileB + F::kKeyB + k * (32 * F::VB) + lane * F::VB);
 #pragma unroll
                     for (int e = 0; e < F::VB / 4; e++) {
-                        const uint32_t at = __vcmpeq4(v[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                        if (at) v[e] &= ~at;
-                        nan |= at ? 1u << k : 0u;
+                        const uint32_t at = __vcmpeq4(x[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                        if (at) x[e] &= ~at;
+                        nan |= at ? 1u << (2 * tig + (k & 1) + 8 * (k >> 1)) : 0u;
                     }
                 }
                 return nan;
@@ -536,36 +651,39 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
     __syncthreads();
 
     // ---- merge the warps, in warp order. A row's output lies in the order
-    // of the lanes' columns: entry 8 nt + c is dim c * VB + nt ----
+    // of the lanes: entry 8 x + c is dim c * VB + x ----
     float *mg = reinterpret_cast<float *>(smem) + warp * RT * F::kPitch;
+    float2 *ml = reinterpret_cast<float2 *>(reinterpret_cast<float *>(smem) + kK8Warps * RT * F::kPitch);
+    const float unit = exp2_fast(eref - kPBits);
 #pragma unroll
-    for (int j = 0; j < RL; j++) {
-        l[j] += __shfl_xor_sync(0xffffffffu, l[j], 1);
-        l[j] += __shfl_xor_sync(0xffffffffu, l[j], 2);
-        float *o = mg + (gid + 8 * j) * F::kPitch;
-        if (tig == 0) *reinterpret_cast<float2 *>(o + DP) = make_float2(m2[j], l[j]);
-        const float f = exp2_fast(eref - kPBits);
+    for (int g = 0; g < NB; g++)
 #pragma unroll
-        for (int nt = 0; nt < F::NT; nt++)
-            *reinterpret_cast<float2 *>(o + 8 * nt + 2 * tig) =
-                make_float2(f * (F::kTwo ? O[nt][0] + O[nt][2] : O[nt][2 * j]),
-                            f * (F::kTwo ? O[nt][1] + O[nt][3] : O[nt][1 + 2 * j]));
-    }
+        for (int e = 0; e < 2; e++) {
+            const int r = 8 * g + 2 * tig + e;
+            l[g][e] += __shfl_xor_sync(0xffffffffu, l[g][e], 4);
+            l[g][e] += __shfl_xor_sync(0xffffffffu, l[g][e], 8);
+            l[g][e] += __shfl_xor_sync(0xffffffffu, l[g][e], 16);
+            if (gid == 0) ml[warp * RT + r] = make_float2(m2[g][e], l[g][e]);
+#pragma unroll
+            for (int mt = 0; mt < F::MT; mt++) {
+                mg[r * F::kPitch + 16 * mt + gid] = unit * O[g][mt][e];
+                mg[r * F::kPitch + 16 * mt + 8 + gid] = unit * O[g][mt][2 + e];
+            }
+        }
     __syncthreads();
     const int live = min(rows, RT), group = blockIdx.z * gridDim.y + blockIdx.y;
     float *part = P.part + ((int64_t)group * P.splits + split) * RT * (DP + 2);
     for (int i = tid; i < live * DP; i += kK8Threads) {
         const int r = i / DP, c = i - r * DP, d = (c & 7) * F::VB + (c >> 3);
-        const float *o = reinterpret_cast<const float *>(smem) + r * F::kPitch;
+        const float *o = reinterpret_cast<const float *>(smem) + r * F::kPitch + c;
         float M = kLowest, L = 0.0f, A = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kK8Warps; w++) M = fmaxf(M, o[w * RT * F::kPitch + DP]);
+        for (int w = 0; w < kK8Warps; w++) M = fmaxf(M, ml[w * RT + r].x);
 #pragma unroll
         for (int w = 0; w < kK8Warps; w++) {
-            const float *ow = o + w * RT * F::kPitch;
-            const float f = exp2_fast(ow[DP] - M);
-            L += f * ow[DP + 1];
-            A += f * ow[c];
+            const float f = exp2_fast(ml[w * RT + r].x - M);
+            L += f * ml[w * RT + r].y;
+            A += f * o[w * RT * F::kPitch];
         }
         if (n_act == 1) {
             const int R = rt * RT + r, t = R / G;
@@ -581,9 +699,9 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
 
 // Merges the chunks of a row, in chunk order within each of the W warps that
 // share the row, then across the warps. One CTA does kK8Warps / W rows.
-template <typename T, int DP, int W>
+template <typename T, int DP, int NB, int W>
 __global__ void __launch_bounds__(kK8Threads) k_kv8_merge(const K8Params P) {
-    constexpr int RT = K8Cfg<T, DP>::RT;
+    constexpr int RT = 8 * NB;
     __shared__ float s_part[W > 1 ? kK8Warps : 1][DP + 2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c = 4 * lane;
     const int Dh = P.c.head_dim, H = P.a.n_heads, G = P.G, s = blockIdx.y;
@@ -644,7 +762,7 @@ __global__ void __launch_bounds__(kK8Threads) k_kv8_merge(const K8Params P) {
 }
 
 struct K8Plan {
-    int G, row_tiles, splits, chunk;
+    int G, rt, row_tiles, splits, chunk;   // rt: rows of a tile
     size_t bytes;
 };
 
@@ -654,8 +772,8 @@ struct K8Plan {
 static K8Plan k8_plan(const SepiaKv8Cache &c, const SepiaKv8Step &b, const SepiaKv8Attn &a) {
     constexpr int64_t kUnit = kK8Unit * kK8Warps, kMaxChunk = 1024;
     K8Plan p;
-    const int rt = a.x_f16 ? 16 : 8;
     p.G = a.n_heads / c.n_kv_heads;
+    const int rt = p.rt = (int64_t)b.max_new * p.G <= 8 ? 8 : 16;
     p.row_tiles = (int)(((int64_t)b.max_new * p.G + rt - 1) / rt);
     const int64_t span = a.window ? std::min<int64_t>(b.max_kv, (int64_t)a.window + b.max_new + kK8Tile) : b.max_kv;
     const int64_t groups = (int64_t)b.n_seqs * c.n_kv_heads * p.row_tiles;
@@ -667,28 +785,32 @@ static K8Plan k8_plan(const SepiaKv8Cache &c, const SepiaKv8Step &b, const Sepia
     return p;
 }
 
-template <typename T, int DP, bool FULL>
-static int k8_launch(K8Params &P, cudaStream_t st) {
-    using F = K8Cfg<T, DP>;
+template <typename T, int DP, int NB, bool FULL>
+static int k8_launch(const K8Params &P, cudaStream_t st) {
+    using F = K8Cfg<T, DP, NB>;
     const int64_t rows = (int64_t)P.b.max_new * P.a.n_heads;
-    P.bias_rows = P.a.rel_extent == 0 ? 0 : (int64_t)P.b.max_new * P.G <= 8 ? 1 : F::RL;
-    const int smem = std::max(kK8Warps * kK8Stages * F::stage(P.bias_rows), F::kMergeB);
-    if (!ensure_smem((const void *)k_kv8_attn<T, DP, FULL>, smem)) return 0;
+    const int smem = std::max(F::kQB + kK8Warps * kK8Stages * F::stage(P.a.rel_extent > 0), F::kMergeB);
+    if (!ensure_smem((const void *)k_kv8_attn<T, DP, NB, FULL>, smem)) return 0;
     const dim3 grid((unsigned)P.splits, (unsigned)(P.c.n_kv_heads * P.row_tiles), (unsigned)P.b.n_seqs);
-    if (!check(launch_pdl(k_kv8_attn<T, DP, FULL>, grid, dim3(kK8Threads), smem, st, P), "kv8_attn launch")) return 0;
+    if (!check(launch_pdl(k_kv8_attn<T, DP, NB, FULL>, grid, dim3(kK8Threads), smem, st, P), "kv8_attn launch")) return 0;
     if (P.splits == 1) return 1;
     // one warp per row while a row has few chunks, four beyond
     const dim3 g1((unsigned)((rows + kK8Warps - 1) / kK8Warps), (unsigned)P.b.n_seqs), g4((unsigned)rows, (unsigned)P.b.n_seqs);
-    const cudaError_t e = P.splits <= 8 ? launch_pdl(k_kv8_merge<T, DP, 1>, g1, dim3(kK8Threads), 0, st, P)
-                                        : launch_pdl(k_kv8_merge<T, DP, 4>, g4, dim3(kK8Threads), 0, st, P);
+    const cudaError_t e = P.splits <= 8 ? launch_pdl(k_kv8_merge<T, DP, NB, 1>, g1, dim3(kK8Threads), 0, st, P)
+                                        : launch_pdl(k_kv8_merge<T, DP, NB, 4>, g4, dim3(kK8Threads), 0, st, P);
     return check(e, "kv8_attn merge launch");
 }
 
+template <typename T, int DP, bool FULL>
+static int k8_launch_rows(const K8Params &P, int rt, cudaStream_t st) {
+    return rt == 8 ? k8_launch<T, DP, 1, FULL>(P, st) : k8_launch<T, DP, 2, FULL>(P, st);
+}
+
 template <typename T>
-static int k8_launch_dim(K8Params &P, cudaStream_t st) {
+static int k8_launch_dim(const K8Params &P, int rt, cudaStream_t st) {
     const int Dh = P.c.head_dim;
-    if (Dh <= 64) return Dh == 64 ? k8_launch<T, 64, true>(P, st) : k8_launch<T, 64, false>(P, st);
-    return Dh == 128 ? k8_launch<T, 128, true>(P, st) : k8_launch<T, 128, false>(P, st);
+    if (Dh <= 64) return Dh == 64 ? k8_launch_rows<T, 64, true>(P, rt, st) : k8_launch_rows<T, 64, false>(P, rt, st);
+    return Dh == 128 ? k8_launch_rows<T, 128, true>(P, rt, st) : k8_launch_rows<T, 128, false>(P, rt, st);
 }
 
 static int k8_check(const SepiaKv8Cache *c, const SepiaKv8Step *b, const SepiaKv8Attn *a) {
@@ -732,9 +854,10 @@ extern "C" int sepia_cuda_kv8_attn(const SepiaKv8Cache *c, const SepiaKv8Step *b
     P.row_tiles = p.row_tiles;
     P.splits = p.splits;
     P.chunk = p.chunk;
-    P.two16 = 65536u;
+    const int64_t q_b = a->x_f16 ? 8 : 16, q_sz = a->x_f16 ? 2 : 4;
+    P.q_vec = reinterpret_cast<uintptr_t>(a->q) % q_b == 0 && a->q_stride * q_sz % q_b == 0;
     P.part = (float *)ws;
     P.err = dev_info().err;
     cudaStream_t st = as_stream(stream);
-    return a->x_f16 ? k8_launch_dim<__half>(P, st) : k8_launch_dim<float>(P, st);
+    return a->x_f16 ? k8_launch_dim<__half>(P, p.rt, st) : k8_launch_dim<float>(P, p.rt, st);
 }
