@@ -19,8 +19,11 @@
 //   Layout    the dims of a k step and of an output tile are permuted so that
 //             a lane's codes are 16 consecutive bytes of a key row (K) or of
 //             four key rows (V). Each lane copies just the bytes that it will
-//             use into a ring of its own in shared memory (cp.async), so no
-//             lane waits for another and nothing conflicts.
+//             use into slots of its own in shared memory (cp.async), so no
+//             lane waits for another and nothing conflicts. A warp's slots hold
+//             one step: keys are fetched again as soon as their scores are
+//             done, values when their output is, each behind the other half
+//             of the step and three more warps of the scheduler.
 #include "kv8.cuh"
 #include "runtime.h"
 
@@ -34,8 +37,8 @@ constexpr int kK8Warps = 4;
 constexpr int kK8Threads = 32 * kK8Warps;
 constexpr int kK8Tile = 16;              // keys of one scale: a block is a multiple of it
 constexpr int kK8Unit = 2 * kK8Tile;     // keys per warp step
-constexpr int kK8Stages = 2;             // steps in a warp's ring
-constexpr int kK8CtasPerSm = 3;
+// CTAs an SM holds: by registers (128 or 168 a thread)
+constexpr int k8_ctas(int nb) { return nb == 1 ? 4 : 3; }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLowest = -3.402823466e38f;
 // Weights reach the tensor core as 2^(score - maximum + kPBits), in base 2.
@@ -112,15 +115,16 @@ struct K8Cfg {
     static constexpr int kHeadB = 16;                 // a step's scales
     static constexpr int kPitch = DP + 4;             // of a merge row: the lanes' stores meet no bank twice
     static constexpr int kMergeB = kK8Warps * RT * (kPitch + 2) * 4;
-    static constexpr int kQB = NB > 1 ? NB * KS * 32 * 8 * TERMS : 0;   // q operands, kept in registers with one group
-    // bytes of a ring stage, with room for a band where there is one
+    static constexpr bool kQRegs = NB == 1 && TERMS == 1;   // q operands in registers, else in shared memory
+    static constexpr int kQB = kQRegs ? 0 : NB * KS * 32 * 8 * TERMS;
+    // bytes of a warp's slots, with room for a band where there is one
     static constexpr int stage(bool band) { return 2 * kTileB + kHeadB + (band ? NB * 8 * 128 : 0); }
 };
 
 // FULL: head_dim is DP (64 or 128), every offset a constant; otherwise the
 // dims past head_dim are read as zeros.
 template <typename T, int DP, int NB, bool FULL>
-__global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8Params P) {
+__global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Params P) {
     using F = K8Cfg<T, DP, NB>;
     constexpr int RT = F::RT, TERMS = F::TERMS;
     extern __shared__ __align__(16) uint8_t smem[];
@@ -151,13 +155,13 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
     if (split >= n_act) return;
     const int c0 = lo + split * P.chunk, c1 = min(pb + 1, c0 + P.chunk);
 
-    // ---- coded steps: this warp's share of [c0, min(c1, tail0)), through its ring ----
+    // ---- coded steps: this warp's share of [c0, min(c1, tail0)), through its slots ----
     const int ce = min(c1, tail0);
     const int n_units = ce > c0 ? (ce - c0 + kK8Unit - 1) / kK8Unit : 0;
     const int mine = n_units > warp ? (n_units - warp + kK8Warps - 1) / kK8Warps : 0;
     const int stage_b = F::stage(E > 0);
-    uint8_t *ring = smem + F::kQB + warp * kK8Stages * stage_b;
-    const uint32_t ring_u = smem_u32(ring);
+    uint8_t *st = smem + F::kQB + warp * stage_b;
+    const uint32_t st_u = smem_u32(st);
     // the pool's block of this lane's tile: tile lane % 2 of step i + lane / 2
     int id_l = -1;
     auto look_up = [&](int i) {
@@ -172,35 +176,122 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
         t = R / G;
         h = hk * G + R - t * G;
     };
-    constexpr int NQ = NB == 1 ? F::KS : 1;
-    uint32_t qb[NQ][2 * TERMS];                        // [k step][term][half]
-    float qx[NB];                                      // row gid's factor on its products
-#pragma unroll
-    for (int g = 0; g < NB; g++) {
-        if (NB > 1 && (g & (kK8Warps - 1)) != warp) continue;   // one warp writes a group's operands
+    T q_raw[F::KS][4];                                 // of group `warp` (or the only one), fetched before all else
+    const int q_group = F::kQRegs ? 0 : warp;
+    if (q_group < NB) {
         int t, h;
-        row_of(8 * g + gid, t, h);
-        const bool on = 8 * g + gid < rows;
+        row_of(8 * q_group + gid, t, h);
         const T *q = (const T *)P.a.q + (int64_t)(sq.n0 + t) * P.a.q_stride + (int64_t)h * Dh;
-        float x[F::KS][4], amax = 0.0f;
+        const bool on = 8 * q_group + gid < rows;
 #pragma unroll
         for (int ks = 0; ks < F::KS; ks++) {
             const int d = 64 * (ks / 4) + 16 * tig + 4 * (ks % 4);
-            T v[4] = {};
             if (on && d < Dh) {
                 if (P.q_vec) {
-                    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(q + d);
-                    else *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(q + d);
+                    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(q_raw[ks]) = *reinterpret_cast<const uint4 *>(q + d);
+                    else *reinterpret_cast<uint2 *>(q_raw[ks]) = *reinterpret_cast<const uint2 *>(q + d);
                 } else {
-                    for (int e = 0; e < 4; e++) v[e] = q[d + e];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) q_raw[ks][e] = q[d + e];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) q_raw[ks][e] = (T)0.0f;
+            }
+        }
+    }
+    // this lane's rows of each group as columns of a product: 2 tig and 2 tig + 1
+    int pos[NB][2];
+    int rel_at[NB][2];                                 // their bands, from the first token's
+    const float *rel = P.a.rel_logits + (int64_t)(sq.n0 + ta) * H * E;
+#pragma unroll
+    for (int g = 0; g < NB; g++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            int t, h;
+            row_of(8 * g + 2 * tig + e, t, h);
+            pos[g][e] = sq.held + t;
+            rel_at[g][e] = ((t - ta) * H + h) * E;
+        }
+
+    auto fetch_keys = [&](int i) {                     // and the scales
+        if (i < mine) {
+            if (i && (i & 15) == 0) look_up(i);
+            if ((lane >> 1) == (i & 15)) {             // a tile that is not there: hidden
+                const int to = 2 * F::kTileB + 8 * (lane & 1);
+                if (id_l >= 0) {
+                    cp_async_bytes<4>(st_u + to, P.c.k_scale + (int64_t)id_l * Hkv + hk);
+                    cp_async_bytes<4>(st_u + to + 4, P.c.v_scale + (int64_t)id_l * Hkv + hk);
+                } else {
+                    *reinterpret_cast<float2 *>(st + to) = make_float2(-1.0f, 1.0f);
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                x[ks][e] = (float)v[e];
-                amax = fmaxf(amax, fabsf(x[ks][e]));
+            for (int u = 0; u < 2; u++) {
+                const int id = max(0, __shfl_sync(0xffffffffu, id_l, (2 * i + u) & 31));
+                const int at = c0 + (warp + kK8Warps * i) * kK8Unit + u * kK8Tile;
+                const uint8_t *K = (const uint8_t *)P.c.k + (((int64_t)id * Hkv + hk) * B + (at & (B - 1)) + gid) * Dh + 16 * tig;
+                const uint32_t to = st_u + u * F::kTileB + lane * 16;
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int j = 0; j < F::KW; j++) {
+                        const bool on = FULL || 64 * j + 16 * tig < Dh;
+                        if constexpr (FULL) cp_async_bytes<16>(to + (n * F::KW + j) * 512, K + n * 8 * Dh + j * 64);
+                        else cp_async_or_zero<16>(to + (n * F::KW + j) * 512, on ? K + n * 8 * Dh + j * 64 : P.c.k, on);
+                    }
             }
         }
+        cp_async_commit();
+    };
+    auto fetch_values = [&](int i) {                   // and the band
+        if (i < mine) {
+            const int t0 = c0 + (warp + kK8Warps * i) * kK8Unit;
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int id = max(0, __shfl_sync(0xffffffffu, id_l, (2 * i + u) & 31));
+                const uint8_t *V = (const uint8_t *)P.c.v +
+                                   (((int64_t)id * Hkv + hk) * B + ((t0 + u * kK8Tile) & (B - 1)) + 2 * tig) * Dh + gid * F::VB;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t to = st_u + u * F::kTileB + F::kKeyB + k * (32 * F::VB) + lane * F::VB;
+                    const uint8_t *src = V + ((k & 1) + 8 * (k >> 1)) * Dh;
+                    const bool on = FULL || gid * F::VB < Dh;
+                    if constexpr (FULL) cp_async_bytes<F::VB>(to, src);
+                    else cp_async_or_zero<F::VB>(to, on ? src : P.c.v, on);
+                }
+            }
+            if (E && pa - (t0 + kK8Unit - 1) < E) {
+#pragma unroll
+                for (int g = 0; g < NB; g++)
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {      // key gid + 8 (k / 2), row 2 tig + k % 2
+                        const int far = pos[g][k & 1] - (t0 + gid + 8 * (k >> 1));
+                        const bool on = far >= 0 && far < E;
+                        cp_async_or_zero<4>(st_u + 2 * F::kTileB + F::kHeadB + (8 * g + k) * 128 + lane * 4,
+                                            rel + rel_at[g][k & 1] + (on ? far : 0), on);
+                    }
+            }
+        }
+        cp_async_commit();
+    };
+    fetch_keys(0);
+    fetch_values(0);
+
+    // ---- q as operands ----
+    static_assert(NB <= kK8Warps, "a warp per group writes its operands");
+    constexpr int NQ = F::kQRegs ? F::KS : 1;
+    uint32_t qb[NQ][2 * TERMS];                        // [k step][term][half]
+    float qx = 1.0f;                                   // row gid's factor on its products
+    if (q_group < NB) {
+        float x[F::KS][4], amax = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < F::KS; ks++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x[ks][e] = (float)q_raw[ks][e];
+                amax = fmaxf(amax, fabsf(x[ks][e]));
+            }
         float f = 1.0f;
         if constexpr (TERMS == 2) {
             // the row times a power of two that puts its largest in [2^13, 2^14): both terms stay normal fp16
@@ -208,9 +299,7 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
             const int ex = amax > 0.0f ? max((int)(__float_as_uint(amax) >> 23) - 127, -100) : 13;
             f = __uint_as_float((uint32_t)(127 + 13 - ex) << 23);
-            qx[g] = __uint_as_float((uint32_t)(127 - 13 + ex) << 23);
-        } else {
-            qx[g] = 1.0f;
+            qx = __uint_as_float((uint32_t)(127 - 13 + ex) << 23);
         }
 #pragma unroll
         for (int ks = 0; ks < F::KS; ks++) {
@@ -225,18 +314,18 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
                     w[2 + e] = pack_half2(u - b.x, v - b.y);
                 }
             }
-            if constexpr (NB == 1) {
+            if constexpr (F::kQRegs) {
 #pragma unroll
                 for (int e = 0; e < 2 * TERMS; e++) qb[ks][e] = w[e];
             } else {
-                uint32_t *to = reinterpret_cast<uint32_t *>(smem) + ((g * F::KS + ks) * 32 + lane) * (2 * TERMS);
+                uint32_t *to = reinterpret_cast<uint32_t *>(smem) + ((q_group * F::KS + ks) * 32 + lane) * (2 * TERMS);
 #pragma unroll
                 for (int e = 0; e < 2 * TERMS; e++) to[e] = w[e];
             }
         }
     }
     auto q_op = [&](int g, int ks, uint32_t (&w)[2 * TERMS]) {
-        if constexpr (NB == 1) {
+        if constexpr (F::kQRegs) {
 #pragma unroll
             for (int e = 0; e < 2 * TERMS; e++) w[e] = qb[ks][e];
         } else {
@@ -245,74 +334,6 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
             else *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(from);
         }
     };
-
-    // this lane's rows of each group as columns of a product: 2 tig and 2 tig + 1
-    int pos[NB][2];
-    const float *rel[NB][2];
-#pragma unroll
-    for (int g = 0; g < NB; g++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            int t, h;
-            row_of(8 * g + 2 * tig + e, t, h);
-            pos[g][e] = sq.held + t;
-            rel[g][e] = P.a.rel_logits + ((int64_t)(sq.n0 + t) * H + h) * E;
-        }
-
-    auto issue = [&](int i) {
-        if (i < mine) {
-            if (i && (i & 15) == 0) look_up(i);
-            const int t0 = c0 + (warp + kK8Warps * i) * kK8Unit;
-            const uint32_t st = ring_u + (i & (kK8Stages - 1)) * stage_b;
-            if ((lane >> 1) == (i & 15)) {             // the tile's scales; a tile that is not there: hidden
-                const uint32_t to = st + 2 * F::kTileB + 8 * (lane & 1);
-                if (id_l >= 0) {
-                    cp_async_bytes<4>(to, P.c.k_scale + (int64_t)id_l * Hkv + hk);
-                    cp_async_bytes<4>(to + 4, P.c.v_scale + (int64_t)id_l * Hkv + hk);
-                } else {
-                    *reinterpret_cast<float2 *>(ring + (i & (kK8Stages - 1)) * stage_b + 2 * F::kTileB + 8 * (lane & 1)) =
-                        make_float2(-1.0f, 1.0f);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int id = max(0, __shfl_sync(0xffffffffu, id_l, (2 * i + u) & 31));
-                const int64_t row0 = ((int64_t)id * Hkv + hk) * B + ((t0 + u * kK8Tile) & (B - 1));
-                const uint8_t *K = (const uint8_t *)P.c.k + row0 * Dh + gid * Dh + 16 * tig;
-                const uint8_t *V = (const uint8_t *)P.c.v + row0 * Dh + 2 * tig * Dh + gid * F::VB;
-                const uint32_t at = st + u * F::kTileB + lane * 16;
-#pragma unroll
-                for (int n = 0; n < 2; n++)
-#pragma unroll
-                    for (int j = 0; j < F::KW; j++) {
-                        if constexpr (FULL) cp_async_bytes<16>(at + (n * F::KW + j) * 512, K + n * 8 * Dh + j * 64);
-                        else cp_async_or_zero<16>(at + (n * F::KW + j) * 512, 64 * j + 16 * tig < Dh ? K + n * 8 * Dh + j * 64 : K,
-                                                  64 * j + 16 * tig < Dh);
-                    }
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const uint32_t to = st + u * F::kTileB + F::kKeyB + k * (32 * F::VB) + lane * F::VB;
-                    const uint8_t *src = V + ((k & 1) + 8 * (k >> 1)) * Dh;
-                    if constexpr (FULL) cp_async_bytes<F::VB>(to, src);
-                    else cp_async_or_zero<F::VB>(to, gid * F::VB < Dh ? src : (const uint8_t *)P.c.v, gid * F::VB < Dh);
-                }
-            }
-            if (E && pa - (t0 + kK8Unit - 1) < E) {
-#pragma unroll
-                for (int g = 0; g < NB; g++)
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {      // key gid + 8 (k / 2), row 2 tig + k % 2
-                        const int far = pos[g][k & 1] - (t0 + gid + 8 * (k >> 1));
-                        const bool on = far >= 0 && far < E;
-                        cp_async_or_zero<4>(st + 2 * F::kTileB + F::kHeadB + (8 * g + k) * 128 + lane * 4,
-                                            rel[g][k & 1] + (on ? far : 0), on);
-                    }
-            }
-        }
-        cp_async_commit();
-    };
-#pragma unroll
-    for (int i = 0; i < kK8Stages - 1; i++) issue(i);
 
     float qmul[NB][2], tau[NB][2];                     // of the lane's rows as columns
 #pragma unroll
@@ -323,13 +344,10 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
             row_of(8 * g + 2 * tig + e, t, h);
             tau[g][e] = P.a.tau ? P.a.tau[sq.n0 + t] : 1.0f;
             qmul[g][e] = P.a.scale * kLog2e;
-            if constexpr (NB == 1) qmul[g][e] *= __shfl_sync(0xffffffffu, qx[g], 8 * tig + 4 * e);
         }
-    if constexpr (NB > 1) {
+    if constexpr (!F::kQRegs) {
         __shared__ float s_qx[RT];
-#pragma unroll
-        for (int g = 0; g < NB; g++)
-            if ((g & (kK8Warps - 1)) == warp && tig == 0) s_qx[8 * g + gid] = qx[g];
+        if (q_group < NB && tig == 0) s_qx[8 * q_group + gid] = qx;
         __syncthreads();
 #pragma unroll
         for (int g = 0; g < NB; g++)
@@ -488,7 +506,7 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
     using One = std::integral_constant<int, 1>;
     using Two = std::integral_constant<int, 2>;
 
-    // ---- the tail's fp16 tiles, one a warp, while the ring fills ----
+    // ---- the tail's fp16 tiles, one a warp, while the slots fill ----
     {
         const int t0 = tail0 + kK8Tile * warp;
         if (t0 >= c0 && t0 < c1) {
@@ -537,7 +555,7 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
                 },
                 [&](int g, int i) {
                     const int far = pos[g][i & 1] - (t0 + gid + 8 * (i >> 1));
-                    return far >= 0 && far < E ? rel[g][i & 1][far] : 0.0f;
+                    return far >= 0 && far < E ? rel[rel_at[g][i & 1] + far] : 0.0f;
                 },
                 [&](int) {
                     uint32_t nan = 0;
@@ -555,11 +573,8 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
     }
 
     for (int i = 0; i < mine; i++) {
-        __syncwarp();                                  // every lane is done with the stage that is filled next
-        issue(i + kK8Stages - 1);
-        cp_async_wait<kK8Stages - 1>();
+        cp_async_wait<1>();                            // the keys
         __syncwarp();
-        uint8_t *st = ring + (i & (kK8Stages - 1)) * stage_b;
         const float4 sc = *reinterpret_cast<const float4 *>(st + 2 * F::kTileB);
         const float ksc[2] = {sc.x, sc.z};
         const float ev[2] = {(float)((int)(__float_as_uint(sc.y) >> 23 & 255) - 127),
@@ -614,6 +629,9 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
                     for (int u = 0; u < 2; u++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) S[g][u][e] += R[g][u][e];
+                __syncwarp();                          // every lane has read the scales
+                fetch_keys(i + 1);
+                cp_async_wait<1>();                    // the values
             },
             [&](int u, int mt, uint32_t (&a)[4]) {
                 if (mt == 0) {
@@ -632,7 +650,7 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
             [&](int g, int k) {
                 return *reinterpret_cast<const float *>(st + 2 * F::kTileB + F::kHeadB + (8 * g + k) * 128 + lane * 4);
             },
-            [&](int u) {                               // the lane's own copies, in its ring
+            [&](int u) {                               // the lane's own copies, in its slots
                 uint32_t nan = 0;
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
@@ -646,6 +664,7 @@ __global__ void __launch_bounds__(kK8Threads, kK8CtasPerSm) k_kv8_attn(const K8P
                 }
                 return nan;
             });
+        fetch_values(i + 1);
     }
     cp_async_wait<0>();
     __syncthreads();
@@ -777,7 +796,7 @@ static K8Plan k8_plan(const SepiaKv8Cache &c, const SepiaKv8Step &b, const Sepia
     p.row_tiles = (int)(((int64_t)b.max_new * p.G + rt - 1) / rt);
     const int64_t span = a.window ? std::min<int64_t>(b.max_kv, (int64_t)a.window + b.max_new + kK8Tile) : b.max_kv;
     const int64_t groups = (int64_t)b.n_seqs * c.n_kv_heads * p.row_tiles;
-    const int64_t slots = (int64_t)(dev_info().sm_count > 0 ? dev_info().sm_count : 148) * kK8CtasPerSm;
+    const int64_t slots = (int64_t)(dev_info().sm_count > 0 ? dev_info().sm_count : 148) * k8_ctas(rt / 8);
     const int64_t one = (groups * span + slots - 1) / slots;
     p.chunk = (int)(std::min(kMaxChunk, std::max<int64_t>(one, 1)) + kUnit - 1) / kUnit * kUnit;
     p.splits = (int)std::max<int64_t>(1, (span + p.chunk - 1) / p.chunk);
@@ -789,7 +808,7 @@ template <typename T, int DP, int NB, bool FULL>
 static int k8_launch(const K8Params &P, cudaStream_t st) {
     using F = K8Cfg<T, DP, NB>;
     const int64_t rows = (int64_t)P.b.max_new * P.a.n_heads;
-    const int smem = std::max(F::kQB + kK8Warps * kK8Stages * F::stage(P.a.rel_extent > 0), F::kMergeB);
+    const int smem = std::max(F::kQB + kK8Warps * F::stage(P.a.rel_extent > 0), F::kMergeB);
     if (!ensure_smem((const void *)k_kv8_attn<T, DP, NB, FULL>, smem)) return 0;
     const dim3 grid((unsigned)P.splits, (unsigned)(P.c.n_kv_heads * P.row_tiles), (unsigned)P.b.n_seqs);
     if (!check(launch_pdl(k_kv8_attn<T, DP, NB, FULL>, grid, dim3(kK8Threads), smem, st, P), "kv8_attn launch")) return 0;
@@ -820,6 +839,8 @@ static int k8_check(const SepiaKv8Cache *c, const SepiaKv8Step *b, const SepiaKv
     if (a->n_heads <= 0 || a->n_heads % c->n_kv_heads)
         return fail("%s: %d query heads over %d KV heads", what, a->n_heads, c->n_kv_heads);
     if (a->window < 0 || a->rel_extent < 0) return fail("%s: negative window or rel_extent", what);
+    // offsets inside a tile's bands are 32-bit: at most 17 tokens
+    if ((int64_t)a->n_heads * a->rel_extent > INT32_MAX / 17) return fail("%s: rel_extent %d too large", what, a->rel_extent);
     if ((int64_t)b->max_new * a->n_heads > INT32_MAX / 2) return fail("%s: step too large", what);
     if (b->n_seqs > 65535) return fail("%s: %d sequences (at most 65535)", what, b->n_seqs);
     return 1;
