@@ -18,12 +18,14 @@
 //             the weight are two fp16 terms (22 bits), summed in one result.
 //   Layout    the dims of a k step and of an output tile are permuted so that
 //             a lane's codes are 16 consecutive bytes of a key row (K) or of
-//             four key rows (V). Each lane copies just the bytes that it will
-//             use into slots of its own in shared memory (cp.async), so no
-//             lane waits for another and nothing conflicts. A warp's slots hold
-//             one step: keys are fetched again as soon as their scores are
-//             done, values when their output is, each behind the other half
-//             of the step and three more warps of the scheduler.
+//             four key rows (V). A warp copies its tiles as they lie (cp.async,
+//             512 bytes in a row an instruction; copying each lane's own bytes
+//             instead needed no exchange between lanes but reached 4.1 TB/s
+//             where this reaches 5.8) into shared memory of its own, 16-byte
+//             pieces swizzled so that neither side meets a bank twice. The
+//             slots hold one step: keys are fetched again as soon as their
+//             scores are done, values when their output is, each behind the
+//             other half of the step and three more warps of the scheduler.
 #include "kv8.cuh"
 #include "runtime.h"
 
@@ -111,7 +113,7 @@ struct K8Cfg {
     static constexpr int KW = DP / 64;                // 16-byte pieces of a key row per lane
     static constexpr int VB = DP / 8;                 // bytes of a value row per lane
     static constexpr int MT = DP / 16, KS = DP / 16;  // output tiles of 16 dims, k steps of 16
-    static constexpr int kKeyB = 2 * KW * 512, kValB = 4 * VB * 32, kTileB = kKeyB + kValB;
+    static constexpr int kKeyB = kK8Tile * DP, kValB = kKeyB, kTileB = 2 * kKeyB;
     static constexpr int kHeadB = 16;                 // a step's scales
     static constexpr int kPitch = DP + 4;             // of a merge row: the lanes' stores meet no bank twice
     static constexpr int kMergeB = kK8Warps * RT * (kPitch + 2) * 4;
@@ -214,6 +216,41 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
             rel_at[g][e] = ((t - ta) * H + h) * E;
         }
 
+    // Copies: piece q (16 bytes) of a tile to its place in shared memory. In
+    // lines of 128 bytes, pieces 0-7: keys swap the halves of every second
+    // line of whole rows; values move by twice the row pair.
+    auto place = [&](int q, bool values) {
+        const int row = FULL ? q / (DP / 16) : q / (Dh / 16), c = FULL ? q % (DP / 16) : q - row * (Dh / 16);
+        const int piece = row * (DP / 16) + c, f = values ? ((row >> 1) & 3) * 2 : DP == 128 ? (row & 1) * 4 : 0;
+        return ((piece & ~7) | ((piece & 7) ^ f)) * 16;
+    };
+    constexpr int NC = DP / 32;                        // copies of a lane per tile
+    int to_k[NC], to_v[NC];
+#pragma unroll
+    for (int k = 0; k < NC; k++) to_k[k] = place(lane + 32 * k, false), to_v[k] = place(lane + 32 * k, true);
+    if constexpr (!FULL) {                             // dims past head_dim: zeros, once
+        for (int k = lane; k < 2 * F::kTileB / 16; k += 32) reinterpret_cast<uint4 *>(st)[k] = make_uint4(0, 0, 0, 0);
+        __syncwarp();
+    }
+    auto copy = [&](int i, const uint8_t *from, int offset, const int (&to)[NC]) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int id = max(0, __shfl_sync(0xffffffffu, id_l, (2 * i + u) & 31));
+            const int at = c0 + (warp + kK8Warps * i) * kK8Unit + u * kK8Tile;
+            const uint8_t *src = from + (((int64_t)id * Hkv + hk) * B + (at & (B - 1))) * Dh + lane * 16;
+#pragma unroll
+            for (int k = 0; k < NC; k++)
+                if (FULL || lane + 32 * k < Dh) cp_async_bytes<16>(st_u + u * F::kTileB + offset + to[k], src + k * 512);
+        }
+    };
+    // ... and where the lane's operands lie: keys gid + 8 n, piece 4 j + tig; values of keys 2 tig + {0, 1, 8, 9}
+    int from_k[F::KW], from_v[2];
+#pragma unroll
+    for (int j = 0; j < F::KW; j++) from_k[j] = DP == 128 ? gid * 128 + (4 * (j ^ (gid & 1)) + tig) * 16 : gid * 64 + tig * 16;
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+        from_v[k] = DP == 128 ? (2 * tig + k) * 128 + (gid ^ (2 * tig)) * 16
+                              : tig * 128 + (((4 * k + (gid >> 1)) ^ (2 * tig)) * 16) + (gid & 1) * 8;
     auto fetch_keys = [&](int i) {                     // and the scales
         if (i < mine) {
             if (i && (i & 15) == 0) look_up(i);
@@ -226,41 +263,14 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
                     *reinterpret_cast<float2 *>(st + to) = make_float2(-1.0f, 1.0f);
                 }
             }
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int id = max(0, __shfl_sync(0xffffffffu, id_l, (2 * i + u) & 31));
-                const int at = c0 + (warp + kK8Warps * i) * kK8Unit + u * kK8Tile;
-                const uint8_t *K = (const uint8_t *)P.c.k + (((int64_t)id * Hkv + hk) * B + (at & (B - 1)) + gid) * Dh + 16 * tig;
-                const uint32_t to = st_u + u * F::kTileB + lane * 16;
-#pragma unroll
-                for (int n = 0; n < 2; n++)
-#pragma unroll
-                    for (int j = 0; j < F::KW; j++) {
-                        const bool on = FULL || 64 * j + 16 * tig < Dh;
-                        if constexpr (FULL) cp_async_bytes<16>(to + (n * F::KW + j) * 512, K + n * 8 * Dh + j * 64);
-                        else cp_async_or_zero<16>(to + (n * F::KW + j) * 512, on ? K + n * 8 * Dh + j * 64 : P.c.k, on);
-                    }
-            }
+            copy(i, (const uint8_t *)P.c.k, 0, to_k);
         }
         cp_async_commit();
     };
     auto fetch_values = [&](int i) {                   // and the band
         if (i < mine) {
             const int t0 = c0 + (warp + kK8Warps * i) * kK8Unit;
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const int id = max(0, __shfl_sync(0xffffffffu, id_l, (2 * i + u) & 31));
-                const uint8_t *V = (const uint8_t *)P.c.v +
-                                   (((int64_t)id * Hkv + hk) * B + ((t0 + u * kK8Tile) & (B - 1)) + 2 * tig) * Dh + gid * F::VB;
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const uint32_t to = st_u + u * F::kTileB + F::kKeyB + k * (32 * F::VB) + lane * F::VB;
-                    const uint8_t *src = V + ((k & 1) + 8 * (k >> 1)) * Dh;
-                    const bool on = FULL || gid * F::VB < Dh;
-                    if constexpr (FULL) cp_async_bytes<F::VB>(to, src);
-                    else cp_async_or_zero<F::VB>(to, on ? src : P.c.v, on);
-                }
-            }
+            copy(i, (const uint8_t *)P.c.v, F::kKeyB, to_v);
             if (E && pa - (t0 + kK8Unit - 1) < E) {
 #pragma unroll
                 for (int g = 0; g < NB; g++)
@@ -597,7 +607,7 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
                     for (int u = 0; u < 2; u++)
 #pragma unroll
                         for (int n = 0; n < 2; n++)
-                            k[u][n] = *reinterpret_cast<const uint4 *>(st + u * F::kTileB + (n * F::KW + j) * 512 + lane * 16);
+                            k[u][n] = *reinterpret_cast<const uint4 *>(st + u * F::kTileB + n * 8 * DP + from_k[j]);
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         uint32_t a[2][4];
@@ -629,15 +639,16 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
                     for (int u = 0; u < 2; u++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) S[g][u][e] += R[g][u][e];
-                __syncwarp();                          // every lane has read the scales
+                __syncwarp();                          // every lane has read the keys and the scales
                 fetch_keys(i + 1);
                 cp_async_wait<1>();                    // the values
+                __syncwarp();
             },
             [&](int u, int mt, uint32_t (&a)[4]) {
                 if (mt == 0) {
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        const uint8_t *src = st + u * F::kTileB + F::kKeyB + k * (32 * F::VB) + lane * F::VB;
+                        const uint8_t *src = st + u * F::kTileB + F::kKeyB + (k >> 1) * 8 * DP + from_v[k & 1];
                         if constexpr (F::VB == 16) *reinterpret_cast<uint4 *>(v[k]) = *reinterpret_cast<const uint4 *>(src);
                         else *reinterpret_cast<uint2 *>(v[k]) = *reinterpret_cast<const uint2 *>(src);
                     }
@@ -650,11 +661,11 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
             [&](int g, int k) {
                 return *reinterpret_cast<const float *>(st + 2 * F::kTileB + F::kHeadB + (8 * g + k) * 128 + lane * 4);
             },
-            [&](int u) {                               // the lane's own copies, in its slots
+            [&](int u) {                               // in the slots: no other lane reads these bytes
                 uint32_t nan = 0;
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    uint32_t *x = reinterpret_cast<uint32_t *>(st + u * F::kTileB + F::kKeyB + k * (32 * F::VB) + lane * F::VB);
+                    uint32_t *x = reinterpret_cast<uint32_t *>(st + u * F::kTileB + F::kKeyB + (k >> 1) * 8 * DP + from_v[k & 1]);
 #pragma unroll
                     for (int e = 0; e < F::VB / 4; e++) {
                         const uint32_t at = __vcmpeq4(x[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
@@ -664,6 +675,7 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
                 }
                 return nan;
             });
+        __syncwarp();                                  // every lane has read the values
         fetch_values(i + 1);
     }
     cp_async_wait<0>();
