@@ -55,7 +55,8 @@ struct K8Params {
     SepiaKv8Attn a;
     int G, row_tiles, splits, chunk;     // chunk: positions per split, a multiple of kK8Unit * kK8Warps
     int q_vec;                           // four elements of q in one load
-    float *part;                         // [n_seqs, n_kv_heads * row_tiles, splits, rows of a tile, Dh + 2]
+    float *part;                         // [n_seqs, n_kv_heads * row_tiles, splits, rows of a tile, Dh]
+    float2 *part_ml;                     // [n_seqs, n_kv_heads * row_tiles, splits, rows of a tile]: maximum, sum
     int *err;
 };
 
@@ -123,6 +124,16 @@ struct K8Cfg {
     static constexpr int stage(bool band) { return 2 * kTileB + kHeadB + (band ? NB * 8 * 128 : 0); }
 };
 
+// Four dims of a row: sums over the weights' total; zeros where nothing was seen
+template <typename T>
+__device__ __forceinline__ void put_row(T *to, const float (&A)[4], float L) {
+    T y[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) y[e] = (T)(L == 0.0f ? 0.0f : A[e] / L);
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(y);
+    else *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<const uint2 *>(y);
+}
+
 // FULL: head_dim is DP (64 or 128), every offset a constant; otherwise the
 // dims past head_dim are read as zeros.
 template <typename T, int DP, int NB, bool FULL>
@@ -138,9 +149,11 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
     griddep_launch();
     const Kv8Seq sq = kv8_seq(P.c, P.b, s, P.err);
     const int rows = sq.rows * G - rt * RT;            // rows of this tile that exist (may exceed RT)
+    const int64_t cell = ((int64_t)(s * gridDim.y + blockIdx.y) * P.splits + split) * RT;   // of this chunk's rows
+    if (P.splits > 1 && tid < RT) P.part_ml[cell + tid] = make_float2(kLowest, 0.0f);       // empty until it is not
     if (rows <= 0) return;
     if (sq.add < 0) {                                  // idle or out of bounds: zeros
-        if (split == 0)
+        if (split == 0 && P.splits == 1)
             for (int i = tid; i < min(rows, RT) * Dh; i += kK8Threads) {
                 const int R = rt * RT + i / Dh, t = R / G;
                 ((T *)P.a.out)[((int64_t)(sq.n0 + t) * H + hk * G + (R - t * G)) * Dh + i % Dh] = (T)0.0f;
@@ -702,99 +715,102 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
             }
         }
     __syncthreads();
-    const int live = min(rows, RT), group = blockIdx.z * gridDim.y + blockIdx.y;
-    float *part = P.part + ((int64_t)group * P.splits + split) * RT * (DP + 2);
-    for (int i = tid; i < live * DP; i += kK8Threads) {
-        const int r = i / DP, c = i - r * DP, d = (c & 7) * F::VB + (c >> 3);
-        const float *o = reinterpret_cast<const float *>(smem) + r * F::kPitch + c;
-        float M = kLowest, L = 0.0f, A = 0.0f;
+    // a warp merges whole rows, 4 dims a lane
+    for (int r = warp; r < min(rows, RT); r += kK8Warps) {
+        float M = kLowest, L = 0.0f, A[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        float2 x[kK8Warps];
 #pragma unroll
-        for (int w = 0; w < kK8Warps; w++) M = fmaxf(M, ml[w * RT + r].x);
+        for (int w = 0; w < kK8Warps; w++) x[w] = ml[w * RT + r], M = fmaxf(M, x[w].x);
+        const int d = 4 * lane, c = d / F::VB + 8 * (d % F::VB);
+        const float *o = reinterpret_cast<const float *>(smem) + r * F::kPitch + c;
 #pragma unroll
         for (int w = 0; w < kK8Warps; w++) {
-            const float f = exp2_fast(ml[w * RT + r].x - M);
-            L += f * ml[w * RT + r].y;
-            A += f * o[w * RT * F::kPitch];
+            const float f = exp2_fast(x[w].x - M);
+            L += f * x[w].y;
+            if (d < DP)
+#pragma unroll
+                for (int e = 0; e < 4; e++) A[e] += f * o[w * RT * F::kPitch + 8 * e];
         }
-        if (n_act == 1) {
-            const int R = rt * RT + r, t = R / G;
-            if (d < Dh)
-                ((T *)P.a.out)[((int64_t)(sq.n0 + t) * H + hk * G + (R - t * G)) * Dh + d] = (T)(L == 0.0f ? 0.0f : A / L);
+        if (P.splits == 1) {
+            int t, h;
+            row_of(r, t, h);
+            if (d < Dh) put_row((T *)P.a.out + ((int64_t)(sq.n0 + t) * H + h) * Dh + d, A, L);
         } else {
-            float *to = part + r * (DP + 2);
-            if (c == 0) *reinterpret_cast<float2 *>(to) = make_float2(M, L);
-            to[2 + c] = A;
+            if (d < Dh) *reinterpret_cast<float4 *>(P.part + (cell + r) * Dh + d) = make_float4(A[0], A[1], A[2], A[3]);
+            if (lane == 0) P.part_ml[cell + r] = make_float2(M, L);
         }
     }
 }
 
-// Merges the chunks of a row, in chunk order within each of the W warps that
-// share the row, then across the warps. One CTA does kK8Warps / W rows.
-template <typename T, int DP, int NB, int W>
+// Merges the chunks of a row, W warps to a row: each takes a run of them in
+// order, then their results are added in order. One CTA does kK8Warps / W
+// rows. Chunks that no key fell into hold a sum of 0.
+template <typename T, int NB, int W>
 __global__ void __launch_bounds__(kK8Threads) k_kv8_merge(const K8Params P) {
     constexpr int RT = 8 * NB;
-    __shared__ float s_part[W > 1 ? kK8Warps : 1][DP + 2];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c = 4 * lane;
+    __shared__ float s_part[W > 1 ? kK8Warps : 1][kKv8MaxDh];
+    __shared__ float2 s_ml[kK8Warps];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, d = 4 * lane;
     const int Dh = P.c.head_dim, H = P.a.n_heads, G = P.G, s = blockIdx.y;
+    const int at = blockIdx.x * (kK8Warps / W) + warp / W, h = at % H, t = at / H;
+    const int hk = h / G, R = t * G + h - hk * G, rt = R / RT, r = R - rt * RT;
+    if (t >= P.b.max_new) return;                      // with W > 1 the whole CTA
+    const int64_t cell = ((int64_t)(s * P.c.n_kv_heads + hk) * P.row_tiles + rt) * P.splits * RT + r;
+    const int per = (P.splits + W - 1) / W, k0 = (warp % W) * per, k1 = min(P.splits, k0 + per);
     griddep_wait();
     griddep_launch();
-    const int at = blockIdx.x * (kK8Warps / W) + warp / W, h = at % H, t = at / H;
-    const Kv8Seq sq = kv8_seq(P.c, P.b, s, nullptr);
-    if (sq.add < 0 || t >= sq.add) return;             // with W > 1 the whole CTA
-    // the row's tile, and the chunks that k_kv8_attn cut for it
-    const int hk = h / G, R = t * G + h - hk * G, rt = R / RT, r = R - rt * RT;
-    const int ta = rt * RT / G, tb = min(sq.add - 1, (rt * RT + RT - 1) / G);
-    const int lo = P.a.window ? max(0, sq.held + ta - P.a.window + 1) / kK8Tile * kK8Tile : 0;
-    const int n_act = (sq.held + tb + 1 - lo + P.chunk - 1) / P.chunk;
-    if (n_act <= 1) return;
-    const int group = s * P.c.n_kv_heads * P.row_tiles + hk * P.row_tiles + rt;
-    constexpr int64_t stride = (int64_t)RT * (DP + 2);
-    const float *part = P.part + (int64_t)group * P.splits * stride + r * (DP + 2);
+    const int n0 = P.b.start ? P.b.start[s] : s, n1 = P.b.start ? P.b.start[s + 1] : s + 1;
     float M = kLowest, L = 0.0f, A[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k = lane; k < n_act; k += 32) M = fmaxf(M, part[k * stride]);
-    M = warp_max(M);
-    const int per = (n_act + W - 1) / W, k0 = (warp % W) * per, k1 = min(n_act, k0 + per);
-    constexpr int kAhead = 8;                          // chunks in flight per warp
+    constexpr int kAhead = 16;                         // chunks in flight per warp
     for (int k = k0; k < k1; k += kAhead) {
-        float2 x[kAhead][2], ml[kAhead];
+        float4 x[kAhead];
+        float2 y[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
-            const float2 *p = reinterpret_cast<const float2 *>(part + min(k + i, k1 - 1) * stride);
-            ml[i] = p[0];
-            x[i][0] = c < DP ? p[1 + c / 2] : make_float2(0.0f, 0.0f);
-            x[i][1] = c < DP ? p[2 + c / 2] : make_float2(0.0f, 0.0f);
+            const int64_t c = cell + (int64_t)min(k + i, k1 - 1) * RT;
+            y[i] = __ldcg(P.part_ml + c);
+            x[i] = d < Dh ? __ldcg(reinterpret_cast<const float4 *>(P.part + c * Dh + d)) : make_float4(0, 0, 0, 0);
         }
+        float top = M;
 #pragma unroll
-        for (int i = 0; i < kAhead; i++) {
-            const float f = k + i < k1 ? exp2_fast(ml[i].x - M) : 0.0f;
-            L += f * ml[i].y;
-            A[0] += f * x[i][0].x, A[1] += f * x[i][0].y, A[2] += f * x[i][1].x, A[3] += f * x[i][1].y;
-        }
+        for (int i = 0; i < kAhead; i++) top = fmaxf(top, y[i].x);
+        const float g = exp2_fast(M - top);
+        M = top;
+        L *= g, A[0] *= g, A[1] *= g, A[2] *= g, A[3] *= g;
+#pragma unroll
+        for (int i = 0; i < kAhead; i++)
+            if (k + i < k1 && y[i].y != 0.0f) {        // an empty chunk's row was not written
+                const float f = exp2_fast(y[i].x - M);
+                L += f * y[i].y;
+                A[0] += f * x[i].x, A[1] += f * x[i].y, A[2] += f * x[i].z, A[3] += f * x[i].w;
+            }
     }
     if constexpr (W > 1) {
-        if (c < DP)
-            for (int e = 0; e < 4; e++) s_part[warp][2 + c + e] = A[e];
-        if (lane == 0) s_part[warp][0] = L;
+        if (d < Dh) *reinterpret_cast<float4 *>(&s_part[warp][d]) = make_float4(A[0], A[1], A[2], A[3]);
+        if (lane == 0) s_ml[warp] = make_float2(M, L);
         __syncthreads();
         if (warp) return;
+        M = kLowest;
 #pragma unroll
-        for (int w = 1; w < W; w++) {
-            L += s_part[w][0];
-            if (c < DP)
-                for (int e = 0; e < 4; e++) A[e] += s_part[w][2 + c + e];
+        for (int w = 0; w < W; w++) M = fmaxf(M, s_ml[w].x);
+        L = A[0] = A[1] = A[2] = A[3] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            const float f = exp2_fast(s_ml[w].x - M);
+            L += f * s_ml[w].y;
+            if (d < Dh)
+#pragma unroll
+                for (int e = 0; e < 4; e++) A[e] += f * s_part[w][d + e];
         }
     }
-    T *o = (T *)P.a.out + ((int64_t)(sq.n0 + t) * H + h) * Dh;
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        const int d = ((c + e) & 7) * (DP / 8) + ((c + e) >> 3);
-        if (c < DP && d < Dh) o[d] = (T)(L == 0.0f ? 0.0f : A[e] / L);
-    }
+    // rows outside the step (a sequence out of bounds among them) do not exist
+    if (d < Dh && n0 >= 0 && n1 <= P.b.n_tokens && n1 - n0 <= P.b.max_new && t < n1 - n0)
+        put_row((T *)P.a.out + ((int64_t)(n0 + t) * H + h) * Dh + d, A, L);
 }
 
 struct K8Plan {
     int G, rt, row_tiles, splits, chunk;   // rt: rows of a tile
-    size_t bytes;
+    size_t cells, bytes;
 };
 
 // Chunks: one wave of equal chunks over all CTA slots while that leaves a
@@ -812,7 +828,8 @@ static K8Plan k8_plan(const SepiaKv8Cache &c, const SepiaKv8Step &b, const Sepia
     const int64_t one = (groups * span + slots - 1) / slots;
     p.chunk = (int)(std::min(kMaxChunk, std::max<int64_t>(one, 1)) + kUnit - 1) / kUnit * kUnit;
     p.splits = (int)std::max<int64_t>(1, (span + p.chunk - 1) / p.chunk);
-    p.bytes = p.splits > 1 ? (size_t)groups * p.splits * rt * ((c.head_dim <= 64 ? 64 : 128) + 2) * 4 : 0;
+    p.cells = p.splits > 1 ? (size_t)groups * p.splits * rt : 0;
+    p.bytes = p.cells * (c.head_dim * 4 + 8);
     return p;
 }
 
@@ -827,8 +844,8 @@ static int k8_launch(const K8Params &P, cudaStream_t st) {
     if (P.splits == 1) return 1;
     // one warp per row while a row has few chunks, four beyond
     const dim3 g1((unsigned)((rows + kK8Warps - 1) / kK8Warps), (unsigned)P.b.n_seqs), g4((unsigned)rows, (unsigned)P.b.n_seqs);
-    const cudaError_t e = P.splits <= 8 ? launch_pdl(k_kv8_merge<T, DP, NB, 1>, g1, dim3(kK8Threads), 0, st, P)
-                                        : launch_pdl(k_kv8_merge<T, DP, NB, 4>, g4, dim3(kK8Threads), 0, st, P);
+    const cudaError_t e = P.splits <= 8 ? launch_pdl(k_kv8_merge<T, NB, 1>, g1, dim3(kK8Threads), 0, st, P)
+                                        : launch_pdl(k_kv8_merge<T, NB, 4>, g4, dim3(kK8Threads), 0, st, P);
     return check(e, "kv8_attn merge launch");
 }
 
@@ -873,6 +890,7 @@ extern "C" int sepia_cuda_kv8_attn(const SepiaKv8Cache *c, const SepiaKv8Step *b
     if (!k8_check(c, b, a)) return 0;
     if (b->n_seqs == 0 || b->n_tokens == 0 || b->max_new == 0) return 1;
     if (!a->q || !a->out) return fail("%s: null q or out", what);
+    if (reinterpret_cast<uintptr_t>(a->out) & (a->x_f16 ? 7 : 15)) return fail("%s: out must be aligned to 4 elements", what);
     if (a->q_stride < (int64_t)a->n_heads * c->head_dim) return fail("%s: q_stride is shorter than a token", what);
     if (a->rel_extent && !a->rel_logits) return fail("%s: rel_extent without rel_logits", what);
     const K8Plan p = k8_plan(*c, *b, *a);
@@ -890,6 +908,7 @@ extern "C" int sepia_cuda_kv8_attn(const SepiaKv8Cache *c, const SepiaKv8Step *b
     const int64_t q_b = a->x_f16 ? 8 : 16, q_sz = a->x_f16 ? 2 : 4;
     P.q_vec = reinterpret_cast<uintptr_t>(a->q) % q_b == 0 && a->q_stride * q_sz % q_b == 0;
     P.part = (float *)ws;
+    P.part_ml = (float2 *)(P.part + p.cells * c->head_dim);
     P.err = dev_info().err;
     cudaStream_t st = as_stream(stream);
     return a->x_f16 ? k8_launch_dim<__half>(P, p.rt, st) : k8_launch_dim<float>(P, p.rt, st);
