@@ -315,7 +315,7 @@ int sepia_cuda_kv8_attn(const SepiaKv8Cache *c, const SepiaKv8Step *b, const Sep
  * the result does not depend on the order of summation. NaN logits count as
  * -infinity; a row without any finite or +infinite logit gives id -1 and
  * prob 0. prob (may be NULL): the drawn token's share of the weights in.
- * vocab at most 2^22. */
+ * vocab at most 2^19. */
 int sepia_cuda_sample(int x_f16, const void *logits, int64_t stride, int32_t rows, int32_t vocab, const float *u,
                       const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
                       int32_t *ids, float *prob, void *stream);

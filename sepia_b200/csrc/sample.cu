@@ -3,25 +3,41 @@
 // definition in include/sepia_cuda.h).
 //
 // Each filter keeps a prefix of one order (greater logit first, then lower
-// index), so a row's set is described by a cut: the logit of the last token
-// in, and how many of the tokens with that very logit are in. Weights are
-// integers: counts and masses are sums that no order of summation changes.
+// index), so a row's set is described by a cut: the last token in. Weights
+// are integers: counts and masses are sums that no order of summation changes.
+//
+// The logits cross HBM once: a cluster of up to 8 CTAs holds a row in shared
+// memory, and all passes run there. A cut is found by a histogram over
+// (max - l)/T with linear bins (logits spread over them, so that few lanes
+// meet in one counter), whose threshold bin is gathered and sorted by the
+// cluster's first CTA. A bin that is too full for that (runs of equal logits)
+// is cut by halving the range of keys, 32 passes.
 #include "../../include/sepia_cuda.h"
 #include "common.cuh"
 #include "runtime.h"
 
+#include <cooperative_groups.h>
+
+namespace cg = cooperative_groups;
+
 namespace sepia {
 
-constexpr int kSmThreads = 1024;
+constexpr int kSmThreads = 512;
+constexpr int kSmBins = 1024;                // two per thread
+constexpr int kSmList = 1024;                // tokens of a threshold bin that are sorted
+constexpr int kSmMaxCluster = 8;
+constexpr float kSmRange = 22.25f;           // beyond exp(-this) a weight rounds to 0
 constexpr float kSmOne = 2147483648.0f;      // weight of the best token: 2^31
-constexpr int32_t kSmMaxVocab = 1 << 22;     // sums stay below 2^53: exact in fp64 too
+// 65536 logits a CTA: a bin's sums of 16-bit halves fit 32 bits, the row's mass is exact in fp64
+constexpr int32_t kSmMaxVocab = 1 << 19;
 
 typedef unsigned long long u64;
 
 struct SmParams {
     const void *logits;
     int64_t stride;
-    int32_t vocab;
+    int32_t vocab, slice;                    // slice: logits of a CTA, a multiple of 16
+    int32_t held;                            // the slice fits in shared memory
     const float *u, *temperature, *top_p, *min_p;
     const int32_t *top_k;
     int32_t *ids;
@@ -43,6 +59,26 @@ __device__ __forceinline__ float sm_exp(float l, float best, float inv_t) {
 }
 __device__ __forceinline__ u64 sm_weight(float e) { return (u64)__float2uint_rn(e * kSmOne); }
 
+// The last token in (all of them: key 0)
+struct SmCut {
+    uint32_t key, idx;
+};
+__device__ __forceinline__ bool sm_in(const SmCut &c, uint32_t key, uint32_t idx) {
+    return key > c.key || (key == c.key && idx <= c.idx);
+}
+
+struct SmShared {
+    union {                                  // the list is filled when the bins have been read
+        uint32_t hist[2][kSmBins];           // counts, or masses as sums of low and high 16 bits
+        u64 list[kSmList];                   // key, complement of the index
+    };
+    u64 best[kSmMaxCluster], sums[2][kSmMaxCluster], warp[kSmThreads / 32];
+    u64 found_before;                        // count or mass of the bins above the threshold bin
+    double thr;
+    int bin, n_list;                         // bin: -1 no cut; n_list may pass kSmList
+    SmCut cut;
+};
+
 __device__ u64 sm_block_sum(u64 v, u64 *sh) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -50,7 +86,7 @@ __device__ u64 sm_block_sum(u64 v, u64 *sh) {
     __syncthreads();
     if (lane == 0) sh[warp] = v;
     __syncthreads();
-    v = sh[lane];
+    v = lane < kSmThreads / 32 ? sh[lane] : 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
@@ -67,124 +103,341 @@ __device__ u64 sm_block_before(u64 v, u64 *sh) {
     __syncthreads();
     if (lane == 31) sh[warp] = x;
     __syncthreads();
-    u64 w = lane < warp ? sh[lane] : 0;
+    u64 w = lane < warp && lane < kSmThreads / 32 ? sh[lane] : 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
     return w + x - v;
 }
 
-// One CTA per row; every cut is found bit by bit over the key.
+// f(logit, index in the row) for every logit of the slice, 16 bytes a load
+// where the pointer allows. x: first logit of the slice, n of them from i0.
+template <typename T, typename F>
+__device__ __forceinline__ void sm_each(const T *x, int n, int i0, F f) {
+    constexpr int E = 16 / (int)sizeof(T);
+    const int head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
+    const int body = (n - head) / E;
+    for (int i = threadIdx.x; i < body; i += kSmThreads) {
+        const uint4 raw = *reinterpret_cast<const uint4 *>(x + head + i * E);
+        const T *v = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+        for (int e = 0; e < E; e++) f((float)v[e], i0 + head + i * E + e);
+    }
+    const int rest = head + n - (head + body * E);     // before and after the aligned part
+    if ((int)threadIdx.x < rest) {
+        const int i = (int)threadIdx.x < head ? (int)threadIdx.x : body * E + (int)threadIdx.x;
+        f((float)x[i], i0 + i);
+    }
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kSmThreads) k_sample(const SmParams P) {
-    __shared__ u64 sh[32];
-    const int row = blockIdx.x, tid = threadIdx.x, V = P.vocab;
+__global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
+    extern __shared__ __align__(16) uint8_t sm_raw[];
+    __shared__ SmShared S;
+    cg::cluster_group cl = cg::this_cluster();
+    const int C = cl.num_blocks(), rank = cl.block_rank();
+    const int row = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, V = P.vocab;
+    SmShared *first = cl.map_shared_rank(&S, 0);
     griddep_wait();
     griddep_launch();
-    const T *x = (const T *)P.logits + (int64_t)row * P.stride;
-    if (tid == 0) {
-        P.ids[row] = -1;
-        if (P.prob) P.prob[row] = 0.0f;
-    }
+    const int i0 = min(V, rank * P.slice), n = min(V, i0 + P.slice) - i0;
+    const T *gx = (const T *)P.logits + (int64_t)row * P.stride + i0;
+    // the slice in shared memory keeps the row's place between 16-byte boundaries
+    T *hx = reinterpret_cast<T *>(sm_raw + (reinterpret_cast<uintptr_t>(gx) & 15));
+    const T *x = P.held ? hx : gx;
+    const float t = P.temperature ? P.temperature[row] : 1.0f;
+    const int k = P.top_k ? P.top_k[row] : 0;
+    const float p = P.top_p ? P.top_p[row] : 1.0f;
+    const float mp = P.min_p && P.min_p[row] > 0.0f ? fminf(P.min_p[row], 1.0f) : 0.0f, u = P.u[row];
+
+    // ---- the row into shared memory; its best token ----
     u64 best = 0;
-    for (int i = tid; i < V; i += kSmThreads) {
-        const u64 k = ((u64)sm_key((float)x[i]) << 32) | (0xffffffffu - (uint32_t)i);
-        best = k > best ? k : best;
+    auto meet = [&](float l, int i) {
+        const u64 key = ((u64)sm_key(l) << 32) | (0xffffffffu - (uint32_t)i);
+        best = key > best ? key : best;
+    };
+    {
+        constexpr int E = 16 / (int)sizeof(T), kAhead = 8;
+        const int head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(gx) & 15)) & 15) / (int)sizeof(T));
+        const int body = (n - head) / E;
+        for (int i = tid; i < body; i += kAhead * kSmThreads) {
+            uint4 raw[kAhead];
+#pragma unroll
+            for (int a = 0; a < kAhead; a++)
+                raw[a] = __ldg(reinterpret_cast<const uint4 *>(gx + head + min(i + a * kSmThreads, body - 1) * E));
+#pragma unroll
+            for (int a = 0; a < kAhead; a++) {
+                const int j = i + a * kSmThreads;
+                if (j >= body) break;
+                if (P.held) *reinterpret_cast<uint4 *>(hx + head + j * E) = raw[a];
+                const T *v = reinterpret_cast<const T *>(&raw[a]);
+#pragma unroll
+                for (int e = 0; e < E; e++) meet((float)v[e], i0 + head + j * E + e);
+            }
+        }
+        const int rest = n - body * E;
+        if (tid < rest) {
+            const int i = tid < head ? tid : body * E + tid;
+            const T v = gx[i];
+            if (P.held) hx[i] = v;
+            meet((float)v, i0 + i);
+        }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        const u64 t = __shfl_xor_sync(0xffffffffu, best, o);
-        best = t > best ? t : best;
+        const u64 y = __shfl_xor_sync(0xffffffffu, best, o);
+        best = y > best ? y : best;
     }
-    if ((tid & 31) == 0) sh[tid >> 5] = best;
+    if (lane == 0) S.warp[tid >> 5] = best;
     __syncthreads();
-    for (int w = 0; w < 32; w++) best = sh[w] > best ? sh[w] : best;
-    __syncthreads();
+    if (tid < C) {
+        for (int w = 0; w < kSmThreads / 32; w++) best = S.warp[w] > best ? S.warp[w] : best;
+        cl.map_shared_rank(&S, tid)->best[rank] = best;
+    }
+    cl.sync();
+    best = 0;
+    for (int r = 0; r < C; r++) best = S.best[r] > best ? S.best[r] : best;
     const float top = sm_unkey((uint32_t)(best >> 32));
-    if (top == -INFINITY) return;
-    const float t = P.temperature ? P.temperature[row] : 1.0f;
-    if (!(t > 0.0f)) {
-        if (tid == 0) {
-            P.ids[row] = (int32_t)(0xffffffffu - (uint32_t)best);
-            if (P.prob) P.prob[row] = 1.0f;
+    const uint32_t best_idx = 0xffffffffu - (uint32_t)best;
+    if (top == -INFINITY || !(t > 0.0f)) {
+        if (rank == 0 && tid == 0) {
+            P.ids[row] = top == -INFINITY ? -1 : (int32_t)best_idx;
+            if (P.prob) P.prob[row] = top == -INFINITY ? 0.0f : 1.0f;
         }
         return;
     }
     const float inv_t = __fdiv_rn(1.0f, t);
-    const int k = P.top_k ? P.top_k[row] : 0;
-    const float p = P.top_p ? P.top_p[row] : 1.0f;
-    const float mp = P.min_p ? fminf(P.min_p[row], 1.0f) : 0.0f;
-    uint32_t cut = 0;                 // kept: key > cut, and the first `ties` tokens of key == cut
-    u64 ties = (u64)V;
-    auto sum_ge = [&](uint32_t key, bool mass) {
-        u64 s = 0;
-        for (int i = tid; i < V; i += kSmThreads) {
-            const float l = (float)x[i];
-            if (sm_key(l) >= key) s += mass ? sm_weight(sm_exp(l, top, inv_t)) : 1;
+
+    // ---- sums over the whole row: every CTA tells all ----
+    int turn = 0;
+    auto cluster_sum = [&](u64 v, u64 *mine_before) {
+        const u64 s = sm_block_sum(v, S.warp);
+        if (tid < C) cl.map_shared_rank(&S, tid)->sums[turn][rank] = s;
+        cl.sync();
+        u64 all = 0, before = 0;
+        for (int r = 0; r < C; r++) {
+            before += r < rank ? S.sums[turn][r] : 0;
+            all += S.sums[turn][r];
         }
-        return sm_block_sum(s, sh);
+        turn ^= 1;                                     // the next sum must not overwrite what is still read
+        if (mine_before) *mine_before = before;
+        return all;
     };
-    u64 mass = 0;
-    if (k > 0 && k < V) {
-        for (int b = 31; b >= 0; b--) {
-            const uint32_t c = cut | (1u << b);
-            if (sum_ge(c, false) >= (u64)k) cut = c;
+    SmCut cut = {0u, 0xffffffffu};
+    // The cut at the token where the running count (of the order) reaches
+    // `want`, or the running mass reaches `want` times the mass of the tokens
+    // that are in. range: tokens with (max - l)/T beyond it cannot be the
+    // cut; their mass still counts.
+    auto find_cut = [&](bool mass, double want, float range) {
+        const float per = kSmBins / range;
+        for (int i = tid; i < 2 * kSmBins; i += kSmThreads) (&S.hist[0][0])[i] = 0;
+        if (tid == 0) S.n_list = 0;
+        __syncthreads();
+        u64 beyond = 0;
+        auto bin_of = [&](float l) { return l == top ? 0 : min(kSmBins - 1, (int)((top - l) * inv_t * per)); };
+        sm_each(x, n, i0, [&](float l, int i) {
+            const float far = (top - l) * inv_t;
+            if (!(far < kSmRange) && l != top) return;            // weight 0, or NaN
+            if (!sm_in(cut, sm_key(l), (uint32_t)i)) return;
+            if (!mass) {
+                atomicAdd(&S.hist[0][bin_of(l)], 1u);
+                return;
+            }
+            const uint32_t w = (uint32_t)sm_weight(sm_exp(l, top, inv_t));
+            if (far < range || l == top) {
+                const int b = bin_of(l);
+                atomicAdd(&S.hist[0][b], w & 0xffffu);
+                atomicAdd(&S.hist[1][b], w >> 16);
+            } else {
+                beyond += w;
+            }
+        });
+        const u64 far_mass = mass ? cluster_sum(beyond, nullptr) : 0;
+        if (!mass) cl.sync();
+        if (rank == 0) {                               // the threshold bin
+            u64 v[2] = {0, 0};
+            for (int r = 0; r < C; r++) {
+                const SmShared *q = cl.map_shared_rank(&S, r);
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    v[e] += (u64)q->hist[0][2 * tid + e] + (mass ? (u64)q->hist[1][2 * tid + e] << 16 : 0);
+            }
+            const u64 before = sm_block_before(v[0] + v[1], S.warp);
+            const u64 all = sm_block_sum(v[0] + v[1], S.warp);
+            const double thr = mass ? want * (double)(all + far_mass) : want;
+            if (tid == 0) S.bin = -1, S.thr = thr;
+            __syncthreads();
+            u64 b = before;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                if ((double)b < thr && (double)(b + v[e]) >= thr) S.bin = 2 * tid + e, S.found_before = b;
+                b += v[e];
+            }
+            __syncthreads();
+            if (tid > 0 && tid < C) {
+                SmShared *q = cl.map_shared_rank(&S, tid);
+                q->bin = S.bin;
+                q->thr = S.thr;
+                q->found_before = S.found_before;
+            }
         }
-        ties = (u64)k - (cut == 0xffffffffu ? 0 : sum_ge(cut + 1, false));
-    }
+        cl.sync();
+        const int bin = S.bin;
+        if (bin < 0) return;                           // a count past all tokens of any weight: nothing to cut
+        sm_each(x, n, i0, [&](float l, int i) {        // its tokens to the first CTA
+            const float far = (top - l) * inv_t;
+            if ((!(far < range) && l != top) || bin_of(l) != bin || !sm_in(cut, sm_key(l), (uint32_t)i)) return;
+            const int at = atomicAdd(&first->n_list, 1);
+            if (at < kSmList) first->list[at] = ((u64)sm_key(l) << 32) | (0xffffffffu - (uint32_t)i);
+        });
+        cl.sync();
+        const int have = first->n_list;
+        const double thr = S.thr;
+        const u64 above = S.found_before;
+        if (have <= kSmList) {
+            if (rank == 0) {                           // sorted by the order, then summed
+                int m = 2;
+                while (m < have) m <<= 1;
+                for (int i = have + tid; i < m; i += kSmThreads) S.list[i] = 0;
+                __syncthreads();
+                for (int size = 2; size <= m; size <<= 1)
+                    for (int step = size >> 1; step > 0; step >>= 1) {
+                        for (int i = tid; i < m / 2; i += kSmThreads) {
+                            const int a = 2 * i - (i & (step - 1)), b = a + step;
+                            const u64 va = S.list[a], vb = S.list[b];
+                            if ((va < vb) == ((a & size) == 0)) S.list[a] = vb, S.list[b] = va;
+                        }
+                        __syncthreads();
+                    }
+                u64 v[2] = {0, 0};
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    if (2 * tid + e < have)
+                        v[e] = mass ? sm_weight(sm_exp(sm_unkey((uint32_t)(S.list[2 * tid + e] >> 32)), top, inv_t)) : 1;
+                u64 b = above + sm_block_before(v[0] + v[1], S.warp);
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    if ((double)b < thr && (double)(b + v[e]) >= thr) {
+                        const u64 y = S.list[2 * tid + e];
+                        S.cut.key = (uint32_t)(y >> 32);
+                        S.cut.idx = 0xffffffffu - (uint32_t)y;
+                    }
+                    b += v[e];
+                }
+                __syncthreads();
+                if (tid > 0 && tid < C) cl.map_shared_rank(&S, tid)->cut = S.cut;
+            }
+            cl.sync();
+            cut = S.cut;
+            return;
+        }
+        // Too many for the list: the greatest key whose tokens and those above
+        // reach the threshold, bit by bit; then how many tokens of that very
+        // key are in, and the index of the last of them.
+        auto sum_ge = [&](uint32_t key, bool indexes, uint32_t upto) {
+            u64 s = 0;
+            sm_each(x, n, i0, [&](float l, int i) {
+                const uint32_t y = sm_key(l);
+                if (!sm_in(cut, y, (uint32_t)i)) return;
+                if (indexes ? y == key && (uint32_t)i <= upto : y >= key)
+                    s += mass && !indexes ? sm_weight(sm_exp(l, top, inv_t)) : 1;
+            });
+            return cluster_sum(s, nullptr);
+        };
+        uint32_t key = 0;
+        for (int b = 31; b >= 0; b--)
+            if ((double)sum_ge(key | (1u << b), false, 0) >= thr) key |= 1u << b;
+        const u64 over = sum_ge(key + 1, false, 0), w = mass ? sm_weight(sm_exp(sm_unkey(key), top, inv_t)) : 1;
+        u64 r = (u64)((thr - (double)over) / (double)w);
+        while (r > 0 && (double)(over + (r - 1) * w) >= thr) r--;
+        while ((double)(over + r * w) < thr) r++;
+        uint32_t lo = 0, hi = (uint32_t)V - 1;         // the smallest index that has r of them up to it
+        while (lo < hi) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if (sum_ge(key, true, mid) >= r) hi = mid;
+            else lo = mid + 1;
+        }
+        cl.sync();
+        cut.key = key;
+        cut.idx = lo;
+    };
+    if (k > 0 && k < V) find_cut(false, (double)k, kSmRange);
     if (!(p >= 1.0f)) {
-        const u64 w0 = sm_weight(sm_exp(sm_unkey(cut), top, inv_t));
-        mass = cut ? sum_ge(cut + 1, true) + ties * w0 : sum_ge(0, true);
-        const double thr = (double)p * (double)mass;
-        uint32_t c2 = 0;
-        for (int b = 31; b >= 0; b--) {
-            const uint32_t c = c2 | (1u << b);
-            if (c <= cut || (double)sum_ge(c, true) >= thr) c2 = c;
+        if (p > 0.0f) {
+            // Without top-k, tokens below (1 - p)/(2 V) of the best together weigh
+            // less than half of what lies behind the cut (the other half is room
+            // for rounded weights), so the bins need not reach that far.
+            const float q = 1.0f - p;
+            const bool narrow = !(k > 0 && k < V) && q >= 0.00390625f;
+            find_cut(true, (double)p, narrow ? fminf(kSmRange, logf(2.0f * (float)V / q)) : kSmRange);
+        } else {
+            cut.key = (uint32_t)(best >> 32);
+            cut.idx = best_idx;
         }
-        if (!(thr > 0.0)) c2 = (uint32_t)(best >> 32);
-        const u64 above = sum_ge(c2 + 1, true), w = sm_weight(sm_exp(sm_unkey(c2), top, inv_t));
-        u64 r = w && thr > (double)above ? (u64)((thr - (double)above) / (double)w) : 0;
-        while (r > 0 && (double)(above + (r - 1) * w) >= thr) r--;
-        while (w && (double)(above + r * w) < thr) r++;
-        if (r == 0) r = 1;
-        ties = c2 == cut && ties < r ? ties : r;
-        cut = c2;
     }
-    // the draw: threads own runs of the row in index order
-    const int len = (V + kSmThreads - 1) / kSmThreads;
-    const int i0 = min(V, tid * len), i1 = min(V, i0 + len);
-    u64 eq = 0;
-    for (int i = i0; i < i1; i++) eq += sm_key((float)x[i]) == cut;
-    const u64 eq0 = sm_block_before(eq, sh);
-    auto weight = [&](int i, u64 &seen) -> u64 {
-        const float l = (float)x[i];
-        const uint32_t key = sm_key(l);
+
+    // ---- the draw: the CTA, then the run of tokens, then the token ----
+    auto weight = [&](float l, int i) -> u64 {
+        const float far = (top - l) * inv_t;
+        if ((!(far < kSmRange) && l != top) || !sm_in(cut, sm_key(l), (uint32_t)i)) return 0;
         const float e = sm_exp(l, top, inv_t);
-        bool in = key > cut;
-        if (key == cut) in = seen++ < ties;
-        if (mp > 0.0f) in = in && e >= mp;
-        return in ? sm_weight(e) : 0;
+        return mp > 0.0f && !(e >= mp) ? 0 : sm_weight(e);
     };
-    u64 sum = 0, seen = eq0;
-    for (int i = i0; i < i1; i++) sum += weight(i, seen);
-    const u64 before = sm_block_before(sum, sh);
-    const u64 total = sm_block_sum(sum, sh);
-    const float u = P.u[row];
+    u64 sum = 0, before;
+    sm_each(x, n, i0, [&](float l, int i) { sum += weight(l, i); });
+    const u64 total = cluster_sum(sum, &before);
     const double at = floor((double)u * (double)total);
     u64 target = at > 0.0 ? (u64)at : 0;
     target = target < total ? target : total - 1;
+    const u64 here = S.sums[turn ^ 1][rank];
+    if (target < before || target >= before + here) return;
+    const int len = ((n + kSmThreads - 1) / kSmThreads) | 1;      // odd: a run a thread, no bank met twice
+    const int a = min(n, tid * len), b = min(n, a + len);
+    sum = 0;
+    for (int i = a; i < b; i++) sum += weight((float)x[i], i0 + i);
+    before += sm_block_before(sum, S.warp);
     if (before <= target && target < before + sum) {
         u64 run = before;
-        seen = eq0;
-        for (int i = i0; i < i1; i++) {
-            const u64 w = weight(i, seen);
+        for (int i = a; i < b; i++) {
+            const u64 w = weight((float)x[i], i0 + i);
             run += w;
             if (run > target) {
-                P.ids[row] = i;
+                P.ids[row] = i0 + i;
                 if (P.prob) P.prob[row] = (float)((double)w / (double)total);
                 break;
             }
         }
     }
+}
+
+// A cluster of C CTAs for each row: as few as hold the row with two CTAs an
+// SM, more while SMs would stand idle and a CTA keeps a few thousand logits.
+template <typename T>
+static int sm_launch(SmParams &P, int rows, cudaStream_t st) {
+    const int sms = dev_info().sm_count > 0 ? dev_info().sm_count : 148;
+    constexpr int kRoom = 115712 - (int)sizeof(SmShared) - 16;    // of half an SM
+    auto slice = [&](int c) { return (P.vocab + c - 1) / c + 15 & ~15; };
+    int C = 1;
+    while (C < kSmMaxCluster && ((int64_t)slice(C) * (int)sizeof(T) > kRoom || (rows * C < sms && slice(C) > 4096))) C *= 2;
+    P.slice = slice(C);
+    const int64_t bytes = (int64_t)P.slice * (int)sizeof(T) + 16;
+    P.held = bytes + (int)sizeof(SmShared) + 1024 <= dev_info().smem_optin;
+    const int smem = P.held ? (int)bytes : 0;
+    if (smem && !ensure_smem((const void *)k_sample<T>, smem)) return 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(rows * C));
+    cfg.blockDim = dim3(kSmThreads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)C;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    return check(cudaLaunchKernelEx(&cfg, k_sample<T>, P), "sample launch");
 }
 
 }  // namespace sepia
@@ -199,6 +452,8 @@ extern "C" int sepia_cuda_sample(int x_f16, const void *logits, int64_t stride, 
         return fail("%s: %d rows of %d logits (1 to %d)", what, rows, vocab, kSmMaxVocab);
     if (rows == 0) return 1;
     if (!logits || !u || !ids) return fail("%s: null pointer", what);
+    if (rows > INT32_MAX / kSmMaxCluster) return fail("%s: %d rows are too many", what, rows);
+    if (reinterpret_cast<uintptr_t>(logits) % (x_f16 ? 2 : 4)) return fail("%s: logits are not aligned", what);
     if (stride < vocab) return fail("%s: row stride %lld is shorter than %d", what, (long long)stride, vocab);
     SmParams P;
     P.logits = logits;
@@ -211,7 +466,5 @@ extern "C" int sepia_cuda_sample(int x_f16, const void *logits, int64_t stride, 
     P.top_k = top_k;
     P.ids = ids;
     P.prob = prob;
-    const cudaError_t e = x_f16 ? launch_pdl(k_sample<__half>, (unsigned)rows, kSmThreads, 0, as_stream(stream), P)
-                                : launch_pdl(k_sample<float>, (unsigned)rows, kSmThreads, 0, as_stream(stream), P);
-    return check(e, "sample launch");
+    return x_f16 ? sm_launch<__half>(P, rows, as_stream(stream)) : sm_launch<float>(P, rows, as_stream(stream));
 }
