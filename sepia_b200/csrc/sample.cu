@@ -59,20 +59,21 @@ __device__ __forceinline__ float sm_exp(float l, float best, float inv_t) {
 }
 __device__ __forceinline__ u64 sm_weight(float e) { return (u64)__float2uint_rn(e * kSmOne); }
 
-// The last token in (all of them: key 0)
+// The last token in
 struct SmCut {
-    uint32_t key, idx;
+    float l;
+    int idx;
 };
-__device__ __forceinline__ bool sm_in(const SmCut &c, uint32_t key, uint32_t idx) {
-    return key > c.key || (key == c.key && idx <= c.idx);
-}
 
 struct SmShared {
     union {                                  // the list is filled when the bins have been read
         uint32_t hist[2][kSmBins];           // counts, or masses as sums of low and high 16 bits
         u64 list[kSmList];                   // key, complement of the index
     };
-    u64 best[kSmMaxCluster], sums[2][kSmMaxCluster], warp[kSmThreads / 32];
+    float best[kSmMaxCluster];
+    int best_idx[kSmMaxCluster];
+    u64 sums[2][kSmMaxCluster], warp[kSmThreads / 32];
+    int first_idx;
     u64 found_before;                        // count or mass of the bins above the threshold bin
     double thr;
     int bin, n_list;                         // bin: -1 no cut; n_list may pass kSmList
@@ -149,12 +150,8 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
     const float p = P.top_p ? P.top_p[row] : 1.0f;
     const float mp = P.min_p && P.min_p[row] > 0.0f ? fminf(P.min_p[row], 1.0f) : 0.0f, u = P.u[row];
 
-    // ---- the row into shared memory; its best token ----
-    u64 best = 0;
-    auto meet = [&](float l, int i) {
-        const u64 key = ((u64)sm_key(l) << 32) | (0xffffffffu - (uint32_t)i);
-        best = key > best ? key : best;
-    };
+    // ---- the row into shared memory; its greatest logit ----
+    float top = -INFINITY;                             // NaN loses every fmaxf
     {
         constexpr int E = 16 / (int)sizeof(T), kAhead = 8;
         const int head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(gx) & 15)) & 15) / (int)sizeof(T));
@@ -166,12 +163,11 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
                 raw[a] = __ldg(reinterpret_cast<const uint4 *>(gx + head + min(i + a * kSmThreads, body - 1) * E));
 #pragma unroll
             for (int a = 0; a < kAhead; a++) {
-                const int j = i + a * kSmThreads;
-                if (j >= body) break;
+                const int j = min(i + a * kSmThreads, body - 1);
                 if (P.held) *reinterpret_cast<uint4 *>(hx + head + j * E) = raw[a];
                 const T *v = reinterpret_cast<const T *>(&raw[a]);
 #pragma unroll
-                for (int e = 0; e < E; e++) meet((float)v[e], i0 + head + j * E + e);
+                for (int e = 0; e < E; e++) top = fmaxf(top, (float)v[e]);
             }
         }
         const int rest = n - body * E;
@@ -179,29 +175,43 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
             const int i = tid < head ? tid : body * E + tid;
             const T v = gx[i];
             if (P.held) hx[i] = v;
-            meet((float)v, i0 + i);
+            top = fmaxf(top, (float)v);
         }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const u64 y = __shfl_xor_sync(0xffffffffu, best, o);
-        best = y > best ? y : best;
-    }
-    if (lane == 0) S.warp[tid >> 5] = best;
+    top = warp_max(top);
+    if (lane == 0) reinterpret_cast<float *>(S.warp)[tid >> 5] = top;
+    if (tid == 0) S.first_idx = INT32_MAX;
     __syncthreads();
     if (tid < C) {
-        for (int w = 0; w < kSmThreads / 32; w++) best = S.warp[w] > best ? S.warp[w] : best;
-        cl.map_shared_rank(&S, tid)->best[rank] = best;
+        for (int w = 0; w < kSmThreads / 32; w++) top = fmaxf(top, reinterpret_cast<float *>(S.warp)[w]);
+        cl.map_shared_rank(&S, tid)->best[rank] = top;
     }
     cl.sync();
-    best = 0;
-    for (int r = 0; r < C; r++) best = S.best[r] > best ? S.best[r] : best;
-    const float top = sm_unkey((uint32_t)(best >> 32));
-    const uint32_t best_idx = 0xffffffffu - (uint32_t)best;
-    if (top == -INFINITY || !(t > 0.0f)) {
+    top = S.best[0];
+    for (int r = 1; r < C; r++) top = fmaxf(top, S.best[r]);
+    if (top == -INFINITY) {
         if (rank == 0 && tid == 0) {
-            P.ids[row] = top == -INFINITY ? -1 : (int32_t)best_idx;
-            if (P.prob) P.prob[row] = top == -INFINITY ? 0.0f : 1.0f;
+            P.ids[row] = -1;
+            if (P.prob) P.prob[row] = 0.0f;
+        }
+        return;
+    }
+    auto first_best = [&]() {                          // the lowest index of the greatest logit
+        sm_each(x, n, i0, [&](float l, int i) {
+            if (l == top) atomicMin(&S.first_idx, i);
+        });
+        __syncthreads();
+        if (tid < C) cl.map_shared_rank(&S, tid)->best_idx[rank] = S.first_idx;
+        cl.sync();
+        int i = S.best_idx[0];
+        for (int r = 1; r < C; r++) i = min(i, S.best_idx[r]);
+        return i;
+    };
+    if (!(t > 0.0f)) {
+        const int i = first_best();
+        if (rank == 0 && tid == 0) {
+            P.ids[row] = i;
+            if (P.prob) P.prob[row] = 1.0f;
         }
         return;
     }
@@ -222,28 +232,29 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
         if (mine_before) *mine_before = before;
         return all;
     };
-    SmCut cut = {0u, 0xffffffffu};
+    // Below this a weight rounds to 0: rounding of the bound itself cannot
+    // pass a logit at less than the range (both are fp32 numbers).
+    const float floor_l = top - kSmRange * t;
+    SmCut cut = {floor_l, INT32_MAX};                  // tokens in: l > cut.l, or l == cut.l up to an index
     // The cut at the token where the running count (of the order) reaches
     // `want`, or the running mass reaches `want` times the mass of the tokens
     // that are in. range: tokens with (max - l)/T beyond it cannot be the
     // cut; their mass still counts.
     auto find_cut = [&](bool mass, double want, float range) {
-        const float per = kSmBins / range;
+        const float per = kSmBins / range, near = range < kSmRange ? fmaxf(cut.l, top - range * t) : cut.l;
         for (int i = tid; i < 2 * kSmBins; i += kSmThreads) (&S.hist[0][0])[i] = 0;
         if (tid == 0) S.n_list = 0;
         __syncthreads();
         u64 beyond = 0;
-        auto bin_of = [&](float l) { return l == top ? 0 : min(kSmBins - 1, (int)((top - l) * inv_t * per)); };
+        auto bin_of = [&](float l) { return min(kSmBins - 1, (int)((top - l) * inv_t * per)); };   // inf - inf: 0
         sm_each(x, n, i0, [&](float l, int i) {
-            const float far = (top - l) * inv_t;
-            if (!(far < kSmRange) && l != top) return;            // weight 0, or NaN
-            if (!sm_in(cut, sm_key(l), (uint32_t)i)) return;
+            if (!(l >= cut.l) || (l == cut.l && i > cut.idx)) return;
             if (!mass) {
                 atomicAdd(&S.hist[0][bin_of(l)], 1u);
                 return;
             }
             const uint32_t w = (uint32_t)sm_weight(sm_exp(l, top, inv_t));
-            if (far < range || l == top) {
+            if (l >= near) {
                 const int b = bin_of(l);
                 atomicAdd(&S.hist[0][b], w & 0xffffu);
                 atomicAdd(&S.hist[1][b], w >> 16);
@@ -283,9 +294,10 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
         cl.sync();
         const int bin = S.bin;
         if (bin < 0) return;                           // a count past all tokens of any weight: nothing to cut
-        sm_each(x, n, i0, [&](float l, int i) {        // its tokens to the first CTA
-            const float far = (top - l) * inv_t;
-            if ((!(far < range) && l != top) || bin_of(l) != bin || !sm_in(cut, sm_key(l), (uint32_t)i)) return;
+        // its tokens to the first CTA; a bound of half a bin more spares most of them the bin's arithmetic
+        const float bin_lo = fmaxf(near, top - ((float)bin + 1.5f) / per * t), bin_hi = top - ((float)bin - 0.5f) / per * t;
+        sm_each(x, n, i0, [&](float l, int i) {
+            if (!(l >= bin_lo && (l <= bin_hi || bin == 0)) || bin_of(l) != bin || (l == cut.l && i > cut.idx)) return;
             const int at = atomicAdd(&first->n_list, 1);
             if (at < kSmList) first->list[at] = ((u64)sm_key(l) << 32) | (0xffffffffu - (uint32_t)i);
         });
@@ -318,8 +330,8 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
                 for (int e = 0; e < 2; e++) {
                     if ((double)b < thr && (double)(b + v[e]) >= thr) {
                         const u64 y = S.list[2 * tid + e];
-                        S.cut.key = (uint32_t)(y >> 32);
-                        S.cut.idx = 0xffffffffu - (uint32_t)y;
+                        S.cut.l = sm_unkey((uint32_t)(y >> 32));
+                        S.cut.idx = (int)(0xffffffffu - (uint32_t)y);
                     }
                     b += v[e];
                 }
@@ -336,8 +348,8 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
         auto sum_ge = [&](uint32_t key, bool indexes, uint32_t upto) {
             u64 s = 0;
             sm_each(x, n, i0, [&](float l, int i) {
+                if (!(l >= cut.l) || (l == cut.l && i > cut.idx)) return;
                 const uint32_t y = sm_key(l);
-                if (!sm_in(cut, y, (uint32_t)i)) return;
                 if (indexes ? y == key && (uint32_t)i <= upto : y >= key)
                     s += mass && !indexes ? sm_weight(sm_exp(l, top, inv_t)) : 1;
             });
@@ -357,8 +369,8 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
             else lo = mid + 1;
         }
         cl.sync();
-        cut.key = key;
-        cut.idx = lo;
+        cut.l = sm_unkey(key);
+        cut.idx = (int)lo;
     };
     if (k > 0 && k < V) find_cut(false, (double)k, kSmRange);
     if (!(p >= 1.0f)) {
@@ -370,15 +382,14 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
             const bool narrow = !(k > 0 && k < V) && q >= 0.00390625f;
             find_cut(true, (double)p, narrow ? fminf(kSmRange, logf(2.0f * (float)V / q)) : kSmRange);
         } else {
-            cut.key = (uint32_t)(best >> 32);
-            cut.idx = best_idx;
+            cut.l = top;
+            cut.idx = first_best();
         }
     }
 
     // ---- the draw: the CTA, then the run of tokens, then the token ----
     auto weight = [&](float l, int i) -> u64 {
-        const float far = (top - l) * inv_t;
-        if ((!(far < kSmRange) && l != top) || !sm_in(cut, sm_key(l), (uint32_t)i)) return 0;
+        if (!(l >= cut.l) || (l == cut.l && i > cut.idx)) return 0;
         const float e = sm_exp(l, top, inv_t);
         return mp > 0.0f && !(e >= mp) ? 0 : sm_weight(e);
     };
