@@ -9,9 +9,11 @@
 // The logits cross HBM once: a cluster of up to 8 CTAs holds a row in shared
 // memory, and all passes run there. A cut is found by a histogram over
 // (max - l)/T with linear bins (logits spread over them, so that few lanes
-// meet in one counter), whose threshold bin is gathered and sorted by the
-// cluster's first CTA. A bin that is too full for that (runs of equal logits)
-// is cut by halving the range of keys, 32 passes.
+// meet in one counter); the threshold bin is gathered in the cluster's first
+// CTA, split by a second histogram and the rest sorted. A bin that is too full
+// for that (runs of equal logits) is cut by halving the range of keys, 32
+// passes. Time goes into instructions, some 35 for each logit that has a
+// weight, most of them the exponential and its place in the histogram.
 #include "../../include/sepia_cuda.h"
 #include "common.cuh"
 #include "runtime.h"
@@ -53,9 +55,9 @@ __device__ __forceinline__ uint32_t sm_key(float v) {
 __device__ __forceinline__ float sm_unkey(uint32_t k) {
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
-// e = exp((l - max)/T); the best token's is 1 also where max is infinite
+// e = exp((l - max)/T); the best token's is 1 also where max is infinite (the least of NaN and 0 is 0)
 __device__ __forceinline__ float sm_exp(float l, float best, float inv_t) {
-    return l == best ? 1.0f : expf((l - best) * inv_t);
+    return expf(fminf(l - best, 0.0f) * inv_t);
 }
 __device__ __forceinline__ u64 sm_weight(float e) { return (u64)__float2uint_rn(e * kSmOne); }
 
@@ -73,9 +75,9 @@ struct SmShared {
     float best[kSmMaxCluster];
     int best_idx[kSmMaxCluster];
     u64 sums[2][kSmMaxCluster], warp[kSmThreads / 32];
-    int first_idx;
+    int first_idx, n_short;
+    u64 short_list[32];                      // tokens of the threshold's part of the bin
     u64 found_before;                        // count or mass of the bins above the threshold bin
-    double thr;
     int bin, n_list;                         // bin: -1 no cut; n_list may pass kSmList
     SmCut cut;
 };
@@ -110,25 +112,52 @@ __device__ u64 sm_block_before(u64 v, u64 *sh) {
     return w + x - v;
 }
 
-// f(logit, index in the row) for every logit of the slice, 16 bytes a load
-// where the pointer allows. x: first logit of the slice, n of them from i0.
-template <typename T, typename F>
-__device__ __forceinline__ void sm_each(const T *x, int n, int i0, F f) {
-    constexpr int E = 16 / (int)sizeof(T);
-    const int head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
-    const int body = (n - head) / E;
-    for (int i = threadIdx.x; i < body; i += kSmThreads) {
-        const uint4 raw = *reinterpret_cast<const uint4 *>(x + head + i * E);
-        const T *v = reinterpret_cast<const T *>(&raw);
+// A slice in index order: logits before the first 16-byte boundary (warp 0
+// takes them), whole vectors (a run for each warp), the rest (the last warp).
+template <typename T>
+struct SmSlice {
+    static constexpr int E = 16 / (int)sizeof(T);
+    const T *x;
+    int n, i0, head, body, lo, hi;           // i0: the slice's first index in the row; lo, hi: this warp's vectors
+    __device__ __forceinline__ SmSlice(const T *x_, int n_, int i0_) : x(x_), n(n_), i0(i0_) {
+        const int warp = threadIdx.x >> 5;
+        head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T));
+        body = (n - head) / E;
+        const int run = (body + kSmThreads / 32 - 1) / (kSmThreads / 32);
+        lo = min(body, warp * run);
+        hi = min(body, lo + run);
+    }
+    __device__ __forceinline__ void load(int j, float (&v)[E]) const {
+        const uint4 raw = *reinterpret_cast<const uint4 *>(x + head + j * E);
+        const T *y = reinterpret_cast<const T *>(&raw);
 #pragma unroll
-        for (int e = 0; e < E; e++) f((float)v[e], i0 + head + i * E + e);
+        for (int e = 0; e < E; e++) v[e] = (float)y[e];
     }
-    const int rest = head + n - (head + body * E);     // before and after the aligned part
-    if ((int)threadIdx.x < rest) {
-        const int i = (int)threadIdx.x < head ? (int)threadIdx.x : body * E + (int)threadIdx.x;
-        f((float)x[i], i0 + i);
+    __device__ __forceinline__ int index(int j) const { return i0 + head + j * E; }
+    // The lane's logit (the others NaN) of the part before (0) or after (1) the vectors; its index, or -1
+    __device__ __forceinline__ int ragged(int part, float (&v)[E]) const {
+        const int lane = threadIdx.x & 31, at = part ? head + body * E + lane : lane;
+        const bool on = part ? (threadIdx.x >> 5) == kSmThreads / 32 - 1 && at < n : (threadIdx.x >> 5) == 0 && lane < head;
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = __int_as_float(0x7fffffff);
+        if (on) v[0] = (float)x[at];
+        return on ? i0 + at : -1;
     }
-}
+    // f(vector, index of its first logit) over the slice; NaN where there is none
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+        float v[E];
+        for (int j = lo + (threadIdx.x & 31); j < hi; j += 32) {
+            load(j, v);
+            f(v, index(j));
+        }
+#pragma unroll 1
+        for (int part = 0; part < 2; part++) {
+            const int i = ragged(part, v);
+            if (i >= 0) f(v, i);
+        }
+    }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
@@ -144,7 +173,8 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
     const T *gx = (const T *)P.logits + (int64_t)row * P.stride + i0;
     // the slice in shared memory keeps the row's place between 16-byte boundaries
     T *hx = reinterpret_cast<T *>(sm_raw + (reinterpret_cast<uintptr_t>(gx) & 15));
-    const T *x = P.held ? hx : gx;
+    constexpr int E = SmSlice<T>::E;
+    const SmSlice<T> X(P.held ? hx : gx, n, i0);
     const float t = P.temperature ? P.temperature[row] : 1.0f;
     const int k = P.top_k ? P.top_k[row] : 0;
     const float p = P.top_p ? P.top_p[row] : 1.0f;
@@ -153,22 +183,33 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
     // ---- the row into shared memory; its greatest logit ----
     float top = -INFINITY;                             // NaN loses every fmaxf
     {
-        constexpr int E = 16 / (int)sizeof(T), kAhead = 8;
+        constexpr int kAhead = 8;
         const int head = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(gx) & 15)) & 15) / (int)sizeof(T));
         const int body = (n - head) / E;
-        for (int i = tid; i < body; i += kAhead * kSmThreads) {
+        const uint4 *from = reinterpret_cast<const uint4 *>(gx + head) + tid;
+        uint4 *to = reinterpret_cast<uint4 *>(hx + head) + tid;
+        auto take = [&](int j, const uint4 &raw) {
+            if (P.held) to[j] = raw;
+            const T *v = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+            for (int e = 0; e < E; e++) top = fmaxf(top, (float)v[e]);
+        };
+        int j = 0;
+        for (; j + tid + (kAhead - 1) * kSmThreads < body; j += kAhead * kSmThreads) {
             uint4 raw[kAhead];
 #pragma unroll
-            for (int a = 0; a < kAhead; a++)
-                raw[a] = __ldg(reinterpret_cast<const uint4 *>(gx + head + min(i + a * kSmThreads, body - 1) * E));
+            for (int a = 0; a < kAhead; a++) raw[a] = __ldg(from + j + a * kSmThreads);
 #pragma unroll
-            for (int a = 0; a < kAhead; a++) {
-                const int j = min(i + a * kSmThreads, body - 1);
-                if (P.held) *reinterpret_cast<uint4 *>(hx + head + j * E) = raw[a];
-                const T *v = reinterpret_cast<const T *>(&raw[a]);
+            for (int a = 0; a < kAhead; a++) take(j + a * kSmThreads, raw[a]);
+        }
+        {
+            uint4 raw[kAhead - 1];                     // fewer than kAhead are left
 #pragma unroll
-                for (int e = 0; e < E; e++) top = fmaxf(top, (float)v[e]);
-            }
+            for (int a = 0; a < kAhead - 1; a++)
+                if (j + tid + a * kSmThreads < body) raw[a] = __ldg(from + j + a * kSmThreads);
+#pragma unroll
+            for (int a = 0; a < kAhead - 1; a++)
+                if (j + tid + a * kSmThreads < body) take(j + a * kSmThreads, raw[a]);
         }
         const int rest = n - body * E;
         if (tid < rest) {
@@ -183,6 +224,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
     if (tid == 0) S.first_idx = INT32_MAX;
     __syncthreads();
     if (tid < C) {
+#pragma unroll
         for (int w = 0; w < kSmThreads / 32; w++) top = fmaxf(top, reinterpret_cast<float *>(S.warp)[w]);
         cl.map_shared_rank(&S, tid)->best[rank] = top;
     }
@@ -197,8 +239,10 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
         return;
     }
     auto first_best = [&]() {                          // the lowest index of the greatest logit
-        sm_each(x, n, i0, [&](float l, int i) {
-            if (l == top) atomicMin(&S.first_idx, i);
+        X.each([&](const float (&v)[E], int i) {
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (v[e] == top) atomicMin(&S.first_idx, i + e);
         });
         __syncthreads();
         if (tid < C) cl.map_shared_rank(&S, tid)->best_idx[rank] = S.first_idx;
@@ -236,104 +280,201 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
     // pass a logit at less than the range (both are fp32 numbers).
     const float floor_l = top - kSmRange * t;
     SmCut cut = {floor_l, INT32_MAX};                  // tokens in: l > cut.l, or l == cut.l up to an index
+    auto in = [&](float l, int i) { return l >= cut.l && !(l == cut.l && i > cut.idx); };
+    // Weights of a vector's tokens that are in, 0 for the others; false: all 0
+    auto weigh = [&](const float (&v)[E], int i, uint32_t (&w)[E]) {
+        float most = v[0];
+#pragma unroll
+        for (int e = 1; e < E; e++) most = fmaxf(most, v[e]);
+        if (!(most >= cut.l)) return false;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const uint32_t y = __float2uint_rn(sm_exp(v[e], top, inv_t) * kSmOne);
+            w[e] = v[e] >= cut.l ? y : 0u;
+        }
+        if (cut.idx != INT32_MAX) {                    // the whole cluster
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (v[e] == cut.l && i + e > cut.idx) w[e] = 0u;
+        }
+        return true;
+    };
     // The cut at the token where the running count (of the order) reaches
     // `want`, or the running mass reaches `want` times the mass of the tokens
     // that are in. range: tokens with (max - l)/T beyond it cannot be the
     // cut; their mass still counts.
     auto find_cut = [&](bool mass, double want, float range) {
-        const float per = kSmBins / range, near = range < kSmRange ? fmaxf(cut.l, top - range * t) : cut.l;
+        const float per = kSmBins / range * inv_t, near = range < kSmRange ? fmaxf(cut.l, top - range * t) : cut.l;
         for (int i = tid; i < 2 * kSmBins; i += kSmThreads) (&S.hist[0][0])[i] = 0;
         if (tid == 0) S.n_list = 0;
         __syncthreads();
         u64 beyond = 0;
-        auto bin_of = [&](float l) { return min(kSmBins - 1, (int)((top - l) * inv_t * per)); };   // inf - inf: 0
-        sm_each(x, n, i0, [&](float l, int i) {
-            if (!(l >= cut.l) || (l == cut.l && i > cut.idx)) return;
+        auto place_of = [&](float l) { return (top - l) * per; };       // NaN where both are infinite: bin 0
+        auto bin_of = [&](float l) { return min(kSmBins - 1, (int)place_of(l)); };
+        X.each([&](const float (&v)[E], int i) {
             if (!mass) {
-                atomicAdd(&S.hist[0][bin_of(l)], 1u);
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (in(v[e], i + e)) atomicAdd(&S.hist[0][bin_of(v[e])], 1u);
                 return;
             }
-            const uint32_t w = (uint32_t)sm_weight(sm_exp(l, top, inv_t));
-            if (l >= near) {
-                const int b = bin_of(l);
-                atomicAdd(&S.hist[0][b], w & 0xffffu);
-                atomicAdd(&S.hist[1][b], w >> 16);
-            } else {
-                beyond += w;
+            uint32_t w[E];
+            if (!weigh(v, i, w)) return;
+            if (range < kSmRange) {                    // such weights are below 2^31 (1 - p)/(2 V): E of them fit 32 bits
+                uint32_t far = 0;
+#pragma unroll
+                for (int e = 0; e < E; e++) far += v[e] < near ? w[e] : 0u;
+                beyond += far;
             }
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (v[e] >= near && w[e]) {
+                    const int b = bin_of(v[e]);
+                    atomicAdd(&S.hist[0][b], w[e] & 0xffffu);
+                    atomicAdd(&S.hist[1][b], w[e] >> 16);
+                }
         });
         const u64 far_mass = mass ? cluster_sum(beyond, nullptr) : 0;
         if (!mass) cl.sync();
-        if (rank == 0) {                               // the threshold bin
-            u64 v[2] = {0, 0};
-            for (int r = 0; r < C; r++) {
-                const SmShared *q = cl.map_shared_rank(&S, r);
+        // The threshold bin: each CTA adds its share of the bins over the cluster
+        const int share = kSmBins / C;                 // bins of a CTA, up to two a thread
+        u64 v[2] = {0, 0};
 #pragma unroll
-                for (int e = 0; e < 2; e++)
-                    v[e] += (u64)q->hist[0][2 * tid + e] + (mass ? (u64)q->hist[1][2 * tid + e] << 16 : 0);
-            }
-            const u64 before = sm_block_before(v[0] + v[1], S.warp);
-            const u64 all = sm_block_sum(v[0] + v[1], S.warp);
-            const double thr = mass ? want * (double)(all + far_mass) : want;
-            if (tid == 0) S.bin = -1, S.thr = thr;
-            __syncthreads();
-            u64 b = before;
+        for (int e = 0; e < 2; e++)
+            if (tid + e * kSmThreads < share) {
+                // thread order is bin order: with two bins a thread they are neighbours
+                const int b = rank * share + (share > kSmThreads ? 2 * tid + e : tid);
+                uint32_t x[kSmMaxCluster][2];
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                if ((double)b < thr && (double)(b + v[e]) >= thr) S.bin = 2 * tid + e, S.found_before = b;
-                b += v[e];
+                for (int r = 0; r < kSmMaxCluster; r++) {
+                    const SmShared *q = cl.map_shared_rank(&S, r < C ? r : 0);
+                    x[r][0] = r < C ? q->hist[0][b] : 0;
+                    x[r][1] = r < C && mass ? q->hist[1][b] : 0;
+                }
+#pragma unroll
+                for (int r = 0; r < kSmMaxCluster; r++) v[e] += (u64)x[r][0] + ((u64)x[r][1] << 16);
             }
-            __syncthreads();
-            if (tid > 0 && tid < C) {
-                SmShared *q = cl.map_shared_rank(&S, tid);
-                q->bin = S.bin;
-                q->thr = S.thr;
-                q->found_before = S.found_before;
-            }
+        u64 b = 0;
+        const u64 all = cluster_sum(v[0] + v[1], &b) + far_mass;
+        const double thr = mass ? want * (double)all : want;
+        b += sm_block_before(v[0] + v[1], S.warp);
+        if (tid == 0) S.bin = -1;
+        cl.sync();                                     // every CTA's bin is unset before one is found
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            if ((double)b < thr && (double)(b + v[e]) >= thr)
+                for (int r = 0; r < C; r++) {
+                    SmShared *q = cl.map_shared_rank(&S, r);
+                    q->bin = rank * share + (share > kSmThreads ? 2 * tid + e : tid);
+                    q->found_before = b;
+                }
+            b += v[e];
         }
         cl.sync();
         const int bin = S.bin;
         if (bin < 0) return;                           // a count past all tokens of any weight: nothing to cut
-        // its tokens to the first CTA; a bound of half a bin more spares most of them the bin's arithmetic
-        const float bin_lo = fmaxf(near, top - ((float)bin + 1.5f) / per * t), bin_hi = top - ((float)bin - 0.5f) / per * t;
-        sm_each(x, n, i0, [&](float l, int i) {
-            if (!(l >= bin_lo && (l <= bin_hi || bin == 0)) || bin_of(l) != bin || (l == cut.l && i > cut.idx)) return;
-            const int at = atomicAdd(&first->n_list, 1);
-            if (at < kSmList) first->list[at] = ((u64)sm_key(l) << 32) | (0xffffffffu - (uint32_t)i);
+        // its tokens to the first CTA; bounds of a bin more on either side spare most of them the bin's arithmetic
+        const float bin_lo = fmaxf(near, top - ((float)bin + 2.0f) / per), bin_hi = top - ((float)bin - 1.0f) / per;
+        const float mid = bin ? 0.5f * (bin_lo + bin_hi) : top, half = bin ? bin_hi - mid : top - bin_lo;
+        X.each([&](const float (&v)[E], int i) {
+            float d = fabsf(v[0] - mid);               // NaN at an infinite maximum: passes
+#pragma unroll
+            for (int e = 1; e < E; e++) d = fminf(d, fabsf(v[e] - mid));
+            if (d > half) return;
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (v[e] >= near && bin_of(v[e]) == bin && in(v[e], i + e)) {
+                    const int at = atomicAdd(&first->n_list, 1);
+                    if (at < kSmList) first->list[at] = ((u64)sm_key(v[e]) << 32) | (0xffffffffu - (uint32_t)(i + e));
+                }
         });
         cl.sync();
         const int have = first->n_list;
-        const double thr = S.thr;
         const u64 above = S.found_before;
         if (have <= kSmList) {
-            if (rank == 0) {                           // sorted by the order, then summed
-                int m = 2;
-                while (m < have) m <<= 1;
-                for (int i = have + tid; i < m; i += kSmThreads) S.list[i] = 0;
-                __syncthreads();
-                for (int size = 2; size <= m; size <<= 1)
-                    for (int step = size >> 1; step > 0; step >>= 1) {
-                        for (int i = tid; i < m / 2; i += kSmThreads) {
-                            const int a = 2 * i - (i & (step - 1)), b = a + step;
-                            const u64 va = S.list[a], vb = S.list[b];
-                            if ((va < vb) == ((a & size) == 0)) S.list[a] = vb, S.list[b] = va;
-                        }
-                        __syncthreads();
-                    }
-                u64 v[2] = {0, 0};
+            if (rank == 0) {
+                auto value = [&](u64 y) -> u64 {
+                    return !mass ? 1 : sm_weight(sm_exp(sm_unkey((uint32_t)(y >> 32)), top, inv_t));
+                };
+                // this thread's two tokens of the list, and their part of the bin
+                u64 y[2], val[2] = {0, 0}, over = above;
+                int part[2] = {-1, -1};
 #pragma unroll
                 for (int e = 0; e < 2; e++)
-                    if (2 * tid + e < have)
-                        v[e] = mass ? sm_weight(sm_exp(sm_unkey((uint32_t)(S.list[2 * tid + e] >> 32)), top, inv_t)) : 1;
-                u64 b = above + sm_block_before(v[0] + v[1], S.warp);
+                    if (tid + e * kSmThreads < have) {
+                        y[e] = S.list[tid + e * kSmThreads];
+                        val[e] = value(y[e]);
+                        part[e] = max(0, min(kSmBins - 1, (int)((place_of(sm_unkey((uint32_t)(y[e] >> 32))) - (float)bin) * kSmBins)));
+                    }
+                __syncthreads();                       // the list is read: its room becomes counters again
+                for (int i = tid; i < 2 * kSmBins; i += kSmThreads) (&S.hist[0][0])[i] = 0;
+                if (tid == 0) S.bin = 0, S.n_short = 0;
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    if (part[e] >= 0) {
+                        atomicAdd(&S.hist[0][part[e]], (uint32_t)val[e] & 0xffffu);
+                        atomicAdd(&S.hist[1][part[e]], (uint32_t)val[e] >> 16);
+                    }
+                __syncthreads();
+                u64 z[2];
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    z[e] = (u64)S.hist[0][2 * tid + e] + ((u64)S.hist[1][2 * tid + e] << 16);
+                u64 q = above + sm_block_before(z[0] + z[1], S.warp);
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    if ((double)b < thr && (double)(b + v[e]) >= thr) {
-                        const u64 y = S.list[2 * tid + e];
-                        S.cut.l = sm_unkey((uint32_t)(y >> 32));
-                        S.cut.idx = (int)(0xffffffffu - (uint32_t)y);
+                    if ((double)q < thr && (double)(q + z[e]) >= thr) S.bin = 2 * tid + e, S.found_before = q;
+                    q += z[e];
+                }
+                __syncthreads();
+                over = S.found_before;
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    if (part[e] == S.bin) {
+                        const int at = atomicAdd(&S.n_short, 1);
+                        if (at < 32) S.short_list[at] = y[e];
                     }
-                    b += v[e];
+                __syncthreads();
+                if (S.n_short <= 32) {                 // one warp: each token's sum of those before it
+                    if (tid < 32) {
+                        const u64 mine = tid < S.n_short ? S.short_list[tid] : 0, w = tid < S.n_short ? value(mine) : 0;
+                        u64 c = over;
+                        for (int i = 0; i < S.n_short; i++) {
+                            const u64 other = __shfl_sync(0xffffffffu, mine, i), ow = __shfl_sync(0xffffffffu, w, i);
+                            c += other > mine ? ow : 0;
+                        }
+                        if (tid < S.n_short && (double)c < thr && (double)(c + w) >= thr) {
+                            S.cut.l = sm_unkey((uint32_t)(mine >> 32));
+                            S.cut.idx = (int)(0xffffffffu - (uint32_t)mine);
+                        }
+                    }
+                } else {                               // the list once more, sorted by the order, then summed
+                    int m = 2;
+                    while (m < have) m <<= 1;
+#pragma unroll
+                    for (int e = 0; e < 2; e++) S.list[tid + e * kSmThreads] = part[e] >= 0 ? y[e] : 0;
+                    __syncthreads();
+                    for (int size = 2; size <= m; size <<= 1)
+                        for (int step = size >> 1; step > 0; step >>= 1) {
+                            for (int i = tid; i < m / 2; i += kSmThreads) {
+                                const int a = 2 * i - (i & (step - 1)), b = a + step;
+                                const u64 va = S.list[a], vb = S.list[b];
+                                if ((va < vb) == ((a & size) == 0)) S.list[a] = vb, S.list[b] = va;
+                            }
+                            __syncthreads();
+                        }
+#pragma unroll
+                    for (int e = 0; e < 2; e++) z[e] = 2 * tid + e < have ? value(S.list[2 * tid + e]) : 0;
+                    q = above + sm_block_before(z[0] + z[1], S.warp);
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        if ((double)q < thr && (double)(q + z[e]) >= thr) {
+                            S.cut.l = sm_unkey((uint32_t)(S.list[2 * tid + e] >> 32));
+                            S.cut.idx = (int)(0xffffffffu - (uint32_t)S.list[2 * tid + e]);
+                        }
+                        q += z[e];
+                    }
                 }
                 __syncthreads();
                 if (tid > 0 && tid < C) cl.map_shared_rank(&S, tid)->cut = S.cut;
@@ -347,11 +488,13 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
         // key are in, and the index of the last of them.
         auto sum_ge = [&](uint32_t key, bool indexes, uint32_t upto) {
             u64 s = 0;
-            sm_each(x, n, i0, [&](float l, int i) {
-                if (!(l >= cut.l) || (l == cut.l && i > cut.idx)) return;
-                const uint32_t y = sm_key(l);
-                if (indexes ? y == key && (uint32_t)i <= upto : y >= key)
-                    s += mass && !indexes ? sm_weight(sm_exp(l, top, inv_t)) : 1;
+            X.each([&](const float (&v)[E], int i) {
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const uint32_t y = sm_key(v[e]);
+                    if (in(v[e], i + e) && (indexes ? y == key && (uint32_t)(i + e) <= upto : y >= key))
+                        s += mass && !indexes ? sm_weight(sm_exp(v[e], top, inv_t)) : 1;
+                }
             });
             return cluster_sum(s, nullptr);
         };
@@ -387,37 +530,73 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
         }
     }
 
-    // ---- the draw: the CTA, then the run of tokens, then the token ----
-    auto weight = [&](float l, int i) -> u64 {
-        if (!(l >= cut.l) || (l == cut.l && i > cut.idx)) return 0;
-        const float e = sm_exp(l, top, inv_t);
-        return mp > 0.0f && !(e >= mp) ? 0 : sm_weight(e);
+    // ---- the draw: the CTA, then the warp's run, then the token ----
+    auto weigh_min_p = [&](const float (&v)[E], int i, uint32_t (&w)[E]) {
+        u64 s = 0;
+        if (!weigh(v, i, w)) {
+#pragma unroll
+            for (int e = 0; e < E; e++) w[e] = 0u;
+            return s;
+        }
+        if (mp > 0.0f) {                               // the whole cluster
+#pragma unroll
+            for (int e = 0; e < E; e++)
+                if (!(sm_exp(v[e], top, inv_t) >= mp)) w[e] = 0u;
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++) s += w[e];
+        return s;
     };
     u64 sum = 0, before;
-    sm_each(x, n, i0, [&](float l, int i) { sum += weight(l, i); });
+    X.each([&](const float (&v)[E], int i) {
+        uint32_t w[E];
+        sum += weigh_min_p(v, i, w);
+    });
     const u64 total = cluster_sum(sum, &before);
     const double at = floor((double)u * (double)total);
     u64 target = at > 0.0 ? (u64)at : 0;
     target = target < total ? target : total - 1;
     const u64 here = S.sums[turn ^ 1][rank];
     if (target < before || target >= before + here) return;
-    const int len = ((n + kSmThreads - 1) / kSmThreads) | 1;      // odd: a run a thread, no bank met twice
-    const int a = min(n, tid * len), b = min(n, a + len);
-    sum = 0;
-    for (int i = a; i < b; i++) sum += weight((float)x[i], i0 + i);
-    before += sm_block_before(sum, S.warp);
-    if (before <= target && target < before + sum) {
-        u64 run = before;
-        for (int i = a; i < b; i++) {
-            const u64 w = weight((float)x[i], i0 + i);
-            run += w;
-            if (run > target) {
-                P.ids[row] = i0 + i;
-                if (P.prob) P.prob[row] = (float)((double)w / (double)total);
-                break;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    before += sm_block_before(lane == 0 ? sum : 0, S.warp);
+    before = __shfl_sync(0xffffffffu, before, 0);      // of the warps before this one
+    if (target < before || target >= before + sum) return;
+    // steps of the warp's run, in index order; true when the token was in this one
+    auto step = [&](const float (&v)[E], int i, bool on) {
+        uint32_t w[E];
+        const u64 mine = on ? weigh_min_p(v, i, w) : 0;
+        u64 up = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 y = __shfl_up_sync(0xffffffffu, up, o);
+            if (lane >= o) up += y;
+        }
+        u64 run = before + up - mine;
+        if (on && run <= target && target < run + mine) {
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                if (run <= target && target < run + w[e]) {
+                    P.ids[row] = i + e;
+                    if (P.prob) P.prob[row] = (float)((double)w[e] / (double)total);
+                }
+                run += w[e];
             }
         }
+        before += __shfl_sync(0xffffffffu, up, 31);
+        return target < before;
+    };
+    float v[E];
+    int i = X.ragged(0, v);
+    if (step(v, i, i >= 0)) return;
+    for (int j = X.lo; j < X.hi; j += 32) {
+        const bool on = j + lane < X.hi;
+        if (on) X.load(j + lane, v);
+        if (step(v, X.index(j + lane), on)) return;
     }
+    i = X.ragged(1, v);
+    step(v, i, i >= 0);
 }
 
 // A cluster of C CTAs for each row: as few as hold the row with two CTAs an
