@@ -24,8 +24,9 @@ namespace cg = cooperative_groups;
 
 namespace sepia {
 
-constexpr int kSmThreads = 512;
-constexpr int kSmBins = 1024;                // two per thread
+constexpr int kSmThreads = 512;              // 256 save a fifth of the instructions but wait longer: 228 us for 192 x 200058, 512 take 201
+constexpr int kSmBins = 1024;
+constexpr int kSmPer = kSmBins / kSmThreads; // bins (and list entries) of a thread
 constexpr int kSmList = 1024;                // tokens of a threshold bin that are sorted
 constexpr int kSmMaxCluster = 8;
 constexpr float kSmRange = 22.25f;           // beyond exp(-this) a weight rounds to 0
@@ -74,7 +75,7 @@ struct SmShared {
     };
     float best[kSmMaxCluster];
     int best_idx[kSmMaxCluster];
-    u64 sums[2][kSmMaxCluster], warp[kSmThreads / 32];
+    u64 sums[2][kSmMaxCluster][2], warp[kSmThreads / 32];
     int first_idx, n_short;
     u64 short_list[32];                      // tokens of the threshold's part of the bin
     u64 found_before;                        // count or mass of the bins above the threshold bin
@@ -263,17 +264,23 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
 
     // ---- sums over the whole row: every CTA tells all ----
     int turn = 0;
-    auto cluster_sum = [&](u64 v, u64 *mine_before) {
-        const u64 s = sm_block_sum(v, S.warp);
-        if (tid < C) cl.map_shared_rank(&S, tid)->sums[turn][rank] = s;
+    auto cluster_sum = [&](u64 v, u64 other, u64 *before, u64 *other_all) {
+        const u64 s = sm_block_sum(v, S.warp), o = other_all ? sm_block_sum(other, S.warp) : 0;
+        if (tid < C) {
+            SmShared *q = cl.map_shared_rank(&S, tid);
+            q->sums[turn][rank][0] = s;
+            q->sums[turn][rank][1] = o;
+        }
         cl.sync();
-        u64 all = 0, before = 0;
+        u64 all = 0, less = 0, others = 0;
         for (int r = 0; r < C; r++) {
-            before += r < rank ? S.sums[turn][r] : 0;
-            all += S.sums[turn][r];
+            less += r < rank ? S.sums[turn][r][0] : 0;
+            all += S.sums[turn][r][0];
+            others += S.sums[turn][r][1];
         }
         turn ^= 1;                                     // the next sum must not overwrite what is still read
-        if (mine_before) *mine_before = before;
+        if (before) *before = less;
+        if (other_all) *other_all = others;
         return all;
     };
     // Below this a weight rounds to 0: rounding of the bound itself cannot
@@ -306,7 +313,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
     auto find_cut = [&](bool mass, double want, float range) {
         const float per = kSmBins / range * inv_t, near = range < kSmRange ? fmaxf(cut.l, top - range * t) : cut.l;
         for (int i = tid; i < 2 * kSmBins; i += kSmThreads) (&S.hist[0][0])[i] = 0;
-        if (tid == 0) S.n_list = 0;
+        if (tid == 0) S.n_list = 0, S.bin = -1;
         __syncthreads();
         u64 beyond = 0;
         auto place_of = [&](float l) { return (top - l) * per; };       // NaN where both are infinite: bin 0
@@ -334,38 +341,35 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
                     atomicAdd(&S.hist[1][b], w[e] >> 16);
                 }
         });
-        const u64 far_mass = mass ? cluster_sum(beyond, nullptr) : 0;
-        if (!mass) cl.sync();
-        // The threshold bin: each CTA adds its share of the bins over the cluster
-        const int share = kSmBins / C;                 // bins of a CTA, up to two a thread
-        u64 v[2] = {0, 0};
+        cl.sync();
+        // The threshold bin: each CTA adds its share of the bins over the
+        // cluster, a run of `each` neighbours a thread
+        const int share = kSmBins / C, each = max(1, share / kSmThreads), first_bin = rank * share + tid * each;
+        u64 v[kSmPer] = {}, mine = 0;
 #pragma unroll
-        for (int e = 0; e < 2; e++)
-            if (tid + e * kSmThreads < share) {
-                // thread order is bin order: with two bins a thread they are neighbours
-                const int b = rank * share + (share > kSmThreads ? 2 * tid + e : tid);
+        for (int e = 0; e < kSmPer; e++)
+            if (e < each && tid * each < share) {
                 uint32_t x[kSmMaxCluster][2];
 #pragma unroll
                 for (int r = 0; r < kSmMaxCluster; r++) {
                     const SmShared *q = cl.map_shared_rank(&S, r < C ? r : 0);
-                    x[r][0] = r < C ? q->hist[0][b] : 0;
-                    x[r][1] = r < C && mass ? q->hist[1][b] : 0;
+                    x[r][0] = r < C ? q->hist[0][first_bin + e] : 0;
+                    x[r][1] = r < C && mass ? q->hist[1][first_bin + e] : 0;
                 }
 #pragma unroll
                 for (int r = 0; r < kSmMaxCluster; r++) v[e] += (u64)x[r][0] + ((u64)x[r][1] << 16);
+                mine += v[e];
             }
-        u64 b = 0;
-        const u64 all = cluster_sum(v[0] + v[1], &b) + far_mass;
-        const double thr = mass ? want * (double)all : want;
-        b += sm_block_before(v[0] + v[1], S.warp);
-        if (tid == 0) S.bin = -1;
-        cl.sync();                                     // every CTA's bin is unset before one is found
+        u64 b = 0, far_mass = 0;
+        const u64 all = cluster_sum(mine, beyond, &b, &far_mass);
+        const double thr = mass ? want * (double)(all + far_mass) : want;
+        b += sm_block_before(mine, S.warp);
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
+        for (int e = 0; e < kSmPer; e++) {
             if ((double)b < thr && (double)(b + v[e]) >= thr)
                 for (int r = 0; r < C; r++) {
                     SmShared *q = cl.map_shared_rank(&S, r);
-                    q->bin = rank * share + (share > kSmThreads ? 2 * tid + e : tid);
+                    q->bin = first_bin + e;
                     q->found_before = b;
                 }
             b += v[e];
@@ -396,41 +400,43 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
                 auto value = [&](u64 y) -> u64 {
                     return !mass ? 1 : sm_weight(sm_exp(sm_unkey((uint32_t)(y >> 32)), top, inv_t));
                 };
-                // this thread's two tokens of the list, and their part of the bin
-                u64 y[2], val[2] = {0, 0}, over = above;
-                int part[2] = {-1, -1};
+                // this thread's tokens of the list, and their part of the bin
+                u64 y[kSmPer], val[kSmPer], z[kSmPer], over, q = 0;
+                int part[kSmPer];
 #pragma unroll
-                for (int e = 0; e < 2; e++)
-                    if (tid + e * kSmThreads < have) {
-                        y[e] = S.list[tid + e * kSmThreads];
-                        val[e] = value(y[e]);
-                        part[e] = max(0, min(kSmBins - 1, (int)((place_of(sm_unkey((uint32_t)(y[e] >> 32))) - (float)bin) * kSmBins)));
-                    }
+                for (int e = 0; e < kSmPer; e++) {
+                    const bool on = tid + e * kSmThreads < have;
+                    y[e] = on ? S.list[tid + e * kSmThreads] : 0;
+                    val[e] = on ? value(y[e]) : 0;
+                    const float at = (place_of(sm_unkey((uint32_t)(y[e] >> 32))) - (float)bin) * kSmBins;
+                    part[e] = on ? max(0, min(kSmBins - 1, (int)at)) : -1;
+                }
                 __syncthreads();                       // the list is read: its room becomes counters again
                 for (int i = tid; i < 2 * kSmBins; i += kSmThreads) (&S.hist[0][0])[i] = 0;
-                if (tid == 0) S.bin = 0, S.n_short = 0;
+                if (tid == 0) S.n_short = 0;
                 __syncthreads();
 #pragma unroll
-                for (int e = 0; e < 2; e++)
+                for (int e = 0; e < kSmPer; e++)
                     if (part[e] >= 0) {
                         atomicAdd(&S.hist[0][part[e]], (uint32_t)val[e] & 0xffffu);
                         atomicAdd(&S.hist[1][part[e]], (uint32_t)val[e] >> 16);
                     }
                 __syncthreads();
-                u64 z[2];
 #pragma unroll
-                for (int e = 0; e < 2; e++)
-                    z[e] = (u64)S.hist[0][2 * tid + e] + ((u64)S.hist[1][2 * tid + e] << 16);
-                u64 q = above + sm_block_before(z[0] + z[1], S.warp);
+                for (int e = 0; e < kSmPer; e++) {
+                    z[e] = (u64)S.hist[0][kSmPer * tid + e] + ((u64)S.hist[1][kSmPer * tid + e] << 16);
+                    q += z[e];
+                }
+                q = above + sm_block_before(q, S.warp);
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    if ((double)q < thr && (double)(q + z[e]) >= thr) S.bin = 2 * tid + e, S.found_before = q;
+                for (int e = 0; e < kSmPer; e++) {
+                    if ((double)q < thr && (double)(q + z[e]) >= thr) S.bin = kSmPer * tid + e, S.found_before = q;
                     q += z[e];
                 }
                 __syncthreads();
                 over = S.found_before;
 #pragma unroll
-                for (int e = 0; e < 2; e++)
+                for (int e = 0; e < kSmPer; e++)
                     if (part[e] == S.bin) {
                         const int at = atomicAdd(&S.n_short, 1);
                         if (at < 32) S.short_list[at] = y[e];
@@ -453,7 +459,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
                     int m = 2;
                     while (m < have) m <<= 1;
 #pragma unroll
-                    for (int e = 0; e < 2; e++) S.list[tid + e * kSmThreads] = part[e] >= 0 ? y[e] : 0;
+                    for (int e = 0; e < kSmPer; e++) S.list[tid + e * kSmThreads] = y[e];
                     __syncthreads();
                     for (int size = 2; size <= m; size <<= 1)
                         for (int step = size >> 1; step > 0; step >>= 1) {
@@ -464,14 +470,18 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
                             }
                             __syncthreads();
                         }
+                    q = 0;
 #pragma unroll
-                    for (int e = 0; e < 2; e++) z[e] = 2 * tid + e < have ? value(S.list[2 * tid + e]) : 0;
-                    q = above + sm_block_before(z[0] + z[1], S.warp);
+                    for (int e = 0; e < kSmPer; e++) {
+                        z[e] = kSmPer * tid + e < have ? value(S.list[kSmPer * tid + e]) : 0;
+                        q += z[e];
+                    }
+                    q = above + sm_block_before(q, S.warp);
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
+                    for (int e = 0; e < kSmPer; e++) {
                         if ((double)q < thr && (double)(q + z[e]) >= thr) {
-                            S.cut.l = sm_unkey((uint32_t)(S.list[2 * tid + e] >> 32));
-                            S.cut.idx = (int)(0xffffffffu - (uint32_t)S.list[2 * tid + e]);
+                            S.cut.l = sm_unkey((uint32_t)(S.list[kSmPer * tid + e] >> 32));
+                            S.cut.idx = (int)(0xffffffffu - (uint32_t)S.list[kSmPer * tid + e]);
                         }
                         q += z[e];
                     }
@@ -496,7 +506,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
                         s += mass && !indexes ? sm_weight(sm_exp(v[e], top, inv_t)) : 1;
                 }
             });
-            return cluster_sum(s, nullptr);
+            return cluster_sum(s, 0, nullptr, nullptr);
         };
         uint32_t key = 0;
         for (int b = 31; b >= 0; b--)
@@ -552,11 +562,11 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
         uint32_t w[E];
         sum += weigh_min_p(v, i, w);
     });
-    const u64 total = cluster_sum(sum, &before);
+    const u64 total = cluster_sum(sum, 0, &before, nullptr);
     const double at = floor((double)u * (double)total);
     u64 target = at > 0.0 ? (u64)at : 0;
     target = target < total ? target : total - 1;
-    const u64 here = S.sums[turn ^ 1][rank];
+    const u64 here = S.sums[turn ^ 1][rank][0];
     if (target < before || target >= before + here) return;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -566,7 +576,13 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
     // steps of the warp's run, in index order; true when the token was in this one
     auto step = [&](const float (&v)[E], int i, bool on) {
         uint32_t w[E];
-        const u64 mine = on ? weigh_min_p(v, i, w) : 0;
+        const u64 mine = on ? weigh_min_p(v, i, w) : 0;    // below 2^35
+        const u64 all = (u64)__reduce_add_sync(0xffffffffu, (uint32_t)mine & 0xfffffu) +
+                        ((u64)__reduce_add_sync(0xffffffffu, (uint32_t)(mine >> 20)) << 20);
+        if (target >= before + all) {
+            before += all;
+            return false;
+        }
         u64 up = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -584,8 +600,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
                 run += w[e];
             }
         }
-        before += __shfl_sync(0xffffffffu, up, 31);
-        return target < before;
+        return true;
     };
     float v[E];
     int i = X.ragged(0, v);
