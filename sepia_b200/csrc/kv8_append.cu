@@ -54,11 +54,12 @@ __device__ __forceinline__ void load4(const T *p, int vec, float (&x)[4]) {
 }
 
 // fp16 with magnitudes above the largest finite value saturated; NaN stays NaN
-__device__ __forceinline__ __half to_half_sat(float x) {
-    const __half h = __float2half_rn(x);
+__device__ __forceinline__ __half sat_half(__half h) {
     const unsigned short u = __half_as_ushort(h);
     return (u & 0x7fffu) == 0x7c00u ? __ushort_as_half((unsigned short)(u - 1u)) : h;
 }
+__device__ __forceinline__ __half to_half(float x) { return sat_half(__float2half_rn(x)); }
+__device__ __forceinline__ __half to_half(double x) { return sat_half(__double2half(x)); }
 
 // The smallest power of two s with amax / s <= 448 = 1.75 * 2^8. amax is the
 // magnitude of an fp16 number, so it is a normal fp32 number or zero.
@@ -68,29 +69,38 @@ __device__ __forceinline__ float block_scale(float amax) {
     return __uint_as_float((((u >> 23) - 8u) + ((u & 0x7fffffu) > 0x600000u ? 1u : 0u)) << 23);
 }
 
-// RMS norm of the warp's row, then the rotation; lane owns dims 4*lane ..+3.
-__device__ __forceinline__ void norm_rotate(float (&x)[4], const float *w, const SepiaKv8Append &a, int Dh, int pos,
-                                            bool positions_ok) {
+// 1/sqrt(mean square + eps) of a warp's row from its lanes' sums of squares
+__device__ __forceinline__ float inv_rms(float s, int Dh, float eps) {
+    return rsqrtf(warp_sum(s) / (float)Dh + eps);
+}
+__device__ __forceinline__ double inv_rms(double s, int Dh, float eps) {
+    return rsqrt(warp_sum_d(s) / (double)Dh + (double)eps);
+}
+
+// RMS norm of the warp's row (w: the lane's weights), then the rotation; a
+// lane owns dims 4*lane ..+3. Queries are worked out in fp32, keys in fp64:
+// a key is rounded to fp16 and then to 8 bits, and only with the exact value
+// at hand are these the roundings of the key itself.
+template <typename R>
+__device__ __forceinline__ void norm_rotate(R (&x)[4], const float *w, const SepiaKv8Append &a, int Dh, const float2 *cs) {
     const int lane = threadIdx.x & 31, d = 4 * lane;
     if (w) {
-        float s = 0.0f;
+        R s = 0;
 #pragma unroll
-        for (int i = 0; i < 4; i++) s = fmaf(x[i], x[i], s);
-        s = warp_sum(s);
-        const float inv = __fdiv_rn(1.0f, __fsqrt_rn(s / (float)Dh + a.eps));
+        for (int i = 0; i < 4; i++) s += x[i] * x[i];
+        s = inv_rms(s, Dh, a.eps);
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = d < Dh ? w[d + i] * (x[i] * inv) : 0.0f;
+        for (int i = 0; i < 4; i++) x[i] = (R)w[i] * (x[i] * s);
     }
-    if (a.rot_dim && positions_ok) {
-        const float2 *cs = reinterpret_cast<const float2 *>(a.rotation) + (int64_t)pos * (a.rot_dim / 2);
+    if (cs) {                                          // the position's cosines and sines; the whole warp
         if (a.rot_adjacent) {
             if (d < a.rot_dim) {
 #pragma unroll
                 for (int i = 0; i < 4; i += 2) {
                     const float2 t = cs[(d + i) / 2];
-                    const float u = x[i], v = x[i + 1];
-                    x[i] = u * t.x - v * t.y;
-                    x[i + 1] = v * t.x + u * t.y;
+                    const R u = x[i], v = x[i + 1];
+                    x[i] = u * (R)t.x - v * (R)t.y;
+                    x[i + 1] = v * (R)t.x + u * (R)t.y;
                 }
             }
         } else {
@@ -99,18 +109,26 @@ __device__ __forceinline__ void norm_rotate(float (&x)[4], const float *w, const
             const int from = low ? lane + hl : lane - hl;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float y = __shfl_sync(0xffffffffu, x[i], from & 31);
+                const R y = __shfl_sync(0xffffffffu, x[i], from & 31);
                 if (d < a.rot_dim) {
                     const float2 t = cs[low ? d + i : d - half + i];
-                    x[i] = low ? x[i] * t.x - y * t.y : x[i] * t.x + y * t.y;
+                    x[i] = low ? x[i] * (R)t.x - y * (R)t.y : x[i] * (R)t.x + y * (R)t.y;
                 }
             }
         }
     }
 }
 
+// The position's row of the rotation table; NULL (and the error word) past its end
+__device__ __forceinline__ const float2 *rotation_row(const SepiaKv8Append &a, int pos, int *err) {
+    if (!a.rot_dim) return nullptr;
+    if (pos < a.rot_positions) return reinterpret_cast<const float2 *>(a.rotation) + (int64_t)pos * (a.rot_dim / 2);
+    set_error(err, kErrBadArgs);
+    return nullptr;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kApThreads) k_kv8_append(const ApParams P) {
+__global__ void __launch_bounds__(kApThreads, 4) k_kv8_append(const ApParams P) {
     __shared__ float s_amax[kApWarps];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, d = 4 * lane;
     const int Dh = P.c.head_dim, B = P.c.block, Hkv = P.c.n_kv_heads;
@@ -121,35 +139,44 @@ __global__ void __launch_bounds__(kApThreads) k_kv8_append(const ApParams P) {
         const int item = blockIdx.x - P.kv_ctas;
         const int s = item / P.q_items, H = P.a.n_heads;
         const Kv8Seq sq = kv8_seq(P.c, P.b, s, P.err);
-        const int64_t rows = (int64_t)sq.rows * H;
-        const int64_t first = ((int64_t)(item - s * P.q_items) * kApWarps + warp) * kApQRows;
-        float x[kApQRows][4];
+        const int rows = sq.rows * H, first = ((item - s * P.q_items) * kApWarps + warp) * kApQRows;
+        if (first >= rows) return;                     // the whole warp
+        if (sq.add < 0) {                              // idle or out of bounds: zeros
+            for (int r = first; r < min(rows, first + kApQRows); r++)
+                for (int e = lane; e < Dh; e += 32) ((T *)P.a.q_out)[((int64_t)sq.n0 * H + r) * Dh + e] = (T)0.0f;
+            return;
+        }
+        const int i0 = first / H, h0 = first - i0 * H; // rows are (token, head); the next row's by counting on
+        float x[kApQRows][4], w[4] = {}, f[kApQRows];
+        if (P.a.q_norm && d < Dh)
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = P.a.q_norm[d + e];
+        int i = i0, h = h0;
 #pragma unroll
         for (int j = 0; j < kApQRows; j++) {
-            const int64_t r = first + j;
-            const int i = (int)(r / H), h = (int)(r - (int64_t)i * H);
 #pragma unroll
             for (int e = 0; e < 4; e++) x[j][e] = 0.0f;
-            if (r < rows && sq.add >= 0 && d < Dh)
-                load4((const T *)P.a.q + (int64_t)(sq.n0 + i) * P.a.q_stride + (int64_t)h * Dh + d, P.vec_q, x[j]);
+            f[j] = 1.0f;
+            if (first + j < rows) {
+                if (d < Dh) load4((const T *)P.a.q + (int64_t)(sq.n0 + i) * P.a.q_stride + h * Dh + d, P.vec_q, x[j]);
+                if (P.a.q_scale) f[j] = P.a.q_scale[sq.n0 + i];
+            }
+            if (++h == H) h = 0, i++;
         }
+        i = i0, h = h0;
 #pragma unroll
         for (int j = 0; j < kApQRows; j++) {
-            const int64_t r = first + j;
-            if (r >= rows) break;                      // the whole warp
-            const int i = (int)(r / H), h = (int)(r - (int64_t)i * H);
-            const int pos = sq.held + i, n = sq.n0 + i;
-            const bool ok = sq.add >= 0 && (!P.a.rot_dim || pos < P.a.rot_positions);
-            if (sq.add >= 0 && !ok && lane == 0) set_error(P.err, kErrBadArgs);
-            norm_rotate(x[j], P.a.q_norm, P.a, Dh, pos, ok);
-            const float f = P.a.q_scale ? P.a.q_scale[n] : 1.0f;
-            if (d < Dh) {
-                T *o = (T *)P.a.q_out + ((int64_t)n * H + h) * Dh + d;
-                T y[4];
+            if (first + j < rows) {                    // the whole warp
+                norm_rotate(x[j], P.a.q_norm ? w : nullptr, P.a, Dh, rotation_row(P.a, sq.held + i, P.err));
+                if (d < Dh) {
+                    T y[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) y[e] = (T)(x[j][e] * f);
-                *reinterpret_cast<typename Vec4<T>::type *>(o) = *reinterpret_cast<const typename Vec4<T>::type *>(y);
+                    for (int e = 0; e < 4; e++) y[e] = (T)(x[j][e] * f[j]);
+                    *reinterpret_cast<typename Vec4<T>::type *>((T *)P.a.q_out + ((int64_t)(sq.n0 + i) * H + h) * Dh + d) =
+                        *reinterpret_cast<const typename Vec4<T>::type *>(y);
+                }
             }
+            if (++h == H) h = 0, i++;
         }
         return;
     }
@@ -167,7 +194,11 @@ __global__ void __launch_bounds__(kApThreads) k_kv8_append(const ApParams P) {
     const T *x_in = (const T *)(is_v ? P.a.v : P.a.k);
     const int64_t stride = is_v ? P.a.v_stride : P.a.k_stride;
     const int vec = is_v ? P.vec_v : P.vec_k;
-    const float *norm = is_v ? nullptr : P.a.k_norm;
+    const bool exact = !is_v && (P.a.k_norm || P.a.rot_dim);   // else the row is rounded as it is
+    float w[4] = {};
+    if (!is_v && P.a.k_norm && d < Dh)
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = P.a.k_norm[d + e];
     __half *tail = (__half *)(is_v ? P.c.v_tail : P.c.k_tail) + ((int64_t)sq.slot * Hkv + hk) * B * Dh;
     uint8_t *codes = (uint8_t *)(is_v ? P.c.v : P.c.k);
     float *scales = is_v ? P.c.v_scale : P.c.k_scale;
@@ -189,14 +220,15 @@ __global__ void __launch_bounds__(kApThreads) k_kv8_append(const ApParams P) {
             float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             if (r >= lo && r < hi && d < Dh)
                 load4(x_in + (int64_t)(sq.n0 + base + r) * stride + (int64_t)hk * Dh + d, vec, x);
-            if (r >= lo && r < hi) {                   // the whole warp
-                const int pos = sq.held + base + r;
-                const bool ok = !P.a.rot_dim || pos < P.a.rot_positions;
-                if (!ok && lane == 0) set_error(P.err, kErrBadArgs);
-                if (!is_v) norm_rotate(x, norm, P.a, Dh, pos, ok);
+            if (exact && r >= lo && r < hi) {          // the whole warp
+                double z[4] = {x[0], x[1], x[2], x[3]};
+                norm_rotate(z, P.a.k_norm ? w : nullptr, P.a, Dh, rotation_row(P.a, sq.held + base + r, P.err));
+                y[j][0] = __halves2half2(to_half(z[0]), to_half(z[1]));
+                y[j][1] = __halves2half2(to_half(z[2]), to_half(z[3]));
+            } else {
+                y[j][0] = __halves2half2(to_half(x[0]), to_half(x[1]));
+                y[j][1] = __halves2half2(to_half(x[2]), to_half(x[3]));
             }
-            y[j][0] = __halves2half2(to_half_sat(x[0]), to_half_sat(x[1]));
-            y[j][1] = __halves2half2(to_half_sat(x[2]), to_half_sat(x[3]));
             if (full && r < lo && d < Dh) {
                 const uint2 raw = *reinterpret_cast<const uint2 *>(tail + r * Dh + d);
                 y[j][0] = *reinterpret_cast<const __half2 *>(&raw.x);
@@ -304,7 +336,7 @@ extern "C" int sepia_cuda_kv8_append(const SepiaKv8Cache *c, const SepiaKv8Step 
     const int64_t per = kApWarps * kApQRows;
     const int64_t kv_ctas = (int64_t)b->n_seqs * P.touched * c->n_kv_heads * 2;
     const int64_t q_items = (rows + per - 1) / per, all = kv_ctas + b->n_seqs * q_items;
-    if (all > INT32_MAX) return fail("%s: step too large", what);
+    if (all > INT32_MAX || rows > INT32_MAX - per) return fail("%s: step too large", what);
     P.kv_ctas = (int)kv_ctas;
     P.q_items = (int)(q_items ? q_items : 1);
     P.vec_k = rows_vec(a->k, a->k_stride, a->x_f16);
