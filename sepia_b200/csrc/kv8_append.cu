@@ -29,6 +29,7 @@ struct ApParams {
     int q_items;             // query CTAs per sequence
     int kv_ctas;             // CTAs of keys and values, before those of queries
     int vec_k, vec_v, vec_q; // the tensor's rows allow one vector load per lane
+    double inv_dh;           // 1 / head_dim
     int *err;
 };
 
@@ -70,11 +71,11 @@ __device__ __forceinline__ float block_scale(float amax) {
 }
 
 // 1/sqrt(mean square + eps) of a warp's row from its lanes' sums of squares
-__device__ __forceinline__ float inv_rms(float s, int Dh, float eps) {
-    return rsqrtf(warp_sum(s) / (float)Dh + eps);
+__device__ __forceinline__ float inv_rms(float s, double inv_dh, float eps) {
+    return rsqrtf(fmaf(warp_sum(s), (float)inv_dh, eps));
 }
-__device__ __forceinline__ double inv_rms(double s, int Dh, float eps) {
-    return rsqrt(warp_sum_d(s) / (double)Dh + (double)eps);
+__device__ __forceinline__ double inv_rms(double s, double inv_dh, float eps) {
+    return rsqrt(fma(warp_sum_d(s), inv_dh, (double)eps));
 }
 
 // RMS norm of the warp's row (w: the lane's weights), then the rotation; a
@@ -82,13 +83,13 @@ __device__ __forceinline__ double inv_rms(double s, int Dh, float eps) {
 // a key is rounded to fp16 and then to 8 bits, and only with the exact value
 // at hand are these the roundings of the key itself.
 template <typename R>
-__device__ __forceinline__ void norm_rotate(R (&x)[4], const float *w, const SepiaKv8Append &a, int Dh, const float2 *cs) {
+__device__ __forceinline__ void norm_rotate(R (&x)[4], const float *w, const SepiaKv8Append &a, double inv_dh, const float2 *cs) {
     const int lane = threadIdx.x & 31, d = 4 * lane;
     if (w) {
         R s = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) s += x[i] * x[i];
-        s = inv_rms(s, Dh, a.eps);
+        s = inv_rms(s, inv_dh, a.eps);
 #pragma unroll
         for (int i = 0; i < 4; i++) x[i] = (R)w[i] * (x[i] * s);
     }
@@ -167,7 +168,7 @@ __global__ void __launch_bounds__(kApThreads, 4) k_kv8_append(const ApParams P) 
 #pragma unroll
         for (int j = 0; j < kApQRows; j++) {
             if (first + j < rows) {                    // the whole warp
-                norm_rotate(x[j], P.a.q_norm ? w : nullptr, P.a, Dh, rotation_row(P.a, sq.held + i, P.err));
+                norm_rotate(x[j], P.a.q_norm ? w : nullptr, P.a, P.inv_dh, rotation_row(P.a, sq.held + i, P.err));
                 if (d < Dh) {
                     T y[4];
 #pragma unroll
@@ -212,27 +213,32 @@ __global__ void __launch_bounds__(kApThreads, 4) k_kv8_append(const ApParams P) 
         const int lo = blk == b0 ? r0 : 0;             // rows below wait in the tail
         const int hi = full ? B : tail_rows;
         const int base = blk * B - sq.held;            // row r of the block is new token base + r
+        // every row first, new ones and (where the block ends) those of the tail: one round of loads
+        float x[kApMaxRows][4];
+#pragma unroll
+        for (int j = 0; j < kApMaxRows; j++) {
+            const int r = warp + kApWarps * j;
+            x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0.0f;
+            if (r >= hi || d >= Dh) continue;
+            if (r >= lo) {
+                load4(x_in + (int64_t)(sq.n0 + base + r) * stride + hk * Dh + d, vec, x[j]);
+            } else if (full) {
+                load4(tail + r * Dh + d, 1, x[j]);
+            }
+        }
         __half2 y[kApMaxRows][2];
         float amax = 0.0f;
 #pragma unroll
         for (int j = 0; j < kApMaxRows; j++) {
             const int r = warp + kApWarps * j;
-            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (r >= lo && r < hi && d < Dh)
-                load4(x_in + (int64_t)(sq.n0 + base + r) * stride + (int64_t)hk * Dh + d, vec, x);
             if (exact && r >= lo && r < hi) {          // the whole warp
-                double z[4] = {x[0], x[1], x[2], x[3]};
-                norm_rotate(z, P.a.k_norm ? w : nullptr, P.a, Dh, rotation_row(P.a, sq.held + base + r, P.err));
+                double z[4] = {x[j][0], x[j][1], x[j][2], x[j][3]};
+                norm_rotate(z, P.a.k_norm ? w : nullptr, P.a, P.inv_dh, rotation_row(P.a, sq.held + base + r, P.err));
                 y[j][0] = __halves2half2(to_half(z[0]), to_half(z[1]));
                 y[j][1] = __halves2half2(to_half(z[2]), to_half(z[3]));
             } else {
-                y[j][0] = __halves2half2(to_half(x[0]), to_half(x[1]));
-                y[j][1] = __halves2half2(to_half(x[2]), to_half(x[3]));
-            }
-            if (full && r < lo && d < Dh) {
-                const uint2 raw = *reinterpret_cast<const uint2 *>(tail + r * Dh + d);
-                y[j][0] = *reinterpret_cast<const __half2 *>(&raw.x);
-                y[j][1] = *reinterpret_cast<const __half2 *>(&raw.y);
+                y[j][0] = __halves2half2(to_half(x[j][0]), to_half(x[j][1]));
+                y[j][1] = __halves2half2(to_half(x[j][2]), to_half(x[j][3]));
             }
             if (!full && r >= lo && r < hi && d < Dh) {
                 uint2 raw;
@@ -331,6 +337,7 @@ extern "C" int sepia_cuda_kv8_append(const SepiaKv8Cache *c, const SepiaKv8Step 
     P.b = *b;
     P.a = *a;
     P.err = dev_info().err;
+    P.inv_dh = 1.0 / (double)c->head_dim;
     P.touched = (c->block - 1 + b->max_new - 1) / c->block + 1;
     const int64_t rows = a->q ? (int64_t)b->max_new * a->n_heads : 0;
     const int64_t per = kApWarps * kApQRows;
