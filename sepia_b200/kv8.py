@@ -23,24 +23,33 @@ from .lib import SepiaKv8Append, SepiaKv8Attn, SepiaKv8Cache, SepiaKv8Step, last
 _F16 = {torch.float32: 0, torch.float16: 1}
 
 
-def _need(cond, what):
-    if not cond:
-        raise ValueError(f"sepia_b200: kv8: {what}")
+def _fail(what):
+    raise ValueError(f"sepia_b200: kv8: {what}")
 
 
-def _check(t, name, dtype, shape=None):
-    _need(t.is_cuda and t.is_contiguous() and t.dtype == dtype, f"{name} must be a contiguous CUDA tensor of {dtype}")
-    _need(shape is None or tuple(t.shape) == tuple(shape), f"{name} has shape {tuple(t.shape)}, expected {shape}")
+def _check(t, name, dtype, shape):
+    """The pointer of a contiguous CUDA tensor of this type and shape."""
+    if t.dtype is not dtype or not t.is_cuda or not t.is_contiguous():
+        _fail(f"{name} must be a contiguous CUDA tensor of {dtype}")
+    if t.shape != shape:
+        _fail(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     return t.data_ptr()
 
 
-def _rows(t, name, heads, dim, n):
+def _rows(t, name, dtype, heads, dim, n):
     """A [tokens, heads, dim] tensor whose heads lie side by side; returns (pointer, token stride)."""
-    _need(t.is_cuda and t.dtype in _F16, f"{name} must be a float32 or float16 CUDA tensor")
-    _need(tuple(t.shape) == (n, heads, dim), f"{name} has shape {tuple(t.shape)}, expected {(n, heads, dim)}")
-    st = t.stride()
-    _need(n == 0 or (st[2] == 1 and (heads == 1 or st[1] == dim)), f"the heads of {name} must lie side by side")
-    return t.data_ptr(), st[0] if n > 1 else heads * dim
+    if t.dtype is not dtype or not t.is_cuda:
+        _fail(f"{name} must be a CUDA tensor; q, k and v must have one type, float32 or float16")
+    if t.shape != (n, heads, dim):
+        _fail(f"{name} has shape {tuple(t.shape)}, expected {(n, heads, dim)}")
+    s0, s1, s2 = t.stride()
+    if n and (s2 != 1 or (heads > 1 and s1 != dim)):
+        _fail(f"the heads of {name} must lie side by side")
+    return t.data_ptr(), s0 if n > 1 else heads * dim
+
+
+def _stream(index, stream):
+    return torch._C._cuda_getCurrentRawStream(index) if stream is None else stream.cuda_stream
 
 
 def rotation_table(n_positions: int, rot_dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -59,7 +68,8 @@ class Kv8Step:
 
     def __init__(self, table, kv_len, start=None, slot=None, n_tokens=None, max_new=1, max_kv=None):
         n = kv_len.shape[0]
-        _need(table.dim() == 2, "table must have two dimensions")
+        if table.dim() != 2:
+            _fail("table must have two dimensions")
         st = SepiaKv8Step()
         st.table = _check(table, "table", torch.int32, (n, table.shape[1]))
         st.kv_len = _check(kv_len, "kv_len", torch.int32, (n,))
@@ -68,13 +78,13 @@ class Kv8Step:
         st.n_seqs, st.table_cols, st.max_new = n, table.shape[1], int(max_new)
         st.n_tokens = n if n_tokens is None else int(n_tokens)
         st.max_kv = -1 if max_kv is None else int(max_kv)
-        self.struct, self._keep = st, (table, kv_len, start, slot)
-        self.device = kv_len.device
+        self.n_tokens, self.struct, self._keep = st.n_tokens, st, (table, kv_len, start, slot)
+        self.device, self.index = kv_len.device, kv_len.device.index
         self._max_kv, self._bound, self._ws = max_kv, {}, {}
 
     def _for(self, cache):
         """The step as a struct for this cache's block size, by reference."""
-        b = cache.struct.block
+        b = cache.block
         r = self._bound.get(b)
         if r is None:
             st = SepiaKv8Step.from_buffer_copy(self.struct)
@@ -102,7 +112,8 @@ class Kv8Cache:
     block, head_dim]."""
 
     def __init__(self, k, v, k_scale, v_scale, k_tail, v_tail):
-        _need(k.dim() == 4 and k_tail.dim() == 4, "k and k_tail must have four dimensions")
+        if k.dim() != 4 or k_tail.dim() != 4:
+            _fail("k and k_tail must have four dimensions")
         n, hk, b, d = k.shape
         st = SepiaKv8Cache()
         st.n_blocks, st.n_slots, st.n_kv_heads, st.head_dim, st.block = n, k_tail.shape[0], hk, d, b
@@ -112,9 +123,10 @@ class Kv8Cache:
             setattr(st, name, _check(t, name, torch.float32, (n, hk)))
         for name, t in (("k_tail", k_tail), ("v_tail", v_tail)):
             setattr(st, name, _check(t, name, torch.float16, (k_tail.shape[0], hk, b, d)))
-        self.struct = st
+        self.struct, self.n_kv_heads, self.head_dim, self.block = st, hk, d, b
         self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail = k, v, k_scale, v_scale, k_tail, v_tail
-        self._ref, self._lib = C.byref(st), load()
+        self._ref, lib = C.byref(st), load()
+        self._append, self._attn = lib.sepia_cuda_kv8_append, lib.sepia_cuda_kv8_attn
 
     @classmethod
     def allocate(cls, n_blocks, n_slots, n_kv_heads, head_dim, block=32, device="cuda"):
@@ -136,33 +148,34 @@ class Kv8Cache:
         stride): norm of each head, rotation by position, 8 bits. With q, also
         norms, rotates and scales (q_scale float32 [n_tokens]) the queries into
         q_out, which is returned."""
-        c, n = self.struct, step.struct.n_tokens
+        d, hk, n, dt = self.head_dim, self.n_kv_heads, step.n_tokens, k.dtype
+        if dt not in _F16:
+            _fail("k must be float32 or float16")
         a = SepiaKv8Append()
-        a.x_f16 = _F16.get(k.dtype, 0)
-        a.k, a.k_stride = _rows(k, "k", c.n_kv_heads, c.head_dim, n)
-        a.v, a.v_stride = _rows(v, "v", c.n_kv_heads, c.head_dim, n)
-        _need(v.dtype == k.dtype, "k and v must have one type")
-        a.eps = eps
+        a.x_f16, a.eps = _F16[dt], eps
+        a.k, a.k_stride = _rows(k, "k", dt, hk, d, n)
+        a.v, a.v_stride = _rows(v, "v", dt, hk, d, n)
         if k_norm is not None:
-            a.k_norm = _check(k_norm, "k_norm", torch.float32, (c.head_dim,))
+            a.k_norm = _check(k_norm, "k_norm", torch.float32, (d,))
         if q is not None:
-            _need(q.dtype == k.dtype, "q and k must have one type")
-            h = q.shape[1]
-            a.n_heads = h
-            a.q, a.q_stride = _rows(q, "q", h, c.head_dim, n)
+            a.n_heads = h = q.shape[1]
+            a.q, a.q_stride = _rows(q, "q", dt, h, d, n)
             if q_out is None:
-                q_out = torch.empty((n, h, c.head_dim), dtype=q.dtype, device=q.device)
-            a.q_out = _check(q_out, "q_out", q.dtype, (n, h, c.head_dim))
+                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+                a.q_out = q_out.data_ptr()
+            else:
+                a.q_out = _check(q_out, "q_out", dt, (n, h, d))
             if q_norm is not None:
-                a.q_norm = _check(q_norm, "q_norm", torch.float32, (c.head_dim,))
+                a.q_norm = _check(q_norm, "q_norm", torch.float32, (d,))
             if q_scale is not None:
                 a.q_scale = _check(q_scale, "q_scale", torch.float32, (n,))
         if rotation is not None:
-            _need(rotation.dim() == 3 and rotation.shape[2] == 2, "rotation must be [positions, rot_dim/2, 2]")
-            a.rotation = _check(rotation, "rotation", torch.float32)
-            a.rot_positions, a.rot_dim, a.rot_adjacent = rotation.shape[0], 2 * rotation.shape[1], int(adjacent)
-        st = stream if stream is not None else torch.cuda.current_stream(step.device)
-        if not self._lib.sepia_cuda_kv8_append(self._ref, step._for(self), C.byref(a), st.cuda_stream):
+            r = rotation.shape
+            if len(r) != 3 or r[2] != 2:
+                _fail("rotation must be [positions, rot_dim/2, 2]")
+            a.rotation = _check(rotation, "rotation", torch.float32, r)
+            a.rot_positions, a.rot_dim, a.rot_adjacent = r[0], 2 * r[1], adjacent
+        if not self._append(self._ref, step._for(self), a, _stream(step.index, stream)):
             raise RuntimeError(f"sepia_b200: kv8_append failed: {last_error()}")
         return q_out
 
@@ -170,22 +183,26 @@ class Kv8Cache:
         """Causal attention of the new tokens (after append) over what the
         cache holds of their sequences. rel_logits float32 [n_tokens, heads,
         extent] is added at distance 0 .. extent-1, times tau[token]."""
-        c, n = self.struct, step.struct.n_tokens
-        _need(q.dim() == 3, "q must be [tokens, heads, head_dim]")
-        h = q.shape[1]
+        d, n, dt = self.head_dim, step.n_tokens, q.dtype
+        if dt not in _F16 or q.dim() != 3:
+            _fail("q must be float32 or float16 [tokens, heads, head_dim]")
         a = SepiaKv8Attn()
-        a.x_f16, a.n_heads, a.scale, a.window = _F16.get(q.dtype, 0), h, scale, window
-        a.q, a.q_stride = _rows(q, "q", h, c.head_dim, n)
+        a.n_heads = h = q.shape[1]
+        a.x_f16, a.scale, a.window = _F16[dt], scale, window
+        a.q, a.q_stride = _rows(q, "q", dt, h, d, n)
         if out is None:
-            out = torch.empty((n, h, c.head_dim), dtype=q.dtype, device=q.device)
-        a.out = _check(out, "out", q.dtype, (n, h, c.head_dim))
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            a.out = out.data_ptr()
+        else:
+            a.out = _check(out, "out", dt, (n, h, d))
         if rel_logits is not None:
-            a.rel_extent = rel_logits.shape[-1]
-            a.rel_logits = _check(rel_logits, "rel_logits", torch.float32, (n, h, a.rel_extent))
+            e = rel_logits.shape[-1]
+            a.rel_logits = _check(rel_logits, "rel_logits", torch.float32, (n, h, e))
+            a.rel_extent = e
         if tau is not None:
             a.tau = _check(tau, "tau", torch.float32, (n,))
-        st = (stream if stream is not None else torch.cuda.current_stream(step.device)).cuda_stream
-        ws = step.workspace(self, a, (st, a.x_f16, h, c.n_kv_heads, c.head_dim, c.block, window))
-        if not self._lib.sepia_cuda_kv8_attn(self._ref, step._for(self), C.byref(a), ws[0], ws[1], st):
+        st = _stream(step.index, stream)
+        ws = step.workspace(self, a, (st, a.x_f16, h, self.n_kv_heads, d, self.block, window))
+        if not self._attn(self._ref, step._for(self), a, ws[0], ws[1], st):
             raise RuntimeError(f"sepia_b200: kv8_attn failed: {last_error()}")
         return out

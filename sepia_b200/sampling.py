@@ -9,10 +9,8 @@ from .lib import last_error, load
 _F16 = {torch.float32: 0, torch.float16: 1}
 
 
-def _row_arg(t, name, dtype, n):
-    if t is None:
-        return None
-    if not (t.is_cuda and t.is_contiguous() and t.dtype == dtype and t.shape == (n,)):
+def _row(t, name, dtype, n):
+    if t.dtype is not dtype or not t.is_cuda or not t.is_contiguous() or t.shape != (n,):
         raise ValueError(f"sepia_b200: sample: {name} must be a contiguous CUDA tensor of {dtype}, one value per row")
     return t.data_ptr()
 
@@ -23,22 +21,28 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, ids=
     min_p (float32) and top_k (int32) hold a value per row; None turns one off.
     Returns (ids int32, prob float32): the tokens and their share of the
     weights that the filters left in; -1 and 0 where a row has no token."""
-    if not (logits.is_cuda and logits.dim() == 2 and logits.dtype in _F16):
+    f16 = _F16.get(logits.dtype)
+    if f16 is None or not logits.is_cuda or logits.dim() != 2:
         raise ValueError("sepia_b200: sample: logits must be a float32 or float16 CUDA tensor [rows, vocab]")
     n, v = logits.shape
-    if v > 1 and logits.stride(1) != 1:
+    s0, s1 = logits.stride()
+    if v > 1 and s1 != 1:
         raise ValueError("sepia_b200: sample: the logits of a row must lie side by side")
-    dev = logits.device
+    f, i = torch.float32, torch.int32
+    ids_p = _row(ids, "ids", i, n) if ids is not None else None
+    prob_p = _row(prob, "prob", f, n) if prob is not None else None
+    u_p = _row(u, "u", f, n)
     if ids is None:
-        ids = torch.empty(n, dtype=torch.int32, device=dev)
+        ids = torch.empty_like(u, dtype=i)
+        ids_p = ids.data_ptr()
     if prob is None:
-        prob = torch.empty(n, dtype=torch.float32, device=dev)
-    st = (stream if stream is not None else torch.cuda.current_stream(dev)).cuda_stream
-    f = torch.float32
-    if not load().sepia_cuda_sample(_F16[logits.dtype], logits.data_ptr(), logits.stride(0) if n > 1 else v, n, v,
-                                    _row_arg(u, "u", f, n), _row_arg(temperature, "temperature", f, n),
-                                    _row_arg(top_k, "top_k", torch.int32, n), _row_arg(top_p, "top_p", f, n),
-                                    _row_arg(min_p, "min_p", f, n), _row_arg(ids, "ids", torch.int32, n),
-                                    _row_arg(prob, "prob", f, n), st):
+        prob = torch.empty_like(u)
+        prob_p = prob.data_ptr()
+    st = stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(logits.device.index)
+    if not load().sepia_cuda_sample(f16, logits.data_ptr(), s0 if n > 1 else v, n, v, u_p,
+                                    None if temperature is None else _row(temperature, "temperature", f, n),
+                                    None if top_k is None else _row(top_k, "top_k", i, n),
+                                    None if top_p is None else _row(top_p, "top_p", f, n),
+                                    None if min_p is None else _row(min_p, "min_p", f, n), ids_p, prob_p, st):
         raise RuntimeError(f"sepia_b200: sample failed: {last_error()}")
     return ids, prob
