@@ -87,6 +87,12 @@ typedef struct SepiaModel SepiaModel;
  * histories and scratch on the current device, and computes the tau table
  * (double, per position). The layer array is copied; weights are not. */
 int sepia_model_create(const SepiaModelDesc *d, SepiaModel **out);
+/* The same engine over the paged 8-bit K/V cache of sepia_cuda.h
+ * (SepiaKv8Cache), in blocks of 16, 32 or 64 tokens: a quarter of the fp32
+ * cache's memory. Every layer's head_dim must be a multiple of 16. Keys and
+ * values are rounded to e4m3 (2^-4 relative), so logits differ from the fp32
+ * cache's and greedy ids need not be the same. */
+int sepia_model_create_kv8(const SepiaModelDesc *d, int32_t block, SepiaModel **out);
 void sepia_model_destroy(SepiaModel *m);
 /* Device bytes the engine allocated (caches + scratch). */
 size_t sepia_model_device_bytes(const SepiaModel *m);
@@ -103,6 +109,16 @@ int sepia_model_prefill(SepiaModel *m, const int32_t *ids, int32_t n, int32_t wa
  * the argmax of its logits. Replays a CUDA graph captured on first use
  * (capture happens on `stream`; make the first call outside any capture). */
 int sepia_model_decode(SepiaModel *m, int32_t n, int32_t *out_ids, void *stream);
+/* Sampled decode: sepia_cuda_sample in place of the argmax, with one setting
+ * for the sequence (temperature <= 0: greedy; top_k 0, top_p >= 1, min_p <= 0:
+ * off) and one given uniform number per draw (DEVICE floats in [0, 1)).
+ * draw: the pending token from the last logits (of a prefill, say) and u[0].
+ * decode_sampled: as sepia_model_decode, each step drawing the next token with
+ * u[i]; its own graph is captured on first use and kept while out_ids and u
+ * are the same arrays. Settings are read on the device at each step. */
+int sepia_model_set_sampling(SepiaModel *m, float temperature, int32_t top_k, float top_p, float min_p, void *stream);
+int sepia_model_draw(SepiaModel *m, const float *u, void *stream);
+int sepia_model_decode_sampled(SepiaModel *m, int32_t n, int32_t *out_ids, const float *u, void *stream);
 /* Device pointer to the last computed logits [unpadded_vocab]. */
 const float *sepia_model_logits(const SepiaModel *m);
 /* Copies the last logits into dst (device, unpadded_vocab floats). */

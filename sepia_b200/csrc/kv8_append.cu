@@ -60,7 +60,7 @@ __device__ __forceinline__ __half sat_half(__half h) {
     return (u & 0x7fffu) == 0x7c00u ? __ushort_as_half((unsigned short)(u - 1u)) : h;
 }
 __device__ __forceinline__ __half to_half(float x) { return sat_half(__float2half_rn(x)); }
-__device__ __forceinline__ __half to_half(double x) { return sat_half(__double2half(x)); }
+__device__ __forceinline__ __half to_half(double x) { return sat_half(__float2half_rn((float)x)); }
 
 // The smallest power of two s with amax / s <= 448 = 1.75 * 2^8. amax is the
 // magnitude of an fp16 number, so it is a normal fp32 number or zero.
@@ -80,8 +80,8 @@ __device__ __forceinline__ double inv_rms(double s, double inv_dh, float eps) {
 
 // RMS norm of the warp's row (w: the lane's weights), then the rotation; a
 // lane owns dims 4*lane ..+3. Queries are worked out in fp32, keys in fp64:
-// a key is rounded to fp16 and then to 8 bits, and only with the exact value
-// at hand are these the roundings of the key itself.
+// a key is rounded to fp16 and then to 8 bits, and with fp32 noise before
+// them some of these roundings would go the other way.
 template <typename R>
 __device__ __forceinline__ void norm_rotate(R (&x)[4], const float *w, const SepiaKv8Append &a, double inv_dh, const float2 *cs) {
     const int lane = threadIdx.x & 31, d = 4 * lane;

@@ -13,7 +13,11 @@
 //      -> k_residual: MLP-output short convolution + residual, then the next
 //         layer's attention norm (or the final norm / mup for the head)
 // then the logits head (matvec_q over the unpadded rows) and k_argmax, whose
-// 64-bit (value, index) key feeds the next step's k_embed. Token ids,
+// 64-bit (value, index) key feeds the next step's k_embed. With the 8-bit
+// cache (sepia_model_create_kv8) k_attn_prep only convolves K and V and
+// works out the band; sepia_cuda_kv8_append norms, scales and stores, and
+// sepia_cuda_kv8_attn reads. A sampled step draws the next token
+// (sepia_cuda_sample) where a greedy one takes the argmax. Token ids,
 // positions and the argmax live in device memory, so a decode step needs no
 // host value and is replayed from one CUDA graph.
 #include "../../include/sepia_model.h"
@@ -54,6 +58,9 @@ struct ModelState {
     int32_t bad_token;         // set when an input token id is out of range
     int64_t kv_lo, kv_hi;      // attention range of the current token (this layer)
     double tau;                // tau of the current token (this layer)
+    float tau_f;               // the same in fp32 (8-bit cache)
+    float u;                   // number of the draw in hand (sampled steps)
+    int32_t drawn;             // its token
 };
 
 // ------------------------------------------------------------ reductions
@@ -200,6 +207,9 @@ struct PrepArgs {
     const float *r_vec, *rel_proj;
     float *rel_logits;
     int d_rel, E;
+    // 8-bit cache: the convolved K and V rows go here, un-normed, and the
+    // query heads are left to sepia_cuda_kv8_append
+    float *k_conv, *v_conv;
 };
 
 // Depthwise causal convolution of one channel at T = 1 with its history,
@@ -244,6 +254,10 @@ __global__ void __launch_bounds__(128) k_attn_prep(const PrepArgs A) {
     const double tau = (A.is_sliding || !A.tau_table) ? 1.0 : A.tau_table[pos];
     if ((int)blockIdx.x < A.H) {
         const int h = blockIdx.x;
+        if (A.k_conv) {
+            if (h == 0 && d == 0) A.st->tau_f = (float)tau;
+            return;
+        }
         const float qw = d < A.Dh ? A.q_norm[d] : 0.0f;
         if (d < A.Dh) v_sm[d] = A.q_raw[(int64_t)h * A.Dh + d];
         __syncthreads();
@@ -267,9 +281,15 @@ __global__ void __launch_bounds__(128) k_attn_prep(const PrepArgs A) {
     if (d < A.Dh) {
         kv = sconv1(A.k_sconv, A.k_hist, A.kv_dim, A.K, c, A.k_raw[c]);
         const float vv = sconv1(A.v_sconv, A.v_hist, A.kv_dim, A.K, c, A.v_raw[c]);
-        A.v_cache[pos * A.kv_dim + c] = vv;
-        v_sm[d] = kv;
+        if (A.k_conv) {
+            A.k_conv[c] = kv;
+            A.v_conv[c] = vv;
+        } else {
+            A.v_cache[pos * A.kv_dim + c] = vv;
+            v_sm[d] = kv;
+        }
     }
+    if (A.k_conv) return;
     __syncthreads();
     const float inv = rms_inv(v_sm, A.Dh, A.eps, sh);
     if (d < A.Dh) A.k_cache[pos * A.kv_dim + c] = __fmul_rn(kw, __fmul_rn(kv, inv));
@@ -372,6 +392,26 @@ __global__ void __launch_bounds__(256) k_argmax(const float *logits, int32_t n, 
     }
 }
 
+// Sampled steps: the number for the draw after generated token `gen - 1`, and
+// the drawn token as the pending one (a row without any token: 0 and the
+// error word).
+__global__ void k_draw_number(const float *u, ModelState *st, int in_step) {
+    griddep_wait();
+    griddep_launch();
+    st->u = u[in_step ? st->gen - 1 : 0];
+}
+__global__ void k_draw_take(ModelState *st, int advance, int *err) {
+    griddep_wait();
+    griddep_launch();
+    int32_t id = st->drawn;
+    if (id < 0) {
+        id = 0;
+        set_error(err, kErrBadArgs);
+    }
+    st->best = (1ull << 63) | (unsigned long long)(0xFFFFFFFFu - (uint32_t)id);
+    st->pos += advance;
+}
+
 __global__ void k_state_reset(ModelState *st) {
     st->best = 0ull;
     st->pos = 0;
@@ -414,6 +454,21 @@ struct SepiaModel {
     // expert sharding (world > 1)
     int rank = 0, world = 1;
     SepiaExchange *xchg = nullptr;   // the sharded MoE layers' exchange
+    // 8-bit cache (kv_block > 0): one sequence, its blocks in order
+    int kv_block = 0;
+    std::vector<SepiaKv8Cache> c8;
+    SepiaKv8Step step8{};
+    int32_t *table8 = nullptr;
+    void *ws8 = nullptr;
+    size_t ws8_bytes = 0;
+    // sampled steps
+    float *draw_f = nullptr;         // temperature, top_p, min_p
+    int32_t *draw_k = nullptr;       // top_k
+    bool draw_set = false;
+    cudaGraph_t graph_s = nullptr;
+    cudaGraphExec_t exec_s = nullptr;
+    int32_t *graph_s_out = nullptr;
+    const float *graph_s_u = nullptr;
 };
 
 namespace {
@@ -454,9 +509,42 @@ int mv(const SepiaQTensor &t, const float *x, float *y, int64_t rows, cudaStream
     return launch_matvec_q(t.type, t.data, x, y, rows, t.cols, 1, st);
 }
 
+SepiaKv8Attn attn8(const SepiaModel *m, const SepiaModelLayer &L) {
+    SepiaKv8Attn a = {};
+    a.n_heads = L.n_heads; a.q = m->qs; a.q_stride = (int64_t)L.n_heads * L.head_dim; a.out = m->att;
+    a.scale = (float)(1.0 / L.head_dim); a.window = L.is_sliding ? m->d.window : 0;
+    a.rel_extent = L.rel_extent; a.rel_logits = m->rl; a.tau = &m->st->tau_f;
+    return a;
+}
+
+// Attention of layer l over the 8-bit cache, after k_attn_prep
+int attention8(SepiaModel *m, int l, cudaStream_t st) {
+    const SepiaModelLayer &L = m->layers[l];
+    SepiaKv8Append a = {};
+    a.n_heads = L.n_heads;
+    a.k = m->k; a.v = m->v; a.k_stride = a.v_stride = (int64_t)L.n_kv_heads * L.head_dim;
+    a.q = m->q; a.q_stride = (int64_t)L.n_heads * L.head_dim; a.q_out = m->qs;
+    a.k_norm = L.k_norm; a.q_norm = L.q_norm; a.q_scale = &m->st->tau_f; a.eps = m->d.eps;
+    const SepiaKv8Attn t = attn8(m, L);
+    return sepia_cuda_kv8_append(&m->c8[l], &m->step8, &a, (void *)st) &&
+           sepia_cuda_kv8_attn(&m->c8[l], &m->step8, &t, m->ws8, m->ws8_bytes, (void *)st);
+}
+
+// The pending token from the last logits and number u[0] (or, inside a
+// decode step, the step's own number)
+int draw(SepiaModel *m, const float *u, int in_step, cudaStream_t st) {
+    if (!check(launch_pdl(k_draw_number, 1, 1, 0, st, u, m->st, in_step), "model: draw launch")) return 0;
+    const int32_t V = m->d.unpadded_vocab;
+    if (!sepia_cuda_sample(0, m->logits, V, 1, V, &m->st->u, m->draw_f, m->draw_k, m->draw_f + 1, m->draw_f + 2,
+                           &m->st->drawn, nullptr, (void *)st))
+        return 0;
+    return check(launch_pdl(k_draw_take, 1, 1, 0, st, m->st, in_step, dev_info().err), "model: draw launch");
+}
+
 // Everything of one token after its embedding: the layers, then (want_logits)
-// the head and the argmax. `last_advance`: which kernel moves pos.
-int run_layers(SepiaModel *m, bool want_logits, cudaStream_t st) {
+// the head and the argmax, or with u the draw. `last_advance`: which kernel
+// moves pos.
+int run_layers(SepiaModel *m, bool want_logits, cudaStream_t st, const float *u = nullptr) {
     const SepiaModelDesc &d = m->d;
     const int64_t hidden = d.hidden;
     const int K = d.conv_k;
@@ -482,14 +570,19 @@ int run_layers(SepiaModel *m, bool want_logits, cudaStream_t st) {
         P.st = m->st;
         P.r_vec = m->r; P.rel_proj = L.rel_proj; P.rel_logits = m->rl; P.d_rel = (int)d.d_rel;
         P.E = L.rel_extent;
+        P.k_conv = m->kv_block ? m->k : nullptr;
+        P.v_conv = m->v;
         if (L.rel_extent <= 0 || d.d_rel <= 0 || !L.rel_proj) return fail("model: layer %d has no relative band", l);
         const unsigned rel_blocks = (unsigned)(((int64_t)H * L.rel_extent + 127) / 128);
         launch_pdl(k_attn_prep, (unsigned)(H + Hkv) + rel_blocks, 128, 0, st, P);
         if (!check(cudaGetLastError(), "model: attn_prep launch")) return 0;
-        if (!launch_banded_attn_ex(0, m->qs, m->kc[l], m->vc[l], m->rl, m->att, &m->st->kv_lo, &m->st->kv_hi,
+        if (m->kv_block) {
+            if (!attention8(m, l, st)) return 0;
+        } else if (!launch_banded_attn_ex(0, m->qs, m->kc[l], m->vc[l], m->rl, m->att, &m->st->kv_lo, &m->st->kv_hi,
                                    nullptr, &m->st->tau, &m->st->pos, 1, H, Hkv, Dh, L.rel_extent, 0, kv_dim,
-                                   (float)(1.0 / Dh), m->splits[l], m->part, st))
+                                   (float)(1.0 / Dh), m->splits[l], m->part, st)) {
             return 0;
+        }
         if (!mv(L.wo, m->att, m->blk, hidden, st)) return 0;
         ResArgs R;
         R.x = m->x; R.in = m->blk; R.scale = 1.0f; R.use_scale = 0; R.w = L.attn_sconv; R.hist = m->ah[l];
@@ -517,6 +610,7 @@ int run_layers(SepiaModel *m, bool want_logits, cudaStream_t st) {
     if (want_logits) {
         if (!launch_matvec_q(d.unembed.type, d.unembed.data, m->xn, m->logits, d.unpadded_vocab, hidden, 1, st))
             return 0;
+        if (u) return draw(m, u, 1, st);
         const int sms = dev_info().sm_count > 0 ? dev_info().sm_count : 148;
         launch_pdl(k_argmax, (unsigned)sms, 256, 0, st, (const float *)m->logits, d.unpadded_vocab, m->st, 1);
         if (!check(cudaGetLastError(), "model: argmax launch")) return 0;
@@ -541,9 +635,11 @@ int setup_kernels(const SepiaModelDesc &d) {
 
 }  // namespace
 
-extern "C" int sepia_model_create(const SepiaModelDesc *d, SepiaModel **out) {
+static int model_create(const SepiaModelDesc *d, int kv_block, SepiaModel **out) {
     if (!d || !out) return fail("model: null argument");
     *out = nullptr;
+    if (kv_block && kv_block != 16 && kv_block != 32 && kv_block != 64)
+        return fail("model: 8-bit cache in blocks of %d tokens (16, 32 or 64)", kv_block);
     if (d->n_layers <= 0 || !d->layers) return fail("model: no layers");
     if (d->hidden <= 0 || d->hidden % 32 || d->hidden > 8 * kClThreads * kClusterCtas ||
         (d->hidden + kClusterCtas - 1) / kClusterCtas > kClThreads)
@@ -557,6 +653,7 @@ extern "C" int sepia_model_create(const SepiaModelDesc *d, SepiaModel **out) {
     if (d->mup == 0.0f) return fail("model: mup multiplier is zero");
     SepiaModel *m = new SepiaModel();
     m->d = *d;
+    m->kv_block = kv_block;
     m->layers.assign(d->layers, d->layers + d->n_layers);
     m->d.layers = m->layers.data();
     const int64_t hidden = d->hidden;
@@ -570,6 +667,8 @@ extern "C" int sepia_model_create(const SepiaModelDesc *d, SepiaModel **out) {
         if (L.n_heads <= 0 || L.n_kv_heads <= 0 || L.n_heads % L.n_kv_heads || L.head_dim <= 0 || L.head_dim > 128 ||
             L.rel_extent <= 0)
             { ok = fail("model: layer %d: bad attention geometry", l); break; }
+        if (kv_block && L.head_dim % 16)
+            { ok = fail("model: layer %d: the 8-bit cache needs head_dim %d to be a multiple of 16", l, L.head_dim); break; }
         const int64_t q_dim = (int64_t)L.n_heads * L.head_dim, kv_dim = (int64_t)L.n_kv_heads * L.head_dim;
         const int64_t r_dim = (int64_t)L.n_heads * d->d_rel;
         ok = check_q(L.wq, q_dim, hidden, "attn_q", l) && check_q(L.wk, kv_dim, hidden, "attn_k", l) &&
@@ -638,13 +737,35 @@ extern "C" int sepia_model_create(const SepiaModelDesc *d, SepiaModel **out) {
     add((void **)&m->g, 4 * std::max<int64_t>(1, m->max_ff)); add((void **)&m->u, 4 * std::max<int64_t>(1, m->max_ff));
     add((void **)&m->h, 4 * std::max<int64_t>(1, m->max_ff));
     add((void **)&m->logits, 4 * (size_t)d->unpadded_vocab);
-    add((void **)&m->part, part);
+    add((void **)&m->part, kv_block ? 0 : part);
+    add((void **)&m->draw_f, 3 * sizeof(float)); add((void **)&m->draw_k, sizeof(int32_t));
+    const int64_t blocks8 = kv_block ? (cap + kv_block - 1) / kv_block : 0;
+    if (kv_block) {
+        m->c8.resize(d->n_layers);
+        add((void **)&m->table8, sizeof(int32_t) * blocks8);
+        m->step8.n_seqs = m->step8.n_tokens = m->step8.max_new = 1;
+        m->step8.max_kv = (int32_t)cap;
+        m->step8.table_cols = (int32_t)blocks8;
+        for (int l = 0; l < d->n_layers; l++) {
+            SepiaKv8Cache &c = m->c8[l];
+            c.n_blocks = (int32_t)blocks8; c.n_slots = 1; c.n_kv_heads = m->layers[l].n_kv_heads;
+            c.head_dim = m->layers[l].head_dim; c.block = kv_block;
+        }
+    }
     add((void **)&m->moe_ws_mem, std::max<size_t>(moe_ws, 256));
     m->kc.resize(d->n_layers); m->vc.resize(d->n_layers); m->kh.resize(d->n_layers); m->vh.resize(d->n_layers);
     m->ah.resize(d->n_layers); m->mh.resize(d->n_layers);
     for (int l = 0; l < d->n_layers; l++) {
         const int64_t kv_dim = (int64_t)m->layers[l].n_kv_heads * m->layers[l].head_dim;
-        add((void **)&m->kc[l], 4 * cap * kv_dim); add((void **)&m->vc[l], 4 * cap * kv_dim);
+        if (kv_block) {
+            SepiaKv8Cache &c = m->c8[l];
+            const size_t codes = (size_t)blocks8 * kv_block * kv_dim, scales = 4 * (size_t)blocks8 * c.n_kv_heads;
+            add(&c.k, codes); add(&c.v, codes);
+            add((void **)&c.k_scale, scales); add((void **)&c.v_scale, scales);
+            add(&c.k_tail, 2 * kv_block * kv_dim); add(&c.v_tail, 2 * kv_block * kv_dim);
+        } else {
+            add((void **)&m->kc[l], 4 * cap * kv_dim); add((void **)&m->vc[l], 4 * cap * kv_dim);
+        }
         add((void **)&m->kh[l], 4 * std::max(1, K - 1) * kv_dim); add((void **)&m->vh[l], 4 * std::max(1, K - 1) * kv_dim);
         add((void **)&m->ah[l], 4 * std::max(1, K - 1) * hidden); add((void **)&m->mh[l], 4 * std::max(1, K - 1) * hidden);
     }
@@ -655,6 +776,24 @@ extern "C" int sepia_model_create(const SepiaModelDesc *d, SepiaModel **out) {
     size_t off = 0;
     for (auto &p : plan) { *p.first = (char *)m->mem + off; off += p.second; }
     if (!check(cudaMemset(m->mem, 0, total), "model: clear")) { sepia_model_destroy(m); return 0; }
+    if (kv_block) {
+        std::vector<int32_t> ids(blocks8);
+        for (int64_t b = 0; b < blocks8; b++) ids[b] = (int32_t)b;
+        m->step8.table = m->table8;
+        m->step8.kv_len = &m->st->pos;
+        for (int l = 0; l < d->n_layers; l++) {
+            const SepiaKv8Attn t = attn8(m, m->layers[l]);
+            const size_t b = sepia_cuda_kv8_attn_ws_bytes(&m->c8[l], &m->step8, &t);
+            if (!b) { sepia_model_destroy(m); return 0; }
+            m->ws8_bytes = std::max(m->ws8_bytes, b);
+        }
+        if (!check(cudaMalloc(&m->ws8, m->ws8_bytes), "model: cudaMalloc") ||
+            !check(cudaMemcpy(m->table8, ids.data(), sizeof(int32_t) * blocks8, cudaMemcpyHostToDevice), "model: block table")) {
+            sepia_model_destroy(m);
+            return 0;
+        }
+        m->mem_bytes += m->ws8_bytes;
+    }
     if (moe0 && !sepia_cuda_moe_work_carve(moe0, m->moe_ws_mem, moe_ws, &m->ws)) { sepia_model_destroy(m); return 0; }
     // tau per position in double, as attn_forward_chunk computes it
     // (src/sepia.c:1188-1194), with the host's libm log
@@ -674,10 +813,20 @@ extern "C" int sepia_model_create(const SepiaModelDesc *d, SepiaModel **out) {
     return 1;
 }
 
+extern "C" int sepia_model_create(const SepiaModelDesc *d, SepiaModel **out) { return model_create(d, 0, out); }
+
+extern "C" int sepia_model_create_kv8(const SepiaModelDesc *d, int32_t block, SepiaModel **out) {
+    if (block == 0) return fail("model: 8-bit cache in blocks of 0 tokens (16, 32 or 64)");
+    return model_create(d, block, out);
+}
+
 extern "C" void sepia_model_destroy(SepiaModel *m) {
     if (!m) return;
     if (m->exec) cudaGraphExecDestroy(m->exec);
     if (m->graph) cudaGraphDestroy(m->graph);
+    if (m->exec_s) cudaGraphExecDestroy(m->exec_s);
+    if (m->graph_s) cudaGraphDestroy(m->graph_s);
+    if (m->ws8) cudaFree(m->ws8);
     if (m->mem) cudaFree(m->mem);
     if (m->xchg) sepia_cuda_exchange_destroy(m->xchg);
     delete m;
@@ -703,8 +852,9 @@ extern "C" int sepia_model_reset(SepiaModel *m, void *stream) {
     for (int l = 0; l < d.n_layers; l++) {
         const int64_t kv_dim = (int64_t)m->layers[l].n_kv_heads * m->layers[l].head_dim;
         const int64_t km1 = std::max<int64_t>(1, K - 1);
-        if (!check(cudaMemsetAsync(m->kc[l], 0, 4 * cap * kv_dim, st), "model: reset") ||
-            !check(cudaMemsetAsync(m->vc[l], 0, 4 * cap * kv_dim, st), "model: reset") ||
+        // (the 8-bit cache is never read where it has not been written)
+        if ((!m->kv_block && (!check(cudaMemsetAsync(m->kc[l], 0, 4 * cap * kv_dim, st), "model: reset") ||
+                              !check(cudaMemsetAsync(m->vc[l], 0, 4 * cap * kv_dim, st), "model: reset"))) ||
             !check(cudaMemsetAsync(m->kh[l], 0, 4 * km1 * kv_dim, st), "model: reset") ||
             !check(cudaMemsetAsync(m->vh[l], 0, 4 * km1 * kv_dim, st), "model: reset") ||
             !check(cudaMemsetAsync(m->ah[l], 0, 4 * km1 * hidden, st), "model: reset") ||
@@ -726,22 +876,23 @@ extern "C" int sepia_model_prefill(SepiaModel *m, const int32_t *ids, int32_t n,
     return 1;
 }
 
-extern "C" int sepia_model_decode(SepiaModel *m, int32_t n, int32_t *out_ids, void *stream) {
-    if (!m || !out_ids || n <= 0) return fail("model: decode needs out_ids and n > 0");
-    cudaStream_t st = as_stream(stream);
+// n steps, replayed from a graph kept in (graph, exec) while its arrays are
+// the same; with u each step draws, without it takes the argmax.
+static int decode_steps(SepiaModel *m, int32_t n, int32_t *out_ids, const float *u, cudaGraph_t &graph,
+                        cudaGraphExec_t &exec, bool same, cudaStream_t st) {
     k_state_new_call<<<1, 1, 0, st>>>(m->st);
     if (!check(cudaGetLastError(), "model: decode")) return 0;
-    if (m->exec && m->graph_out != out_ids) {
-        cudaGraphExecDestroy(m->exec);
-        cudaGraphDestroy(m->graph);
-        m->exec = nullptr;
-        m->graph = nullptr;
+    if (exec && !same) {
+        cudaGraphExecDestroy(exec);
+        cudaGraphDestroy(graph);
+        exec = nullptr;
+        graph = nullptr;
     }
     int32_t i0 = 0;
-    if (!m->exec) {
+    if (!exec) {
         // The first step runs eagerly (it sets every kernel's attributes
         // outside any capture), the rest replay its captured twin.
-        if (!embed(m, 1, nullptr, out_ids, st) || !run_layers(m, true, st)) return 0;
+        if (!embed(m, 1, nullptr, out_ids, st) || !run_layers(m, true, st, u)) return 0;
         i0 = 1;
         cudaStream_t cs;
         if (!check(cudaStreamCreateWithFlags(&cs, cudaStreamNonBlocking), "model: capture stream")) return 0;
@@ -749,19 +900,51 @@ extern "C" int sepia_model_decode(SepiaModel *m, int32_t n, int32_t *out_ids, vo
             cudaStreamDestroy(cs);
             return 0;
         }
-        int ok = embed(m, 1, nullptr, out_ids, cs) && run_layers(m, true, cs);
+        int ok = embed(m, 1, nullptr, out_ids, cs) && run_layers(m, true, cs, u);
         cudaGraph_t g = nullptr;
         const cudaError_t e = cudaStreamEndCapture(cs, &g);
         cudaStreamDestroy(cs);
         if (!ok) { if (g) cudaGraphDestroy(g); return 0; }
         if (!check(e, "model: end capture")) return 0;
-        if (!check(cudaGraphInstantiate(&m->exec, g, 0), "model: graph instantiate")) { cudaGraphDestroy(g); return 0; }
-        m->graph = g;
-        m->graph_out = out_ids;
+        if (!check(cudaGraphInstantiate(&exec, g, 0), "model: graph instantiate")) { cudaGraphDestroy(g); return 0; }
+        graph = g;
     }
     for (int32_t i = i0; i < n; i++)
-        if (!check(cudaGraphLaunch(m->exec, st), "model: graph launch")) return 0;
+        if (!check(cudaGraphLaunch(exec, st), "model: graph launch")) return 0;
     return 1;
+}
+
+extern "C" int sepia_model_decode(SepiaModel *m, int32_t n, int32_t *out_ids, void *stream) {
+    if (!m || !out_ids || n <= 0) return fail("model: decode needs out_ids and n > 0");
+    const bool same = m->graph_out == out_ids;
+    m->graph_out = out_ids;
+    return decode_steps(m, n, out_ids, nullptr, m->graph, m->exec, same, as_stream(stream));
+}
+
+extern "C" int sepia_model_set_sampling(SepiaModel *m, float temperature, int32_t top_k, float top_p, float min_p,
+                                        void *stream) {
+    if (!m) return fail("model: null model");
+    const float f[3] = {temperature, top_p, min_p};
+    if (!check(cudaMemcpyAsync(m->draw_f, f, sizeof f, cudaMemcpyHostToDevice, as_stream(stream)), "model: sampling") ||
+        !check(cudaMemcpyAsync(m->draw_k, &top_k, sizeof top_k, cudaMemcpyHostToDevice, as_stream(stream)), "model: sampling"))
+        return 0;
+    m->draw_set = true;
+    return 1;
+}
+
+extern "C" int sepia_model_draw(SepiaModel *m, const float *u, void *stream) {
+    if (!m || !u) return fail("model: draw needs u");
+    if (!m->draw_set) return fail("model: draw before sepia_model_set_sampling");
+    return draw(m, u, 0, as_stream(stream));
+}
+
+extern "C" int sepia_model_decode_sampled(SepiaModel *m, int32_t n, int32_t *out_ids, const float *u, void *stream) {
+    if (!m || !out_ids || !u || n <= 0) return fail("model: decode_sampled needs out_ids, u and n > 0");
+    if (!m->draw_set) return fail("model: decode_sampled before sepia_model_set_sampling");
+    const bool same = m->graph_s_out == out_ids && m->graph_s_u == u;
+    m->graph_s_out = out_ids;
+    m->graph_s_u = u;
+    return decode_steps(m, n, out_ids, u, m->graph_s, m->exec_s, same, as_stream(stream));
 }
 
 extern "C" const float *sepia_model_logits(const SepiaModel *m) { return m ? m->logits : nullptr; }

@@ -178,11 +178,15 @@ _PROTOS = {
     "sepia_cuda_fill_blocks": (C.c_int, [C.c_int, vp, i64, i64, i64, C.c_uint64, i64, i64, C.c_float, C.c_float, vp]),
     # ---- sepia_model.h (whole-token decode engine) ----
     "sepia_model_create": (C.c_int, [C.POINTER(SepiaModelDesc), C.POINTER(vp)]),
+    "sepia_model_create_kv8": (C.c_int, [C.POINTER(SepiaModelDesc), i32, C.POINTER(vp)]),
     "sepia_model_destroy": (None, [vp]),
     "sepia_model_device_bytes": (C.c_size_t, [vp]),
     "sepia_model_reset": (C.c_int, [vp, vp]),
     "sepia_model_prefill": (C.c_int, [vp, vp, i32, i32, vp]),
     "sepia_model_decode": (C.c_int, [vp, i32, vp, vp]),
+    "sepia_model_set_sampling": (C.c_int, [vp, C.c_float, i32, C.c_float, C.c_float, vp]),
+    "sepia_model_draw": (C.c_int, [vp, vp, vp]),
+    "sepia_model_decode_sampled": (C.c_int, [vp, i32, vp, vp, vp]),
     "sepia_model_logits": (vp, [vp]),
     "sepia_model_copy_logits": (C.c_int, [vp, vp, vp]),
     "sepia_model_exchange_handle": (C.c_int, [vp, vp]),

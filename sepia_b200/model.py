@@ -12,11 +12,14 @@ native engine (include/sepia_model.h, csrc/model.cu).
       device (multi-GB synthetic models for the benchmark).
   generate(prompt, n_gen)           prefill + greedy decode, token ids in and
       out (real_generate's loop, src/sepia.c:4114-4158, without the
-      tokenizer).
+      tokenizer); with sampling=Sampling(...) and u the tokens are drawn.
+  kv_block=16, 32 or 64 holds K and V in the paged 8-bit cache
+      (include/sepia_cuda.h, SepiaKv8Cache) instead of fp32.
 """
 from __future__ import annotations
 
 import ctypes as C
+from dataclasses import dataclass
 
 import numpy as np
 import torch
@@ -31,9 +34,20 @@ def _pad256(n: int) -> int:
     return (n + 255) // 256 * 256
 
 
+@dataclass
+class Sampling:
+    """How a sampled decode draws (include/sepia_cuda.h, sepia_cuda_sample); the defaults are off."""
+    temperature: float = 1.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+
+
 class DeviceModel:
-    def __init__(self, cfg: ModelConfig, max_positions: int, rank: int = 0, world: int = 1, device="cuda"):
+    def __init__(self, cfg: ModelConfig, max_positions: int, rank: int = 0, world: int = 1, device="cuda",
+                 kv_block: int = 0):
         self.cfg = cfg
+        self.kv_block = int(kv_block)
         self.max_positions = int(max_positions)
         self.rank, self.world = rank, world
         self.device = torch.device(device)
@@ -43,9 +57,10 @@ class DeviceModel:
 
     # ------------------------------------------------------------ loading
     @classmethod
-    def from_container(cls, path, max_positions: int = 1024, rank: int = 0, world: int = 1, device="cuda"):
+    def from_container(cls, path, max_positions: int = 1024, rank: int = 0, world: int = 1, device="cuda",
+                       kv_block: int = 0):
         ct = Container(path)
-        m = cls(ct.cfg, max_positions, rank, world, device)
+        m = cls(ct.cfg, max_positions, rank, world, device, kv_block)
         for name in ct.tensors:
             t, shape, buf = ct.resident(name)
             m.t[name] = (t, shape, torch.from_numpy(np.array(buf)).to(m.device))
@@ -67,13 +82,13 @@ class DeviceModel:
 
     @classmethod
     def synthetic(cls, cfg: ModelConfig, types: ModelTypes | None = None, seed: int = 7, max_positions: int = 1024,
-                  rank: int = 0, world: int = 1, device="cuda"):
+                  rank: int = 0, world: int = 1, device="cuda", kv_block: int = 0):
         """Seeded random weights generated in HBM in BASELINE's
         distributions (sepia_cuda_fill_blocks for the quantized tensors).
         Every tensor and every routed expert has its own unit id, so a rank's
         shard holds the bytes those experts have on one GPU."""
         types = types or ModelTypes()
-        m = cls(cfg, max_positions, rank, world, device)
+        m = cls(cfg, max_positions, rank, world, device, kv_block)
         L = load()
         st = torch.cuda.current_stream(m.device).cuda_stream
         gen = torch.Generator(device=m.device)
@@ -203,7 +218,10 @@ class DeviceModel:
         d.rank, d.world = self.rank, self.world
         self._desc = d
         h = C.c_void_p()
-        ok(L.sepia_model_create(C.byref(d), C.byref(h)), "model_create")
+        if self.kv_block:
+            ok(L.sepia_model_create_kv8(C.byref(d), self.kv_block, C.byref(h)), "model_create_kv8")
+        else:
+            ok(L.sepia_model_create(C.byref(d), C.byref(h)), "model_create")
         self._h = h
 
     def __del__(self):
@@ -245,6 +263,22 @@ class DeviceModel:
         n = out_ids.numel() if n is None else n
         ok(load().sepia_model_decode(self._h, n, out_ids.data_ptr(), self._st(stream)), "model_decode")
 
+    def set_sampling(self, sampling: Sampling, stream=None):
+        ok(load().sepia_model_set_sampling(self._h, sampling.temperature, sampling.top_k, sampling.top_p,
+                                           sampling.min_p, self._st(stream)), "model_set_sampling")
+
+    def draw(self, u: torch.Tensor, stream=None):
+        """The pending token drawn from the last logits with u[0] (instead of their argmax)."""
+        assert u.dtype == torch.float32 and u.is_cuda and u.numel() >= 1
+        ok(load().sepia_model_draw(self._h, u.data_ptr(), self._st(stream)), "model_draw")
+
+    def decode_sampled(self, out_ids: torch.Tensor, u: torch.Tensor, stream=None):
+        """One step per element of out_ids; step i draws the next token with u[i]."""
+        assert out_ids.dtype == torch.int32 and out_ids.is_cuda and out_ids.is_contiguous()
+        assert u.dtype == torch.float32 and u.is_cuda and u.is_contiguous() and u.numel() >= out_ids.numel()
+        ok(load().sepia_model_decode_sampled(self._h, out_ids.numel(), out_ids.data_ptr(), u.data_ptr(),
+                                             self._st(stream)), "model_decode_sampled")
+
     def logits(self, stream=None) -> torch.Tensor:
         """A copy of the last computed logits [unpadded_vocab]."""
         out = torch.empty(self.cfg.unpadded_vocab_size, dtype=torch.float32, device=self.device)
@@ -254,12 +288,21 @@ class DeviceModel:
     def position(self, stream=None) -> int:
         return int(load().sepia_model_position(self._h, self._st(stream)))
 
-    def generate(self, prompt, n_gen: int, stream=None) -> np.ndarray:
+    def generate(self, prompt, n_gen: int, stream=None, sampling: Sampling | None = None, u=None) -> np.ndarray:
         """Greedy ids: id 0 is the argmax of the prompt's last logits, id i
-        the argmax after feeding id i-1 (real_generate's loop)."""
+        the argmax after feeding id i-1 (real_generate's loop). With sampling
+        and n_gen + 1 uniform numbers u in [0, 1), id i is drawn with u[i]
+        (the last number draws the token that a further step would consume)."""
         ids = torch.as_tensor(np.asarray(prompt, np.int32), device=self.device)
         out = torch.empty(n_gen, dtype=torch.int32, device=self.device)
         self.reset(stream)
         self.prefill(ids, True, stream)
-        self.decode(out, n_gen, stream)
+        if sampling is None:
+            self.decode(out, n_gen, stream)
+        else:
+            u = torch.as_tensor(u, dtype=torch.float32, device=self.device).contiguous()
+            assert u.numel() >= n_gen + 1, "one number per token and one more"
+            self.set_sampling(sampling, stream)
+            self.draw(u, stream)
+            self.decode_sampled(out, u[1:], stream)
         return out.cpu().numpy()
