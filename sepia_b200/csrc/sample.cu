@@ -9,11 +9,14 @@
 // The logits cross HBM once: a cluster of up to 8 CTAs holds a row in shared
 // memory, and all passes run there. A cut is found by a histogram over
 // (max - l)/T with linear bins (logits spread over them, so that few lanes
-// meet in one counter); the threshold bin is gathered in the cluster's first
-// CTA, split by a second histogram and the rest sorted. A bin that is too full
-// for that (runs of equal logits) is cut by halving the range of keys, 32
-// passes. Time goes into instructions, some 35 for each logit that has a
-// weight, most of them the exponential and its place in the histogram.
+// meet in one counter). Where the tokens down to the threshold bin are few,
+// the usual case, the cluster's first CTA takes them all and does the rest
+// (further cuts, the draw) in a sorted list. Otherwise it takes the threshold
+// bin alone, splits it by a second histogram, and the draw is one more pass of
+// the cluster. A bin that is too full for the list (runs of equal logits) is
+// cut by halving the range of keys, 32 passes. Time goes into instructions,
+// some 35 for each logit that has a weight, most of them the exponential and
+// its place in the histogram.
 #include "../../include/sepia_cuda.h"
 #include "common.cuh"
 #include "runtime.h"
@@ -78,7 +81,8 @@ struct SmShared {
     u64 sums[2][kSmMaxCluster][2], warp[kSmThreads / 32];
     int first_idx, n_short;
     u64 short_list[32];                      // tokens of the threshold's part of the bin
-    u64 found_before;                        // count or mass of the bins above the threshold bin
+    u64 found_before, found_here;            // count or mass of the bins above the threshold bin, and of it
+    int counts[kSmMaxCluster];               // tokens that each CTA gathered
     int bin, n_list;                         // bin: -1 no cut; n_list may pass kSmList
     SmCut cut;
 };
@@ -159,6 +163,19 @@ struct SmSlice {
         }
     }
 };
+
+// list[0, m) in descending order; m a power of two
+__device__ void sm_sort(u64 *list, int m) {
+    for (int size = 2; size <= m; size <<= 1)
+        for (int step = size >> 1; step > 0; step >>= 1) {
+            for (int i = threadIdx.x; i < m / 2; i += kSmThreads) {
+                const int a = 2 * i - (i & (step - 1)), b = a + step;
+                const u64 va = list[a], vb = list[b];
+                if ((va < vb) == ((a & size) == 0)) list[a] = vb, list[b] = va;
+            }
+            __syncthreads();
+        }
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
@@ -306,14 +323,66 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
         }
         return true;
     };
+    // The rest of a row whose first `have` tokens are in the list: all cuts and
+    // the draw, by one CTA. by_mass: they end at mass thr, else at k tokens.
+    auto finish = [&](int have, bool by_mass, double thr) {
+        int m = 2;
+        while (m < have) m <<= 1;
+        for (int i = have + tid; i < m; i += kSmThreads) S.list[i] = 0;
+        __syncthreads();
+        sm_sort(S.list, m);
+        u64 y[kSmPer], w[kSmPer], sum = 0;
+#pragma unroll
+        for (int e = 0; e < kSmPer; e++) {
+            const int at = kSmPer * tid + e;
+            y[e] = at < have ? S.list[at] : 0;
+            w[e] = at < have && (by_mass || at < k) ? sm_weight(sm_exp(sm_unkey((uint32_t)(y[e] >> 32)), top, inv_t)) : 0;
+            sum += w[e];
+        }
+        u64 run = sm_block_before(sum, S.warp);
+        if (!by_mass) thr = p >= 1.0f ? 1e300 : (double)p * (double)sm_block_sum(sum, S.warp);
+        __syncthreads();
+        sum = 0;
+#pragma unroll
+        for (int e = 0; e < kSmPer; e++) {
+            const int at = kSmPer * tid + e;
+            const bool is_in = (double)run < thr || at == 0;
+            run += w[e];
+            if (!is_in || (mp > 0.0f && !(sm_exp(sm_unkey((uint32_t)(y[e] >> 32)), top, inv_t) >= mp))) w[e] = 0;
+            sum += w[e];
+            if (at < m) S.list[at] = w[e] ? (y[e] << 32) | w[e] : 0;      // now by the index, which rises
+        }
+        const u64 total = sm_block_sum(sum, S.warp);
+        sm_sort(S.list, m);
+        const double at_u = floor((double)u * (double)total);
+        u64 target = at_u > 0.0 ? (u64)at_u : 0;
+        target = target < total ? target : total - 1;
+        sum = 0;
+#pragma unroll
+        for (int e = 0; e < kSmPer; e++) {
+            y[e] = kSmPer * tid + e < m ? S.list[kSmPer * tid + e] : 0;
+            sum += y[e] & 0xffffffffu;
+        }
+        run = sm_block_before(sum, S.warp);
+#pragma unroll
+        for (int e = 0; e < kSmPer; e++) {
+            const u64 v = y[e] & 0xffffffffu;
+            if (run <= target && target < run + v) {
+                P.ids[row] = (int32_t)(0xffffffffu - (uint32_t)(y[e] >> 32));
+                if (P.prob) P.prob[row] = (float)((double)v / (double)total);
+            }
+            run += v;
+        }
+    };
     // The cut at the token where the running count (of the order) reaches
     // `want`, or the running mass reaches `want` times the mass of the tokens
     // that are in. range: tokens with (max - l)/T beyond it cannot be the
     // cut; their mass still counts.
+    // True: the first CTA has drawn the token, nothing is left to do.
     auto find_cut = [&](bool mass, double want, float range) {
         const float per = kSmBins / range * inv_t, near = range < kSmRange ? fmaxf(cut.l, top - range * t) : cut.l;
         for (int i = tid; i < 2 * kSmBins; i += kSmThreads) (&S.hist[0][0])[i] = 0;
-        if (tid == 0) S.n_list = 0, S.bin = -1;
+        if (tid == 0) S.bin = -1;
         __syncthreads();
         u64 beyond = 0;
         auto place_of = [&](float l) { return (top - l) * per; };       // NaN where both are infinite: bin 0
@@ -371,30 +440,65 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
                     SmShared *q = cl.map_shared_rank(&S, r);
                     q->bin = first_bin + e;
                     q->found_before = b;
+                    q->found_here = v[e];
                 }
             b += v[e];
         }
         cl.sync();
         const int bin = S.bin;
-        if (bin < 0) return;                           // a count past all tokens of any weight: nothing to cut
-        // its tokens to the first CTA; bounds of a bin more on either side spare most of them the bin's arithmetic
-        const float bin_lo = fmaxf(near, top - ((float)bin + 2.0f) / per), bin_hi = top - ((float)bin - 1.0f) / per;
-        const float mid = bin ? 0.5f * (bin_lo + bin_hi) : top, half = bin ? bin_hi - mid : top - bin_lo;
-        X.each([&](const float (&v)[E], int i) {
-            float d = fabsf(v[0] - mid);               // NaN at an infinite maximum: passes
-#pragma unroll
-            for (int e = 1; e < E; e++) d = fminf(d, fabsf(v[e] - mid));
-            if (d > half) return;
-#pragma unroll
-            for (int e = 0; e < E; e++)
-                if (v[e] >= near && bin_of(v[e]) == bin && in(v[e], i + e)) {
-                    const int at = atomicAdd(&first->n_list, 1);
-                    if (at < kSmList) first->list[at] = ((u64)sm_key(v[e]) << 32) | (0xffffffffu - (uint32_t)(i + e));
-                }
-        });
-        cl.sync();
-        const int have = first->n_list;
+        if (bin < 0) return false;                     // a count past all tokens of any weight: nothing to cut
         const u64 above = S.found_before;
+        // Tokens of bins from .. bin into the lists of their CTAs, then
+        // (if they fit) into the first CTA's; how many there are. Bounds of a
+        // bin more on either side spare most tokens the bin's arithmetic.
+        auto gather = [&](int from) {
+            const float bin_lo = fmaxf(near, top - ((float)bin + 2.0f) / per);
+            const float bin_hi = from ? top - ((float)from - 1.0f) / per : top;
+            const float mid = from ? 0.5f * (bin_lo + bin_hi) : top, half = from ? fmaxf(bin_hi - mid, mid - bin_lo) : top - bin_lo;
+            __syncthreads();
+            if (tid == 0) S.n_list = 0;
+            __syncthreads();
+            X.each([&](const float (&v)[E], int i) {
+                float d = fabsf(v[0] - mid);           // NaN at an infinite maximum: passes
+#pragma unroll
+                for (int e = 1; e < E; e++) d = fminf(d, fabsf(v[e] - mid));
+                if (d > half) return;
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    if (!(v[e] >= near)) continue;
+                    const int b = bin_of(v[e]);
+                    if (b >= from && b <= bin && in(v[e], i + e)) {
+                        const int at = atomicAdd(&S.n_list, 1);
+                        if (at < kSmList) S.list[at] = ((u64)sm_key(v[e]) << 32) | (0xffffffffu - (uint32_t)(i + e));
+                    }
+                }
+            });
+            __syncthreads();
+            const int n_here = S.n_list;
+            if (tid < C) cl.map_shared_rank(&S, tid)->counts[rank] = n_here;
+            cl.sync();
+            int all_n = 0, before_n = 0;
+            for (int r = 0; r < C; r++) {
+                before_n += r < rank ? S.counts[r] : 0;
+                all_n += S.counts[r];
+            }
+            if (all_n <= kSmList && rank > 0)
+                for (int i = tid; i < n_here; i += kSmThreads) first->list[before_n + i] = S.list[i];
+            cl.sync();
+            return all_n;
+        };
+        // All tokens down to the threshold: as many as the count says, or at
+        // most their mass over the least weight among them.
+        const u64 down = above + S.found_here;
+        const double least = mass ? exp(-(double)(bin + 1) * (double)(range / kSmBins)) * (double)kSmOne : 1.0;
+        if ((double)down <= least * (mass ? 65536.0 : (double)kSmList)) {
+            const int have = gather(0);
+            if (have <= kSmList) {
+                if (rank == 0) finish(have, mass, thr);
+                return true;
+            }
+        }
+        const int have = gather(bin);
         if (have <= kSmList) {
             if (rank == 0) {
                 auto value = [&](u64 y) -> u64 {
@@ -461,15 +565,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
 #pragma unroll
                     for (int e = 0; e < kSmPer; e++) S.list[tid + e * kSmThreads] = y[e];
                     __syncthreads();
-                    for (int size = 2; size <= m; size <<= 1)
-                        for (int step = size >> 1; step > 0; step >>= 1) {
-                            for (int i = tid; i < m / 2; i += kSmThreads) {
-                                const int a = 2 * i - (i & (step - 1)), b = a + step;
-                                const u64 va = S.list[a], vb = S.list[b];
-                                if ((va < vb) == ((a & size) == 0)) S.list[a] = vb, S.list[b] = va;
-                            }
-                            __syncthreads();
-                        }
+                    sm_sort(S.list, m);
                     q = 0;
 #pragma unroll
                     for (int e = 0; e < kSmPer; e++) {
@@ -491,7 +587,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
             }
             cl.sync();
             cut = S.cut;
-            return;
+            return false;
         }
         // Too many for the list: the greatest key whose tokens and those above
         // reach the threshold, bit by bit; then how many tokens of that very
@@ -524,8 +620,9 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
         cl.sync();
         cut.l = sm_unkey(key);
         cut.idx = (int)lo;
+        return false;
     };
-    if (k > 0 && k < V) find_cut(false, (double)k, kSmRange);
+    if (k > 0 && k < V && find_cut(false, (double)k, kSmRange)) return;
     if (!(p >= 1.0f)) {
         if (p > 0.0f) {
             // Without top-k, tokens below (1 - p)/(2 V) of the best together weigh
@@ -533,7 +630,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
             // for rounded weights), so the bins need not reach that far.
             const float q = 1.0f - p;
             const bool narrow = !(k > 0 && k < V) && q >= 0.00390625f;
-            find_cut(true, (double)p, narrow ? fminf(kSmRange, logf(2.0f * (float)V / q)) : kSmRange);
+            if (find_cut(true, (double)p, narrow ? fminf(kSmRange, logf(2.0f * (float)V / q)) : kSmRange)) return;
         } else {
             cut.l = top;
             cut.idx = first_best();

@@ -185,6 +185,36 @@ def test_many_rows_with_their_own_settings(lib):
     assert np.array_equal(draw(torch.tensor(x, device="cuda"), u, **kw)[0], want)
 
 
+@pytest.mark.parametrize("base", [0.0, 1e4, -3e6, 1e8])
+def test_logits_far_from_zero(lib, base):
+    """A common offset leaves few distinct logits (the spacing of fp32 grows): the cuts are those of the values as they are."""
+    rng = np.random.default_rng(5)
+    x = (rng.standard_normal((6, 30011)) * 4 + base).astype(np.float32)
+    for kw in (dict(top_p=0.7), dict(top_k=2000), dict(temperature=8.0, top_k=90, top_p=0.8), dict(min_p=0.3)):
+        u, want = [], []
+        for r in range(6):
+            at, share = kept64(x[r], kw.get("temperature", 1.0), kw.get("top_k", 0), kw.get("top_p", 1.0), kw.get("min_p", 0.0))
+            j, uu = pick_u(share, rng)
+            u.append(uu)
+            want.append(at[j])
+        assert np.array_equal(draw(torch.tensor(x, device="cuda"), u, **kw)[0], want), kw
+
+
+@pytest.mark.parametrize("k", [900, 1023, 1024, 1025, 1100])
+def test_around_the_lists_capacity(lib, k):
+    """Sets of about 1024 tokens, where the work changes hands; with and without top-p on top."""
+    rng = np.random.default_rng(k)
+    x = (rng.standard_normal((4, 60013)) * 2).astype(np.float32)
+    for kw in (dict(top_k=k), dict(top_k=k, top_p=0.9), dict(top_k=k, min_p=0.1)):
+        u, want = [], []
+        for r in range(4):
+            at, share = kept64(x[r], 1.0, k, kw.get("top_p", 1.0), kw.get("min_p", 0.0))
+            j, uu = pick_u(share, rng)
+            u.append(uu)
+            want.append(at[j])
+        assert np.array_equal(draw(torch.tensor(x, device="cuda"), u, **kw)[0], want), kw
+
+
 def test_refusals(lib):
     from sepia_b200.sampling import sample
     x, u = torch.zeros(2, 8, device="cuda"), torch.zeros(2, device="cuda")
