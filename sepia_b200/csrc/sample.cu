@@ -328,6 +328,46 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
     auto finish = [&](int have, bool by_mass, double thr) {
         int m = 2;
         while (m < have) m <<= 1;
+        if (have <= kSmThreads / 2) {
+            // Few tokens: each one's sums over those before it, by pairs, the
+            // others of a token spread over kSmThreads / m neighbouring lanes
+            // (two sorts of 155 tokens took 11 us, this takes 3).
+            m = max(m, kSmThreads / 32);
+            uint32_t *weight_of = reinterpret_cast<uint32_t *>(S.list + kSmList / 2);
+            const int lanes = kSmThreads / m, me = tid / lanes, part = tid % lanes;
+            const u64 y = me < have ? S.list[me] : 0;
+            const float e = sm_exp(sm_unkey((uint32_t)(y >> 32)), top, inv_t);
+            uint32_t w = me < have ? (uint32_t)sm_weight(e) : 0u;
+            if (part == 0 && me < have) weight_of[me] = w;
+            __syncthreads();
+            u64 mass_before = 0;
+            int rank_of = 0;
+            for (int j = part; j < have; j += lanes)
+                if (S.list[j] > y) rank_of++, mass_before += weight_of[j];
+            for (int o = 1; o < lanes; o <<= 1) {
+                rank_of += __shfl_xor_sync(0xffffffffu, rank_of, o);
+                mass_before += __shfl_xor_sync(0xffffffffu, mass_before, o);
+            }
+            bool is_in = me < have && (by_mass || rank_of < k);
+            if (!by_mass) thr = p >= 1.0f ? 1e300 : (double)p * (double)sm_block_sum(is_in && part == 0 ? w : 0, S.warp);
+            is_in = is_in && ((double)mass_before < thr || rank_of == 0) && !(mp > 0.0f && !(e >= mp));
+            if (!is_in) w = 0;
+            __syncthreads();
+            if (part == 0 && me < have) weight_of[me] = w;
+            const u64 total = sm_block_sum(part == 0 ? w : 0, S.warp);
+            u64 run = 0;                               // of the tokens of lower index
+            for (int j = part; j < have; j += lanes)
+                if ((uint32_t)S.list[j] > (uint32_t)y) run += weight_of[j];
+            for (int o = 1; o < lanes; o <<= 1) run += __shfl_xor_sync(0xffffffffu, run, o);
+            const double at_u = floor((double)u * (double)total);
+            u64 target = at_u > 0.0 ? (u64)at_u : 0;
+            target = target < total ? target : total - 1;
+            if (part == 0 && run <= target && target < run + w) {
+                P.ids[row] = (int32_t)(0xffffffffu - (uint32_t)y);
+                if (P.prob) P.prob[row] = (float)((double)w / (double)total);
+            }
+            return;
+        }
         for (int i = have + tid; i < m; i += kSmThreads) S.list[i] = 0;
         __syncthreads();
         sm_sort(S.list, m);
