@@ -39,7 +39,7 @@ constexpr int kK8Warps = 4;
 constexpr int kK8Threads = 32 * kK8Warps;
 constexpr int kK8Tile = 16;              // keys of one scale: a block is a multiple of it
 constexpr int kK8Unit = 2 * kK8Tile;     // keys per warp step
-// CTAs an SM holds: by registers (128 or 168 a thread)
+// CTAs an SM holds: by registers (128 a thread)
 constexpr int k8_ctas(int nb) { return nb == 1 ? 4 : 3; }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLowest = -3.402823466e38f;
@@ -109,6 +109,7 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
 // NB groups of 8 rows share a warp's converted codes.
 template <typename T, int DP, int NB>
 struct K8Cfg {
+    static constexpr int UNITS = NB == 1 ? 2 : 1;     // 16-key tiles whose scores are in registers at once
     static constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;   // fp16 terms of a row
     static constexpr int RT = 8 * NB;                 // rows of a tile
     static constexpr int KW = DP / 64;                // 16-byte pieces of a key row per lane
@@ -527,7 +528,6 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
         }
     };
     using One = std::integral_constant<int, 1>;
-    using Two = std::integral_constant<int, 2>;
 
     // ---- the tail's fp16 tiles, one a warp, while the slots fill ----
     {
@@ -599,33 +599,36 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
         cp_async_wait<1>();                            // the keys
         __syncwarp();
         const float4 sc = *reinterpret_cast<const float4 *>(st + 2 * F::kTileB);
-        const float ksc[2] = {sc.x, sc.z};
-        const float ev[2] = {(float)((int)(__float_as_uint(sc.y) >> 23 & 255) - 127),
+        float ksc[2] = {sc.x, sc.z};
+        float ev[2] = {(float)((int)(__float_as_uint(sc.y) >> 23 & 255) - 127),
                              (float)((int)(__float_as_uint(sc.w) >> 23 & 255) - 127)};
         uint32_t v[4][F::VB / 4];
+#pragma unroll 1
+        for (int u0 = 0; u0 < 2; u0 += F::UNITS) {
+        uint8_t *at = st + u0 * F::kTileB;
         step(
-            Two(), c0 + (warp + kK8Warps * i) * kK8Unit, ksc, ev,
-            [&](float (&S)[NB][2][4]) {
-                float R[NB][2][4];                     // the second term's sums, or the odd k steps'
+            std::integral_constant<int, F::UNITS>(), c0 + (warp + kK8Warps * i) * kK8Unit + u0 * kK8Tile, ksc + u0, ev + u0,
+            [&](float (&S)[NB][F::UNITS][4]) {
+                float R[NB][F::UNITS][4];              // the second term's sums, or the odd k steps'
 #pragma unroll
                 for (int g = 0; g < NB; g++)
 #pragma unroll
-                    for (int u = 0; u < 2; u++)
+                    for (int u = 0; u < F::UNITS; u++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) S[g][u][e] = R[g][u][e] = 0.0f;
 #pragma unroll
                 for (int j = 0; j < F::KW; j++) {
-                    uint4 k[2][2];
+                    uint4 k[F::UNITS][2];
 #pragma unroll
-                    for (int u = 0; u < 2; u++)
+                    for (int u = 0; u < F::UNITS; u++)
 #pragma unroll
                         for (int n = 0; n < 2; n++)
-                            k[u][n] = *reinterpret_cast<const uint4 *>(st + u * F::kTileB + n * 8 * DP + from_k[j]);
+                            k[u][n] = *reinterpret_cast<const uint4 *>(at + u * F::kTileB + n * 8 * DP + from_k[j]);
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        uint32_t a[2][4];
+                        uint32_t a[F::UNITS][4];
 #pragma unroll
-                        for (int u = 0; u < 2; u++) {
+                        for (int u = 0; u < F::UNITS; u++) {
                             const uint32_t x = e == 0 ? k[u][0].x : e == 1 ? k[u][0].y : e == 2 ? k[u][0].z : k[u][0].w;
                             const uint32_t y = e == 0 ? k[u][1].x : e == 1 ? k[u][1].y : e == 2 ? k[u][1].z : k[u][1].w;
                             a[u][0] = e4m3_lo(x), a[u][1] = e4m3_lo(y), a[u][2] = e4m3_hi(x), a[u][3] = e4m3_hi(y);
@@ -635,7 +638,7 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
                             uint32_t w[2 * TERMS];
                             q_op(g, 4 * j + e, w);
 #pragma unroll
-                            for (int u = 0; u < 2; u++) {
+                            for (int u = 0; u < F::UNITS; u++) {
                                 if constexpr (TERMS == 2) {
                                     mma16(S[g][u], a[u], w[0], w[1]);
                                     mma16(R[g][u], a[u], w[2 * TERMS - 2], w[2 * TERMS - 1]);
@@ -649,19 +652,22 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
 #pragma unroll
                 for (int g = 0; g < NB; g++)
 #pragma unroll
-                    for (int u = 0; u < 2; u++)
+                    for (int u = 0; u < F::UNITS; u++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) S[g][u][e] += R[g][u][e];
                 __syncwarp();                          // every lane has read the keys and the scales
-                fetch_keys(i + 1);
-                cp_async_wait<1>();                    // the values
-                __syncwarp();
+                if (u0 + F::UNITS == 2) fetch_keys(i + 1);
+                if (u0 == 0) {                         // the values
+                    if constexpr (F::UNITS == 2) cp_async_wait<1>();
+                    else cp_async_wait<0>();
+                    __syncwarp();
+                }
             },
             [&](int u, int mt, uint32_t (&a)[4]) {
                 if (mt == 0) {
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        const uint8_t *src = st + u * F::kTileB + F::kKeyB + (k >> 1) * 8 * DP + from_v[k & 1];
+                        const uint8_t *src = at + u * F::kTileB + F::kKeyB + (k >> 1) * 8 * DP + from_v[k & 1];
                         if constexpr (F::VB == 16) *reinterpret_cast<uint4 *>(v[k]) = *reinterpret_cast<const uint4 *>(src);
                         else *reinterpret_cast<uint2 *>(v[k]) = *reinterpret_cast<const uint2 *>(src);
                     }
@@ -672,22 +678,23 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
                 a[0] = e4m3_lo(x), a[1] = e4m3_hi(x), a[2] = e4m3_lo(y), a[3] = e4m3_hi(y);
             },
             [&](int g, int k) {
-                return *reinterpret_cast<const float *>(st + 2 * F::kTileB + F::kHeadB + (8 * g + k) * 128 + lane * 4);
+                return *reinterpret_cast<const float *>(st + 2 * F::kTileB + F::kHeadB + (8 * g + 4 * u0 + k) * 128 + lane * 4);
             },
             [&](int u) {                               // in the slots: no other lane reads these bytes
                 uint32_t nan = 0;
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    uint32_t *x = reinterpret_cast<uint32_t *>(st + u * F::kTileB + F::kKeyB + (k >> 1) * 8 * DP + from_v[k & 1]);
+                    uint32_t *x = reinterpret_cast<uint32_t *>(at + u * F::kTileB + F::kKeyB + (k >> 1) * 8 * DP + from_v[k & 1]);
 #pragma unroll
                     for (int e = 0; e < F::VB / 4; e++) {
-                        const uint32_t at = __vcmpeq4(x[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-                        if (at) x[e] &= ~at;
-                        nan |= at ? 1u << (2 * tig + (k & 1) + 8 * (k >> 1)) : 0u;
+                        const uint32_t y = __vcmpeq4(x[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+                        if (y) x[e] &= ~y;
+                        nan |= y ? 1u << (2 * tig + (k & 1) + 8 * (k >> 1)) : 0u;
                     }
                 }
                 return nan;
             });
+        }
         __syncwarp();                                  // every lane has read the values
         fetch_values(i + 1);
     }

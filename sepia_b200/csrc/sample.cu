@@ -59,10 +59,12 @@ __device__ __forceinline__ uint32_t sm_key(float v) {
 __device__ __forceinline__ float sm_unkey(uint32_t k) {
     return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
-// e = exp((l - max)/T); the best token's is 1 also where max is infinite (the least of NaN and 0 is 0)
-__device__ __forceinline__ float sm_exp(float l, float best, float inv_t) {
-    return expf(fminf(l - best, 0.0f) * inv_t);
+// (l - max)/T, at most 0, and e = exp of it; the best token's is 1 also where
+// max is infinite, or 1/T is (the least of NaN and 0 is 0)
+__device__ __forceinline__ float sm_exponent(float l, float best, float inv_t) {
+    return fminf((l - best) * inv_t, 0.0f);
 }
+__device__ __forceinline__ float sm_exp(float l, float best, float inv_t) { return expf(sm_exponent(l, best, inv_t)); }
 __device__ __forceinline__ u64 sm_weight(float e) { return (u64)__float2uint_rn(e * kSmOne); }
 
 // The last token in
@@ -306,14 +308,15 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
     SmCut cut = {floor_l, INT32_MAX};                  // tokens in: l > cut.l, or l == cut.l up to an index
     auto in = [&](float l, int i) { return l >= cut.l && !(l == cut.l && i > cut.idx); };
     // Weights of a vector's tokens that are in, 0 for the others; false: all 0
-    auto weigh = [&](const float (&v)[E], int i, uint32_t (&w)[E]) {
+    auto weigh = [&](const float (&v)[E], int i, uint32_t (&w)[E], float (&x)[E]) {
         float most = v[0];
 #pragma unroll
         for (int e = 1; e < E; e++) most = fmaxf(most, v[e]);
         if (!(most >= cut.l)) return false;
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            const uint32_t y = __float2uint_rn(sm_exp(v[e], top, inv_t) * kSmOne);
+            x[e] = sm_exponent(v[e], top, inv_t);
+            const uint32_t y = __float2uint_rn(expf(x[e]) * kSmOne);
             w[e] = v[e] >= cut.l ? y : 0u;
         }
         if (cut.idx != INT32_MAX) {                    // the whole cluster
@@ -420,13 +423,14 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
     // cut; their mass still counts.
     // True: the first CTA has drawn the token, nothing is left to do.
     auto find_cut = [&](bool mass, double want, float range) {
-        const float per = kSmBins / range * inv_t, near = range < kSmRange ? fmaxf(cut.l, top - range * t) : cut.l;
+        const float per = -(float)kSmBins / range, near = range < kSmRange ? fmaxf(cut.l, top - range * t) : cut.l;
         for (int i = tid; i < 2 * kSmBins; i += kSmThreads) (&S.hist[0][0])[i] = 0;
         if (tid == 0) S.bin = -1;
         __syncthreads();
         u64 beyond = 0;
-        auto place_of = [&](float l) { return (top - l) * per; };       // NaN where both are infinite: bin 0
-        auto bin_of = [&](float l) { return min(kSmBins - 1, (int)place_of(l)); };
+        auto place_of = [&](float l) { return sm_exponent(l, top, inv_t) * per; };
+        auto bin_at = [&](float place) { return min(kSmBins - 1, (int)place); };   // `near` may be rounded past the range
+        auto bin_of = [&](float l) { return bin_at(place_of(l)); };
         X.each([&](const float (&v)[E], int i) {
             if (!mass) {
 #pragma unroll
@@ -435,7 +439,8 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
                 return;
             }
             uint32_t w[E];
-            if (!weigh(v, i, w)) return;
+            float x[E];
+            if (!weigh(v, i, w, x)) return;
             if (range < kSmRange) {                    // such weights are below 2^31 (1 - p)/(2 V): E of them fit 32 bits
                 uint32_t far = 0;
 #pragma unroll
@@ -444,8 +449,8 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
             }
 #pragma unroll
             for (int e = 0; e < E; e++)
-                if (v[e] >= near && w[e]) {
-                    const int b = bin_of(v[e]);
+                if (v[e] >= near) {                    // some have weight 0: not in after all
+                    const int b = bin_at(x[e] * per);  // bin_of
                     atomicAdd(&S.hist[0][b], w[e] & 0xffffu);
                     atomicAdd(&S.hist[1][b], w[e] >> 16);
                 }
@@ -492,8 +497,8 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
         // (if they fit) into the first CTA's; how many there are. Bounds of a
         // bin more on either side spare most tokens the bin's arithmetic.
         auto gather = [&](int from) {
-            const float bin_lo = fmaxf(near, top - ((float)bin + 2.0f) / per);
-            const float bin_hi = from ? top - ((float)from - 1.0f) / per : top;
+            const float bin_lo = fmaxf(near, top + ((float)bin + 2.0f) / per * t);
+            const float bin_hi = from ? top + ((float)from - 1.0f) / per * t : top;
             const float mid = from ? 0.5f * (bin_lo + bin_hi) : top, half = from ? fmaxf(bin_hi - mid, mid - bin_lo) : top - bin_lo;
             __syncthreads();
             if (tid == 0) S.n_list = 0;
@@ -530,7 +535,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
         // All tokens down to the threshold: as many as the count says, or at
         // most their mass over the least weight among them.
         const u64 down = above + S.found_here;
-        const double least = mass ? exp(-(double)(bin + 1) * (double)(range / kSmBins)) * (double)kSmOne : 1.0;
+        const double least = mass ? exp((double)(bin + 1) / (double)per) * (double)kSmOne : 1.0;
         if ((double)down <= least * (mass ? 65536.0 : (double)kSmList)) {
             const int have = gather(0);
             if (have <= kSmList) {
@@ -680,7 +685,8 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
     // ---- the draw: the CTA, then the warp's run, then the token ----
     auto weigh_min_p = [&](const float (&v)[E], int i, uint32_t (&w)[E]) {
         u64 s = 0;
-        if (!weigh(v, i, w)) {
+        float x[E];
+        if (!weigh(v, i, w, x)) {
 #pragma unroll
             for (int e = 0; e < E; e++) w[e] = 0u;
             return s;
@@ -688,7 +694,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
         if (mp > 0.0f) {                               // the whole cluster
 #pragma unroll
             for (int e = 0; e < E; e++)
-                if (!(sm_exp(v[e], top, inv_t) >= mp)) w[e] = 0u;
+                if (!(expf(x[e]) >= mp)) w[e] = 0u;
         }
 #pragma unroll
         for (int e = 0; e < E; e++) s += w[e];
