@@ -429,7 +429,11 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
         __syncthreads();
         u64 beyond = 0;
         auto place_of = [&](float l) { return sm_exponent(l, top, inv_t) * per; };
-        auto bin_at = [&](float place) { return min(kSmBins - 1, (int)place); };   // `near` may be rounded past the range
+        // The nearest whole number, by adding 2^23 (a conversion would hold up
+        // the exponentials' unit); `near` may be rounded past the range.
+        auto bin_at = [&](float place) {
+            return (int)min(kSmBins - 1u, __float_as_uint(place + 8388608.0f) - 0x4b000000u);
+        };
         auto bin_of = [&](float l) { return bin_at(place_of(l)); };
         X.each([&](const float (&v)[E], int i) {
             if (!mass) {
@@ -494,11 +498,12 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
         if (bin < 0) return false;                     // a count past all tokens of any weight: nothing to cut
         const u64 above = S.found_before;
         // Tokens of bins from .. bin into the lists of their CTAs, then
-        // (if they fit) into the first CTA's; how many there are. Bounds of a
-        // bin more on either side spare most tokens the bin's arithmetic.
+        // (if they fit) into the first CTA's; how many there are. Bounds a
+        // little past the bins (half a bin to either side of whole numbers)
+        // spare most tokens the bin's arithmetic.
         auto gather = [&](int from) {
-            const float bin_lo = fmaxf(near, top + ((float)bin + 2.0f) / per * t);
-            const float bin_hi = from ? top + ((float)from - 1.0f) / per * t : top;
+            const float bin_lo = fmaxf(near, top + ((float)bin + 0.6f) / per * t);
+            const float bin_hi = from ? top + ((float)from - 0.6f) / per * t : top;
             const float mid = from ? 0.5f * (bin_lo + bin_hi) : top, half = from ? fmaxf(bin_hi - mid, mid - bin_lo) : top - bin_lo;
             __syncthreads();
             if (tid == 0) S.n_list = 0;
@@ -510,7 +515,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
                 if (d > half) return;
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    if (!(v[e] >= near)) continue;
+                    if (fabsf(v[e] - mid) > half || !(v[e] >= near)) continue;
                     const int b = bin_of(v[e]);
                     if (b >= from && b <= bin && in(v[e], i + e)) {
                         const int at = atomicAdd(&S.n_list, 1);
@@ -535,7 +540,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
         // All tokens down to the threshold: as many as the count says, or at
         // most their mass over the least weight among them.
         const u64 down = above + S.found_here;
-        const double least = mass ? exp((double)(bin + 1) / (double)per) * (double)kSmOne : 1.0;
+        const double least = mass ? exp(((double)bin + 0.5) / (double)per) * (double)kSmOne : 1.0;
         if ((double)down <= least * (mass ? 65536.0 : (double)kSmList)) {
             const int have = gather(0);
             if (have <= kSmList) {
@@ -557,7 +562,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
                     const bool on = tid + e * kSmThreads < have;
                     y[e] = on ? S.list[tid + e * kSmThreads] : 0;
                     val[e] = on ? value(y[e]) : 0;
-                    const float at = (place_of(sm_unkey((uint32_t)(y[e] >> 32))) - (float)bin) * kSmBins;
+                    const float at = (place_of(sm_unkey((uint32_t)(y[e] >> 32))) - (float)bin + 0.5f) * kSmBins;
                     part[e] = on ? max(0, min(kSmBins - 1, (int)at)) : -1;
                 }
                 __syncthreads();                       // the list is read: its room becomes counters again
