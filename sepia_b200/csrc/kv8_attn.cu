@@ -43,11 +43,12 @@ constexpr int kK8Unit = 2 * kK8Tile;     // keys per warp step
 constexpr int k8_ctas(int nb) { return nb == 1 ? 4 : 3; }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLowest = -3.402823466e38f;
-// Weights reach the tensor core as 2^(score - maximum + kPBits), in base 2.
+// Weights reach the tensor core as 2^(score - maximum + kPBits), in base 2,
+// and as 2^(the value scale's exponent less the greatest one met) of that.
 // The maximum is only moved (and the output rescaled) when a weight would
-// pass 2^15, so it may lag; kPBits leaves it 8 binary places to do so and
-// keeps 22 bits of a weight down to 2^-20 of the largest.
-constexpr float kPBits = 7.0f, kPMax = 15.0f;
+// pass 2^15, so it may lag by two places. The smallest fp16 step, 2^-24, is
+// then 2^-37 of the greatest weight, and 2^-37 + the spread of the scales.
+constexpr float kPBits = 13.0f, kPMax = 15.0f;
 
 struct K8Params {
     SepiaKv8Cache c;
@@ -536,7 +537,6 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
             const int64_t at = (((int64_t)sq.slot * Hkv + hk) * B + (t0 - tail0)) * Dh;
             const __half *K = (const __half *)P.c.k_tail + at, *V = (const __half *)P.c.v_tail + at;
             const int held = sq.held + sq.add - t0;    // keys of the tile that exist
-            const float one = 1.0f, zero = 0.0f;
             uint32_t v[4][F::VB / 2];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
@@ -547,8 +547,26 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
                         r < held && d + 8 * j < Dh ? *reinterpret_cast<const uint4 *>(V + r * Dh + d + 8 * j)
                                                    : make_uint4(0, 0, 0, 0);
             }
+            // Values as codes are: times the power of two that puts the tile's
+            // largest in [2^8, 2^9), so that its weights are of the codes'
+            // size (a scale of 1 would leave those of coded blocks few bits)
+            __half2 most = __half2half2(__ushort_as_half(0));
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+#pragma unroll
+                for (int e = 0; e < F::VB / 2; e++) most = __hmax2(most, __habs2(*reinterpret_cast<const __half2 *>(&v[k][e])));
+            const float amax = warp_max(fmaxf(__low2float(most), __high2float(most)));
+            const int ex = amax > 0.0f ? (int)(__float_as_uint(amax) >> 23) - 127 - 8 : -60;
+            const float f = __uint_as_float((uint32_t)(127 - ex) << 23), one = 1.0f, ev_tail = (float)ex;
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+#pragma unroll
+                for (int e = 0; e < F::VB / 2; e++) {
+                    const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&v[k][e]));
+                    v[k][e] = pack_half2(x.x * f, x.y * f);
+                }
             step(
-                One(), t0, &one, &zero,
+                One(), t0, &one, &ev_tail,
                 [&](float (&S)[NB][1][4]) {
 #pragma unroll
                     for (int g = 0; g < NB; g++) S[g][0][0] = S[g][0][1] = S[g][0][2] = S[g][0][3] = 0.0f;

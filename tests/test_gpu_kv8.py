@@ -42,11 +42,11 @@ def norm_rotate64(x, w, table, pos, adjacent, eps):
 class Batch:
     """A cache and its sequences, with the true rows of every sequence in 64 bits."""
 
-    def __init__(self, held, hk, dim, block, extra_blocks=3, fill=0x7F, seed=0):
+    def __init__(self, held, hk, dim, block, extra_blocks=3, fill=0x7F, seed=0, room=0):
         from sepia_b200.kv8 import Kv8Cache
         self.rng = np.random.default_rng(seed)
         self.hk, self.dim, self.block, self.n = hk, dim, block, len(held)
-        self.cols = max(8, (max(held) if held else 0) // block + 8)
+        self.cols = max(8, (max(held) if held else 0) // block + 8, room // block + 2)
         nb = self.n * self.cols + extra_blocks
         self.cache = Kv8Cache.allocate(nb, self.n + 2, hk, dim, block)
         # whatever is not written is NaN: it must never reach a result
@@ -487,3 +487,33 @@ def test_attention_not_numbers_behind_a_mask(lib, dtype, held, window):
         outs.append(B.cache.attention(step, q, 1.0 / dim, window=window))
     assert torch.equal(outs[0][: new - 1], outs[1][: new - 1])
     assert torch.isnan(outs[1][new - 1]).view(hk, -1).any(dim=1).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("held", [3000, 3001, 3017])
+def test_attention_a_sink_and_a_faint_rest(lib, dtype, held):
+    """One key far above all others, which together still weigh something:
+    thousands of weights of 2^-20 of the largest, values of unlike size beside
+    an unscaled tail."""
+    B = Batch([0], 1, 64, 32, seed=11, room=held + 1)
+    rng = np.random.default_rng(12)
+    k = rng.standard_normal((held, 1, 64)) * 0.05
+    v = 0.01 + 0.002 * rng.standard_normal((held, 1, 64))
+    direction = rng.standard_normal(64)
+    k[5, 0] = 8.0 * direction / np.linalg.norm(direction)
+    v[5] = 0.0
+    v[32:64] *= 40.0
+    B.append([held], k=torch.tensor(k, dtype=F32, device="cuda"), v=torch.tensor(v, dtype=F32, device="cuda"))
+    rows = [torch.tensor(direction / np.linalg.norm(direction) * g, dtype=F32) for g in (60.0, 100.0, 110.0, 0.0)]
+    q = torch.stack(rows)[None].to(dtype).cuda()
+    kn, vn = torch.zeros(1, 1, 64, device="cuda"), torch.full((1, 1, 64), 0.01, device="cuda")
+    step = B.step([1])
+    B.cache.append(step, kn, vn)
+    out = B.cache.attention(step, q, 1.0 / 64)
+    B.kv_len += 1
+    want, top, vmax = attention64(B, q, [held], [1], np.float64(np.float32(1.0 / 64)), 0, None, None)
+    # every output is a share of faint weights: relative to itself, a score's error and the formats'
+    # (fp16: weights of 11 bits, rounded both ways, and the result's 2^-11)
+    tol = (2 * 64 * 2.0 ** -24 * top / 64 + 2.0 ** -13 * (1 if dtype == F32 else 8))[:, :, None] * np.abs(want) + 1e-12
+    err = np.abs(out.cpu().double().numpy() - want)
+    assert np.all(err <= tol + (2.0 ** -24 if dtype == F16 else 0)), float((err / tol).max())
