@@ -840,7 +840,10 @@ struct K8Plan {
 
 // Chunks: one wave of equal chunks over all CTA slots while that leaves a
 // chunk at most kMaxChunk positions; longer work runs in several waves of
-// kMaxChunk, so that ragged sequences even out.
+// kMaxChunk, so that ragged sequences even out (64 ragged sequences: 85 us
+// with 1024, 90 with 512). Where rows alone make four waves (long pieces of
+// prompts) nothing is cut: 512 new tokens on 4096 take 485 us, cut 569, and no
+// workspace.
 static K8Plan k8_plan(const SepiaKv8Cache &c, const SepiaKv8Step &b, const SepiaKv8Attn &a) {
     constexpr int64_t kUnit = kK8Unit * kK8Warps, kMaxChunk = 1024;
     K8Plan p;
@@ -851,7 +854,8 @@ static K8Plan k8_plan(const SepiaKv8Cache &c, const SepiaKv8Step &b, const Sepia
     const int64_t groups = (int64_t)b.n_seqs * c.n_kv_heads * p.row_tiles;
     const int64_t slots = (int64_t)(dev_info().sm_count > 0 ? dev_info().sm_count : 148) * k8_ctas(rt / 8);
     const int64_t one = (groups * span + slots - 1) / slots;
-    p.chunk = (int)(std::min(kMaxChunk, std::max<int64_t>(one, 1)) + kUnit - 1) / kUnit * kUnit;
+    const int64_t want = groups >= 4 * slots ? span : std::min(kMaxChunk, one);
+    p.chunk = (int)((std::max<int64_t>(want, 1) + kUnit - 1) / kUnit * kUnit);
     p.splits = (int)std::max<int64_t>(1, (span + p.chunk - 1) / p.chunk);
     p.cells = p.splits > 1 ? (size_t)groups * p.splits * rt : 0;
     p.bytes = p.cells * (c.head_dim * 4 + 8);
