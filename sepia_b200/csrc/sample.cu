@@ -13,10 +13,11 @@
 // the usual case, the cluster's first CTA takes them all and does the rest
 // (further cuts, the draw) in a sorted list. Otherwise it takes the threshold
 // bin alone, splits it by a second histogram, and the draw is one more pass of
-// the cluster. A bin that is too full for the list (runs of equal logits) is
-// cut by halving the range of keys, 32 passes. Time goes into instructions,
-// some 35 for each logit that has a weight, most of them the exponential and
-// its place in the histogram.
+// the cluster. A bin that is too full for the list is first split by the
+// cluster; what even that leaves too full (runs of equal logits) is cut by
+// halving the range of keys, 32 passes. Time goes into instructions, some 35
+// for each logit that has a weight, most of them the exponential and its place
+// in the histogram, and into the cluster's barriers.
 #include "../../include/sepia_cuda.h"
 #include "common.cuh"
 #include "runtime.h"
@@ -459,50 +460,62 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
                     atomicAdd(&S.hist[1][b], w[e] >> 16);
                 }
         });
-        cl.sync();
-        // The threshold bin: each CTA adds its share of the bins over the
-        // cluster, a run of `each` neighbours a thread
-        const int share = kSmBins / C, each = max(1, share / kSmThreads), first_bin = rank * share + tid * each;
-        u64 v[kSmPer] = {}, mine = 0;
+        // The threshold bin, of counters that start at running sum `from`: each
+        // CTA adds its share of the bins over the cluster, a run of `each`
+        // neighbours a thread. S.bin stays -1 where the threshold is not met.
+        double thr = want;
+        auto add_bins = [&](u64 from, bool know_thr) {
+            cl.sync();
+            const int share = kSmBins / C, each = max(1, share / kSmThreads), first_bin = rank * share + tid * each;
+            u64 v[kSmPer] = {}, mine = 0;
 #pragma unroll
-        for (int e = 0; e < kSmPer; e++)
-            if (e < each && tid * each < share) {
-                uint32_t x[kSmMaxCluster][2];
+            for (int e = 0; e < kSmPer; e++)
+                if (e < each && tid * each < share) {
+                    uint32_t x[kSmMaxCluster][2];
 #pragma unroll
-                for (int r = 0; r < kSmMaxCluster; r++) {
-                    const SmShared *q = cl.map_shared_rank(&S, r < C ? r : 0);
-                    x[r][0] = r < C ? q->hist[0][first_bin + e] : 0;
-                    x[r][1] = r < C && mass ? q->hist[1][first_bin + e] : 0;
+                    for (int r = 0; r < kSmMaxCluster; r++) {
+                        const SmShared *q = cl.map_shared_rank(&S, r < C ? r : 0);
+                        x[r][0] = r < C ? q->hist[0][first_bin + e] : 0;
+                        x[r][1] = r < C && mass ? q->hist[1][first_bin + e] : 0;
+                    }
+#pragma unroll
+                    for (int r = 0; r < kSmMaxCluster; r++) v[e] += (u64)x[r][0] + ((u64)x[r][1] << 16);
+                    mine += v[e];
                 }
+            u64 b = 0, far_mass = 0;
+            const u64 all = cluster_sum(mine, beyond, &b, &far_mass);
+            if (mass && !know_thr) thr = want * (double)(all + far_mass);
+            b += from + sm_block_before(mine, S.warp);
 #pragma unroll
-                for (int r = 0; r < kSmMaxCluster; r++) v[e] += (u64)x[r][0] + ((u64)x[r][1] << 16);
-                mine += v[e];
+            for (int e = 0; e < kSmPer; e++) {
+                if ((double)b < thr && (double)(b + v[e]) >= thr)
+                    for (int r = 0; r < C; r++) {
+                        SmShared *q = cl.map_shared_rank(&S, r);
+                        q->bin = first_bin + e;
+                        q->found_before = b;
+                        q->found_here = v[e];
+                    }
+                b += v[e];
             }
-        u64 b = 0, far_mass = 0;
-        const u64 all = cluster_sum(mine, beyond, &b, &far_mass);
-        const double thr = mass ? want * (double)(all + far_mass) : want;
-        b += sm_block_before(mine, S.warp);
-#pragma unroll
-        for (int e = 0; e < kSmPer; e++) {
-            if ((double)b < thr && (double)(b + v[e]) >= thr)
-                for (int r = 0; r < C; r++) {
-                    SmShared *q = cl.map_shared_rank(&S, r);
-                    q->bin = first_bin + e;
-                    q->found_before = b;
-                    q->found_here = v[e];
-                }
-            b += v[e];
-        }
-        cl.sync();
+            cl.sync();
+        };
+        add_bins(0, false);
         const int bin = S.bin;
         if (bin < 0) return false;                     // a count past all tokens of any weight: nothing to cut
-        const u64 above = S.found_before;
-        // Tokens of bins from .. bin into the lists of their CTAs, then
+        u64 above = S.found_before;
+        // A token's place within the bin, in parts of it (of part `sub`, where a part is in question)
+        int sub = -1;
+        auto place_in_bin = [&](float l) {
+            const float at = (place_of(l) - (float)bin + 0.5f) * kSmBins;
+            return sub < 0 ? at : (at - (float)sub) * kSmBins;
+        };
+        auto part_at = [&](float place) { return bin_at(fmaxf(place - 0.5f, 0.0f)); };
+        // Tokens of bins from .. bin (of part `sub` of the bin) into the lists of their CTAs, then
         // (if they fit) into the first CTA's; how many there are. Bounds a
         // little past the bins (half a bin to either side of whole numbers)
         // spare most tokens the bin's arithmetic.
         auto gather = [&](int from) {
-            const float bin_lo = fmaxf(near, top + ((float)bin + 0.6f) / per * t);
+            const float bin_lo = bin == kSmBins - 1 ? near : fmaxf(near, top + ((float)bin + 0.6f) / per * t);
             const float bin_hi = from ? top + ((float)from - 0.6f) / per * t : top;
             const float mid = from ? 0.5f * (bin_lo + bin_hi) : top, half = from ? fmaxf(bin_hi - mid, mid - bin_lo) : top - bin_lo;
             __syncthreads();
@@ -517,7 +530,8 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
                 for (int e = 0; e < E; e++) {
                     if (fabsf(v[e] - mid) > half || !(v[e] >= near)) continue;
                     const int b = bin_of(v[e]);
-                    if (b >= from && b <= bin && in(v[e], i + e)) {
+                    if (b >= from && b <= bin && in(v[e], i + e) &&
+                        (sub < 0 || part_at((place_of(v[e]) - (float)bin + 0.5f) * kSmBins) == sub)) {
                         const int at = atomicAdd(&S.n_list, 1);
                         if (at < kSmList) S.list[at] = ((u64)sm_key(v[e]) << 32) | (0xffffffffu - (uint32_t)(i + e));
                     }
@@ -550,7 +564,28 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
                 return true;
             }
         }
-        const int have = gather(bin);
+        int have = gather(bin);
+        if (have > kSmList) {
+            // Too many: a second histogram over the bin alone, in as many parts
+            for (int i = tid; i < 2 * kSmBins; i += kSmThreads) (&S.hist[0][0])[i] = 0;
+            if (tid == 0) S.bin = -1;
+            __syncthreads();
+            beyond = 0;
+            X.each([&](const float (&v)[E], int i) {
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (v[e] >= near && bin_of(v[e]) == bin && in(v[e], i + e)) {
+                        const uint32_t w = mass ? sm_weight(sm_exp(v[e], top, inv_t)) : 1u;
+                        const int b = part_at(place_in_bin(v[e]));
+                        atomicAdd(&S.hist[0][b], w & 0xffffu);
+                        if (mass) atomicAdd(&S.hist[1][b], w >> 16);
+                    }
+            });
+            add_bins(above, true);
+            sub = S.bin;
+            above = S.found_before;
+            have = gather(bin);
+        }
         if (have <= kSmList) {
             if (rank == 0) {
                 auto value = [&](u64 y) -> u64 {
@@ -564,8 +599,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
                     const bool on = tid + e * kSmThreads < have;
                     y[e] = on ? S.list[tid + e * kSmThreads] : 0;
                     val[e] = on ? value(y[e]) : 0;
-                    const float at = (place_of(sm_unkey((uint32_t)(y[e] >> 32))) - (float)bin + 0.5f) * kSmBins;
-                    part[e] = on ? max(0, min(kSmBins - 1, (int)at)) : -1;
+                    part[e] = on ? part_at(place_in_bin(sm_unkey((uint32_t)(y[e] >> 32)))) : -1;
                 }
                 __syncthreads();                       // the list is read: its room becomes counters again
                 for (int i = tid; i < 2 * kSmBins; i += kSmThreads) (&S.hist[0][0])[i] = 0;

@@ -267,8 +267,9 @@ def test_attention_lengths(lib, dtype, block, hk, group, dim):
 
 @pytest.mark.parametrize("dtype", [F32, F16])
 @pytest.mark.parametrize("new", [[2, 2, 2], [3, 0, 1], [8, 7, 1], [17, 33, 5], [70, 1, 64]])
-def test_attention_several_new_tokens(lib, dtype, new):
-    check_attention(Batch([40, 130, 0], 2, 64, 16), new, 6, dtype, extent=9)
+@pytest.mark.parametrize("dim", [64, 96, 128])
+def test_attention_several_new_tokens(lib, dtype, new, dim):
+    check_attention(Batch([40, 130, 0], 2, dim, 16), new, 6, dtype, extent=9)
 
 
 @pytest.mark.parametrize("window", [1, 7, 16, 64, 100, 5000])

@@ -215,6 +215,24 @@ def test_around_the_lists_capacity(lib, k):
         assert np.array_equal(draw(torch.tensor(x, device="cuda"), u, **kw)[0], want), kw
 
 
+@pytest.mark.parametrize("kw", [dict(top_p=0.9995), dict(top_k=20000), dict(top_k=30000, top_p=0.8),
+                                dict(temperature=40.0, top_p=0.5), dict(temperature=40.0, top_k=70000)],
+                         ids=lambda kw: "-".join(kw) + str(list(kw.values())[-1]))
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_cuts_in_the_crowd(lib, kw, dtype):
+    """Thresholds among tens of thousands of near logits: bins far past the list's capacity."""
+    rng = np.random.default_rng(6)
+    dev = torch.tensor(rng.standard_normal((3, 200058)) * 2, dtype=dtype, device="cuda")
+    x = dev.float().cpu().numpy()
+    u, want = [], []
+    for r in range(3):
+        at, share = kept64(x[r], kw.get("temperature", 1.0), kw.get("top_k", 0), kw.get("top_p", 1.0), 0.0)
+        j, uu = pick_u(share, rng)
+        u.append(uu)
+        want.append(at[j])
+    assert np.array_equal(draw(dev, u, **kw)[0], want)
+
+
 def test_refusals(lib):
     from sepia_b200.sampling import sample
     x, u = torch.zeros(2, 8, device="cuda"), torch.zeros(2, device="cuda")
