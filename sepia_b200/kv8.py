@@ -83,21 +83,21 @@ class Kv8Step:
         self._max_kv, self._bound, self._ws = max_kv, {}, {}
 
     def _for(self, cache):
-        """The step as a struct for this cache's block size, by reference."""
+        """The address of the step's struct for this cache's block size."""
         b = cache.block
         r = self._bound.get(b)
         if r is None:
             st = SepiaKv8Step.from_buffer_copy(self.struct)
             if self._max_kv is None:
                 st.max_kv = st.table_cols * b
-            r = self._bound[b] = C.byref(st)
-        return r
+            r = self._bound[b] = (C.addressof(st), st)
+        return r[0]
 
     def workspace(self, cache, attn, key):
         """The attention workspace for one shape. One per stream: a workspace serves one call at a time."""
         ws = self._ws.get(key)
         if ws is None:
-            nb = load().sepia_cuda_kv8_attn_ws_bytes(C.byref(cache.struct), self._for(cache), C.byref(attn))
+            nb = load().sepia_cuda_kv8_attn_ws_bytes(cache._ref, self._for(cache), C.addressof(attn))
             if not nb:
                 raise RuntimeError(f"sepia_b200: kv8_attn: {last_error()}")
             t = torch.empty(nb, dtype=torch.uint8, device=self.device)
@@ -125,7 +125,7 @@ class Kv8Cache:
             setattr(st, name, _check(t, name, torch.float16, (k_tail.shape[0], hk, b, d)))
         self.struct, self.n_kv_heads, self.head_dim, self.block = st, hk, d, b
         self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail = k, v, k_scale, v_scale, k_tail, v_tail
-        self._ref, lib = C.byref(st), load()
+        self._ref, lib = C.addressof(st), load()
         self._append, self._attn = lib.sepia_cuda_kv8_append, lib.sepia_cuda_kv8_attn
 
     @classmethod
@@ -175,7 +175,7 @@ class Kv8Cache:
                 _fail("rotation must be [positions, rot_dim/2, 2]")
             a.rotation = _check(rotation, "rotation", torch.float32, r)
             a.rot_positions, a.rot_dim, a.rot_adjacent = r[0], 2 * r[1], adjacent
-        if not self._append(self._ref, step._for(self), a, _stream(step.index, stream)):
+        if not self._append(self._ref, step._for(self), C.addressof(a), _stream(step.index, stream)):
             raise RuntimeError(f"sepia_b200: kv8_append failed: {last_error()}")
         return q_out
 
@@ -203,6 +203,6 @@ class Kv8Cache:
             a.tau = _check(tau, "tau", torch.float32, (n,))
         st = _stream(step.index, stream)
         ws = step.workspace(self, a, (st, a.x_f16, h, self.n_kv_heads, d, self.block, window))
-        if not self._attn(self._ref, step._for(self), a, ws[0], ws[1], st):
+        if not self._attn(self._ref, step._for(self), C.addressof(a), ws[0], ws[1], st):
             raise RuntimeError(f"sepia_b200: kv8_attn failed: {last_error()}")
         return out

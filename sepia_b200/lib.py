@@ -168,12 +168,10 @@ _PROTOS = {
     "sepia_cuda_exchange_connect": (C.c_int, [vp, vp]),
     "sepia_cuda_moe_exchange": (C.c_int, [vp, C.POINTER(SepiaMoeLayer), C.POINTER(SepiaMoeWork), vp, vp]),
     "sepia_cuda_moe_layer_sharded": (C.c_int, [vp, C.POINTER(SepiaMoeLayer), vp, C.POINTER(SepiaMoeWork), vp, vp]),
-    "sepia_cuda_kv8_append": (C.c_int, [C.POINTER(SepiaKv8Cache), C.POINTER(SepiaKv8Step),
-                                        C.POINTER(SepiaKv8Append), vp]),
-    "sepia_cuda_kv8_attn_ws_bytes": (C.c_size_t, [C.POINTER(SepiaKv8Cache), C.POINTER(SepiaKv8Step),
-                                                  C.POINTER(SepiaKv8Attn)]),
-    "sepia_cuda_kv8_attn": (C.c_int, [C.POINTER(SepiaKv8Cache), C.POINTER(SepiaKv8Step), C.POINTER(SepiaKv8Attn),
-                                      vp, C.c_size_t, vp]),
+    # (structs by address: byref() or addressof())
+    "sepia_cuda_kv8_append": (C.c_int, [vp, vp, vp, vp]),
+    "sepia_cuda_kv8_attn_ws_bytes": (C.c_size_t, [vp, vp, vp]),
+    "sepia_cuda_kv8_attn": (C.c_int, [vp, vp, vp, vp, C.c_size_t, vp]),
     "sepia_cuda_sample": (C.c_int, [C.c_int, vp, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
     "sepia_cuda_fill_blocks": (C.c_int, [C.c_int, vp, i64, i64, i64, C.c_uint64, i64, i64, C.c_float, C.c_float, vp]),
     # ---- sepia_model.h (whole-token decode engine) ----
