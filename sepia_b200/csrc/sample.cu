@@ -90,17 +90,18 @@ struct SmShared {
     SmCut cut;
 };
 
+// Sum over the warp, below 2^54: two sums of 27-bit halves, each by one instruction
+__device__ __forceinline__ u64 sm_warp_sum(u64 v) {
+    return (u64)__reduce_add_sync(0xffffffffu, (uint32_t)v & 0x7ffffffu) +
+           ((u64)__reduce_add_sync(0xffffffffu, (uint32_t)(v >> 27)) << 27);
+}
 __device__ u64 sm_block_sum(u64 v, u64 *sh) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    v = sm_warp_sum(v);
     __syncthreads();
     if (lane == 0) sh[warp] = v;
     __syncthreads();
-    v = lane < kSmThreads / 32 ? sh[lane] : 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+    return sm_warp_sum(lane < kSmThreads / 32 ? sh[lane] : 0);
 }
 // Sum over the threads before this one.
 __device__ u64 sm_block_before(u64 v, u64 *sh) {
@@ -114,10 +115,7 @@ __device__ u64 sm_block_before(u64 v, u64 *sh) {
     __syncthreads();
     if (lane == 31) sh[warp] = x;
     __syncthreads();
-    u64 w = lane < warp && lane < kSmThreads / 32 ? sh[lane] : 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-    return w + x - v;
+    return sm_warp_sum(lane < warp && lane < kSmThreads / 32 ? sh[lane] : 0) + x - v;
 }
 
 // A slice in index order: logits before the first 16-byte boundary (warp 0
@@ -159,6 +157,7 @@ struct SmSlice {
             load(j, v);
             f(v, index(j));
         }
+        if (head + body * E == n && head == 0) return;
 #pragma unroll 1
         for (int part = 0; part < 2; part++) {
             const int i = ragged(part, v);
@@ -752,8 +751,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
     target = target < total ? target : total - 1;
     const u64 here = S.sums[turn ^ 1][rank][0];
     if (target < before || target >= before + here) return;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    sum = sm_warp_sum(sum);
     before += sm_block_before(lane == 0 ? sum : 0, S.warp);
     before = __shfl_sync(0xffffffffu, before, 0);      // of the warps before this one
     if (target < before || target >= before + sum) return;
@@ -761,8 +759,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
     auto step = [&](const float (&v)[E], int i, bool on) {
         uint32_t w[E];
         const u64 mine = on ? weigh_min_p(v, i, w) : 0;    // below 2^35
-        const u64 all = (u64)__reduce_add_sync(0xffffffffu, (uint32_t)mine & 0xfffffu) +
-                        ((u64)__reduce_add_sync(0xffffffffu, (uint32_t)(mine >> 20)) << 20);
+        const u64 all = sm_warp_sum(mine);
         if (target >= before + all) {
             before += all;
             return false;
