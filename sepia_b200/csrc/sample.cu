@@ -304,7 +304,8 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
     };
     // Below this a weight rounds to 0: rounding of the bound itself cannot
     // pass a logit at less than the range (both are fp32 numbers).
-    const float floor_l = top - kSmRange * t;
+    // Never as low as -infinity, whatever T: such a logit is out.
+    const float floor_l = fmaxf(top - kSmRange * t, -3.402823466e38f);
     SmCut cut = {floor_l, INT32_MAX};                  // tokens in: l > cut.l, or l == cut.l up to an index
     auto in = [&](float l, int i) { return l >= cut.l && !(l == cut.l && i > cut.idx); };
     // Weights of a vector's tokens that are in, 0 for the others; false: all 0

@@ -141,6 +141,23 @@ def test_not_numbers_and_infinities(lib):
     assert ids.tolist() == [-1, -1, 1, 1, 1]
 
 
+@pytest.mark.parametrize("vocab", [9, 5000, 60000])
+def test_extreme_temperatures(lib, vocab):
+    """Infinite and huge: all finite logits alike, -infinity still out; tiny: the best alone, ties and all."""
+    x = torch.linspace(-5.0, 5.0, vocab, device="cuda").repeat(4, 1)
+    x[:, 0] = x[:, vocab - 1] = -float("inf")
+    x[:, 3] = x[:, 5] = 7.0
+    m = vocab - 2
+    for t in (float("inf"), 3e38):
+        ids, p = draw(x, [0.0, 1 - 2.0 ** -24, 0.5, 0.25], temperature=t)
+        assert ids[0] == 1 and ids[1] == vocab - 2 and np.allclose(p, 1.0 / m, rtol=1e-6)
+        ids, p = draw(x, [0.0, 1 - 2.0 ** -24, 0.0, 0.9], temperature=t, top_k=2)
+        assert ids.tolist() == [3, 5, 3, 5] and p.tolist() == [0.5] * 4
+    for t in (1e-38, 1e-45):
+        ids, p = draw(x, [0.0, 1 - 2.0 ** -24, 0.3, 0.6], temperature=t, top_p=0.9)
+        assert ids.tolist() == [3, 5, 3, 5] and p.tolist() == [0.5] * 4
+
+
 def test_row_stride_and_stream(lib):
     from sepia_b200.sampling import sample
     rng = np.random.default_rng(2)
