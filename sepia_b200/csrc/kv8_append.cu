@@ -11,8 +11,8 @@
 // queries.
 //
 // A prompt is bound by HBM and, close behind, by instructions (a norm is a
-// warp reduction for 4 values a lane): 8192 tokens, 64 heads over 8, fp32, 122
-// us, 5.1 TB/s with 69 % of the issue slots busy. One token is latency, 4.9 us:
+// warp reduction for 4 values a lane): 8192 tokens, 64 heads over 8, fp32, 120
+// us, 5.2 TB/s with 69 % of the issue slots busy. One token is latency, 4.1 us:
 // launch, lengths, rows (one round of loads for a whole block), norm, store.
 // 128-thread CTAs lost on every size (one token 7.8 us, 8192 tokens 144).
 #include "kv8.cuh"
@@ -24,7 +24,6 @@ namespace sepia {
 
 constexpr int kApThreads = 256;
 constexpr int kApWarps = kApThreads / 32;
-constexpr int kApMaxRows = 64 / kApWarps;   // rows of a block per warp
 constexpr int kApQRows = 4;                 // query rows per warp
 
 struct ApParams {
@@ -134,11 +133,15 @@ __device__ __forceinline__ const float2 *rotation_row(const SepiaKv8Append &a, i
     return nullptr;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kApThreads, 4) k_kv8_append(const ApParams P) {
+// MR: rows of a block per warp. A kernel for each block size: with one for
+// blocks of 64 the shorter ones ran through rows that they do not have (48
+// tokens, blocks of 32: 10.0 us, 7.8 now; ragged pieces, blocks of 16: 21.5, 16.3).
+template <typename T, int MR>
+__global__ void __launch_bounds__(kApThreads, MR == 2 ? 5 : 4) k_kv8_append(const ApParams P) {
     __shared__ float s_amax[kApWarps];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, d = 4 * lane;
-    const int Dh = P.c.head_dim, B = P.c.block, Hkv = P.c.n_kv_heads;
+    constexpr int B = MR * kApWarps;
+    const int Dh = P.c.head_dim, Hkv = P.c.n_kv_heads;
     griddep_wait();
     griddep_launch();
     if ((int)blockIdx.x >= P.kv_ctas) {
@@ -219,10 +222,12 @@ __global__ void __launch_bounds__(kApThreads, 4) k_kv8_append(const ApParams P) 
         const int lo = blk == b0 ? r0 : 0;             // rows below wait in the tail
         const int hi = full ? B : tail_rows;
         const int base = blk * B - sq.held;            // row r of the block is new token base + r
+        // a tail's warps without a new row are done
+        if (!full && (hi - 1 - warp < 0 || (hi - 1 - warp) / kApWarps * kApWarps + warp < lo)) return;
         // every row first, new ones and (where the block ends) those of the tail: one round of loads
-        float x[kApMaxRows][4];
+        float x[MR][4];
 #pragma unroll
-        for (int j = 0; j < kApMaxRows; j++) {
+        for (int j = 0; j < MR; j++) {
             const int r = warp + kApWarps * j;
             x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0.0f;
             if (r >= hi || d >= Dh) continue;
@@ -232,10 +237,10 @@ __global__ void __launch_bounds__(kApThreads, 4) k_kv8_append(const ApParams P) 
                 load4(tail + r * Dh + d, 1, x[j]);
             }
         }
-        __half2 y[kApMaxRows][2];
+        __half2 y[MR][2];
         float amax = 0.0f;
 #pragma unroll
-        for (int j = 0; j < kApMaxRows; j++) {
+        for (int j = 0; j < MR; j++) {
             const int r = warp + kApWarps * j;
             if (exact && r >= lo && r < hi) {          // the whole warp
                 double z[4] = {x[j][0], x[j][1], x[j][2], x[j][3]};
@@ -266,7 +271,7 @@ __global__ void __launch_bounds__(kApThreads, 4) k_kv8_append(const ApParams P) 
         if (id >= 0) {
             uint8_t *o = codes + ((int64_t)id * Hkv + hk) * B * Dh;
 #pragma unroll
-            for (int j = 0; j < kApMaxRows; j++) {
+            for (int j = 0; j < MR; j++) {
                 const int r = warp + kApWarps * j;
                 if (r < B && d < Dh) {
                     float2 f0 = __half22float2(y[j][0]), f1 = __half22float2(y[j][1]);
@@ -313,6 +318,15 @@ static int rows_vec(const void *p, int64_t stride, int x_f16) {
     return reinterpret_cast<uintptr_t>(p) % b == 0 && (stride * sz) % b == 0;
 }
 
+template <typename T>
+static int ap_launch(const ApParams &P, unsigned ctas, cudaStream_t st) {
+    const int rows = P.c.block / kApWarps;
+    const cudaError_t e = rows == 2   ? launch_pdl(k_kv8_append<T, 2>, ctas, kApThreads, 0, st, P)
+                          : rows == 4 ? launch_pdl(k_kv8_append<T, 4>, ctas, kApThreads, 0, st, P)
+                                      : launch_pdl(k_kv8_append<T, 8>, ctas, kApThreads, 0, st, P);
+    return check(e, "kv8_append launch");
+}
+
 }  // namespace sepia
 
 using namespace sepia;
@@ -355,7 +369,5 @@ extern "C" int sepia_cuda_kv8_append(const SepiaKv8Cache *c, const SepiaKv8Step 
     P.vec_k = rows_vec(a->k, a->k_stride, a->x_f16);
     P.vec_v = rows_vec(a->v, a->v_stride, a->x_f16);
     P.vec_q = a->q ? rows_vec(a->q, a->q_stride, a->x_f16) : 0;
-    const cudaError_t e = a->x_f16 ? launch_pdl(k_kv8_append<__half>, (unsigned)all, kApThreads, 0, as_stream(stream), P)
-                                   : launch_pdl(k_kv8_append<float>, (unsigned)all, kApThreads, 0, as_stream(stream), P);
-    return check(e, "kv8_append launch");
+    return a->x_f16 ? ap_launch<__half>(P, (unsigned)all, as_stream(stream)) : ap_launch<float>(P, (unsigned)all, as_stream(stream));
 }
