@@ -29,7 +29,7 @@
 //   Measured  1 x 32768, 64 heads over 8, fp32: 21 us, of which 12 (5.6 TB/s)
 //             are key steps and the rest start and merge; 64 ragged sequences
 //             of 2048 to 4096, fp16: 86 us, 4.8 TB/s; a window of 4096: 10.6 us.
-//             With more rows (12 x 6001, 4 new tokens: 79 us) the chains of
+//             With more rows (12 x 6001, 4 new tokens: 78 us) the chains of
 //             conversions and products bind, 25 us at the product's full rate.
 #include "kv8.cuh"
 #include "runtime.h"
