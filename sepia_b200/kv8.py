@@ -52,6 +52,14 @@ def _stream(index, stream):
     return torch._C._cuda_getCurrentRawStream(index) if stream is None else stream.cuda_stream
 
 
+def _empty_like(t, stream):
+    """A result's memory belongs to the stream that fills it."""
+    if stream is None:
+        return torch.empty_like(t, memory_format=torch.contiguous_format)
+    with torch.cuda.stream(stream):
+        return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def rotation_table(n_positions: int, rot_dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
     """Cosines and sines [n_positions, rot_dim/2, 2] of angle position * base^(-2i/rot_dim), from 64-bit angles."""
     freq = float(base) ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device) / rot_dim)
@@ -93,14 +101,15 @@ class Kv8Step:
             r = self._bound[b] = (C.addressof(st), st)
         return r[0]
 
-    def workspace(self, cache, attn, key):
+    def workspace(self, cache, attn, key, stream):
         """The attention workspace for one shape. One per stream: a workspace serves one call at a time."""
         ws = self._ws.get(key)
         if ws is None:
             nb = load().sepia_cuda_kv8_attn_ws_bytes(cache._ref, self._for(cache), C.addressof(attn))
             if not nb:
                 raise RuntimeError(f"sepia_b200: kv8_attn: {last_error()}")
-            t = torch.empty(nb, dtype=torch.uint8, device=self.device)
+            with torch.cuda.stream(stream):            # None: the current one
+                t = torch.empty(nb, dtype=torch.uint8, device=self.device)
             ws = self._ws[key] = (t.data_ptr(), nb, t)
         return ws
 
@@ -161,7 +170,7 @@ class Kv8Cache:
             a.n_heads = h = q.shape[1]
             a.q, a.q_stride = _rows(q, "q", dt, h, d, n)
             if q_out is None:
-                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+                q_out = _empty_like(q, stream)
                 a.q_out = q_out.data_ptr()
             else:
                 a.q_out = _check(q_out, "q_out", dt, (n, h, d))
@@ -191,7 +200,7 @@ class Kv8Cache:
         a.x_f16, a.scale, a.window = _F16[dt], scale, window
         a.q, a.q_stride = _rows(q, "q", dt, h, d, n)
         if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            out = _empty_like(q, stream)
             a.out = out.data_ptr()
         else:
             a.out = _check(out, "out", dt, (n, h, d))
@@ -202,7 +211,7 @@ class Kv8Cache:
         if tau is not None:
             a.tau = _check(tau, "tau", torch.float32, (n,))
         st = _stream(step.index, stream)
-        ws = step.workspace(self, a, (st, a.x_f16, h, self.n_kv_heads, d, self.block, window))
+        ws = step.workspace(self, a, (st, a.x_f16, h, self.n_kv_heads, d, self.block, window), stream)
         if not self._attn(self._ref, step._for(self), C.addressof(a), ws[0], ws[1], st):
             raise RuntimeError(f"sepia_b200: kv8_attn failed: {last_error()}")
         return out

@@ -2,6 +2,8 @@
 sepia_cuda_sample; csrc/sample.cu)."""
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from .lib import last_error, load
@@ -29,15 +31,17 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, ids=
     if v > 1 and s1 != 1:
         raise ValueError("sepia_b200: sample: the logits of a row must lie side by side")
     f, i = torch.float32, torch.int32
-    ids_p = _row(ids, "ids", i, n) if ids is not None else None
-    prob_p = _row(prob, "prob", f, n) if prob is not None else None
+    if ids is not None:
+        _row(ids, "ids", i, n)
+    if prob is not None:
+        _row(prob, "prob", f, n)
     u_p = _row(u, "u", f, n)
-    if ids is None:
-        ids = torch.empty_like(u, dtype=i)
-        ids_p = ids.data_ptr()
-    if prob is None:
-        prob = torch.empty_like(u)
-        prob_p = prob.data_ptr()
+    if ids is None or prob is None:
+        # a result's memory belongs to the stream that fills it
+        with contextlib.nullcontext() if stream is None else torch.cuda.stream(stream):
+            ids = torch.empty_like(u, dtype=i) if ids is None else ids
+            prob = torch.empty_like(u) if prob is None else prob
+    ids_p, prob_p = ids.data_ptr(), prob.data_ptr()
     st = stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(logits.device.index)
     if not load().sepia_cuda_sample(f16, logits.data_ptr(), s0 if n > 1 else v, n, v, u_p,
                                     None if temperature is None else _row(temperature, "temperature", f, n),

@@ -374,6 +374,23 @@ def test_on_another_stream(lib):
         check_rows(B)
 
 
+def test_results_belong_to_their_stream(lib):
+    """Memory that a call takes for another stream is not handed to this one when it is freed."""
+    B = Batch([100, 7], 2, 64, 16)
+    step = B.step([1, 1])
+    k, v, q = (torch.ones(2, heads, 64, device="cuda") for heads in (2, 2, 4))
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream()
+    turned = B.cache.append(step, k, v, q, stream=st)
+    out = B.cache.attention(step, q, 0.125, stream=st)
+    st.synchronize()
+    theirs = {turned.data_ptr(), out.data_ptr()} | {ws[0] for ws in step._ws.values()}
+    assert len(theirs) == 3
+    del turned, out, step
+    mine = [torch.empty(n, dtype=torch.uint8, device="cuda") for n in (2048, 2048, 16, 4096) for _ in range(64)]
+    assert not theirs & {t.data_ptr() for t in mine}
+
+
 def test_graph_replay(lib):
     """A captured step is replayed as the lengths on the device change."""
     hk, h, dim, b = 2, 8, 64, 16

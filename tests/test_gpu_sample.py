@@ -175,6 +175,21 @@ def test_row_stride_and_stream(lib):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and torch.equal(c[0], d[0]) and int(a[0].max()) < 1000
 
 
+def test_results_belong_to_their_stream(lib):
+    """Memory that a call takes for another stream is not handed to this one when it is freed."""
+    from sepia_b200.sampling import sample
+    x, u = torch.zeros(9, 1000, device="cuda"), torch.full((9,), 0.37, device="cuda")
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream()
+    ids, p = sample(x, u, stream=st)
+    st.synchronize()
+    theirs = {ids.data_ptr(), p.data_ptr()}
+    assert ids.tolist() == [370] * 9
+    del ids, p
+    mine = [torch.empty(9, dtype=torch.int32, device="cuda") for _ in range(64)]
+    assert not theirs & {t.data_ptr() for t in mine}
+
+
 def test_frequencies(lib):
     """Evenly spread u meet each token as often as its share says, to one count."""
     rng = np.random.default_rng(3)
