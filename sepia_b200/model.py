@@ -293,16 +293,17 @@ class DeviceModel:
         the argmax after feeding id i-1 (real_generate's loop). With sampling
         and n_gen + 1 uniform numbers u in [0, 1), id i is drawn with u[i]
         (the last number draws the token that a further step would consume)."""
-        ids = torch.as_tensor(np.asarray(prompt, np.int32), device=self.device)
-        out = torch.empty(n_gen, dtype=torch.int32, device=self.device)
-        self.reset(stream)
-        self.prefill(ids, True, stream)
-        if sampling is None:
-            self.decode(out, n_gen, stream)
-        else:
-            u = torch.as_tensor(u, dtype=torch.float32, device=self.device).contiguous()
-            assert u.numel() >= n_gen + 1, "one number per token and one more"
-            self.set_sampling(sampling, stream)
-            self.draw(u, stream)
-            self.decode_sampled(out, u[1:], stream)
-        return out.cpu().numpy()
+        with torch.cuda.stream(stream):                    # copies and results too; None: the current one
+            ids = torch.as_tensor(np.asarray(prompt, np.int32), device=self.device)
+            out = torch.empty(n_gen, dtype=torch.int32, device=self.device)
+            self.reset(stream)
+            self.prefill(ids, True, stream)
+            if sampling is None:
+                self.decode(out, n_gen, stream)
+            else:
+                u = torch.as_tensor(u, dtype=torch.float32, device=self.device).contiguous()
+                assert u.numel() >= n_gen + 1, "one number per token and one more"
+                self.set_sampling(sampling, stream)
+                self.draw(u, stream)
+                self.decode_sampled(out, u[1:], stream)
+            return out.cpu().numpy()

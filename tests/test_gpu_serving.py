@@ -100,6 +100,17 @@ def test_drawn_tokens(built, kv_block):
     assert np.array_equal(m.generate(prompt, n, sampling=Sampling(temperature=0.0), u=u), greedy)
 
 
+def test_generate_on_a_stream(built):
+    from sepia_b200.model import Sampling
+    _, prompt, m = built
+    u = np.linspace(0.05, 0.95, 25).astype(np.float32)
+    st = torch.cuda.Stream()
+    for kw in (dict(), dict(sampling=Sampling(temperature=0.9, top_p=0.95), u=u)):
+        want = m.generate(prompt, 24, **kw)
+        torch.cuda.synchronize()
+        assert (m.generate(prompt, 24, stream=st, **kw) == want).all()
+
+
 def test_refusals(built, lib):
     from sepia_b200.model import DeviceModel, Sampling
     d, prompt, _ = built
