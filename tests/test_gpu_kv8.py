@@ -354,6 +354,23 @@ def test_device_bounds(lib, bad):
     assert lib.sepia_cuda_device_error(None) == 0
 
 
+def test_a_block_out_of_range_is_not_seen(lib):
+    """Positions 16-31 lie in no block: what is left is the sequence of 16. The same keys in the same places, so the
+    same sums."""
+    from sepia_b200.kv8 import Kv8Step
+    B = Batch([31], 2, 64, 16)
+    q = torch.randn(1, 4, 64, device="cuda")
+    table = B.table.clone()
+    table[0, 1] = -1
+    kv_len = torch.tensor([15], dtype=torch.int32, device="cuda")
+    want = B.cache.attention(Kv8Step(B.table, kv_len, slot=B.slot), q, 0.125)
+    torch.cuda.synchronize()
+    lib.sepia_cuda_device_error(None)
+    got = B.cache.attention(Kv8Step(table, B.kv_len, slot=B.slot), q, 0.125)
+    assert lib.sepia_cuda_device_error(None) == 2
+    assert torch.allclose(got, want, rtol=0, atol=1e-6) and want.abs().max() > 0.01
+
+
 def test_offsets_past_32_bits(lib):
     """A pool of more than 2^32 codes; the sequence lives in its last blocks."""
     from sepia_b200.kv8 import Kv8Cache
