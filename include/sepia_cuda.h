@@ -287,7 +287,8 @@ int sepia_cuda_kv8_append(const SepiaKv8Cache *c, const SepiaKv8Step *b, const S
  * to one call at a time. A key or value that is not a number spoils the rows
  * that see its position, and no other. */
 typedef struct {
-    int32_t x_f16;                       /* q and out: 1 fp16, 0 fp32 */
+    int32_t x_f16;                       /* q and out: 1 fp16, 0 fp32; scores, weights' sums and outputs are summed in
+                                            fp32, an fp32 q and the weights are held to 22 bits, an fp16 out is rounded once */
     int32_t n_heads;
     const void *q;                       /* [n_tokens, n_heads, head_dim], token stride q_stride */
     int64_t q_stride;

@@ -14,8 +14,8 @@
 //   Operands  mma m16n8k16 in fp16 with fp32 sums, the codes as the 16-row
 //             operand (scores: 16 keys x 8 rows; output: 16 dims x 8 rows),
 //             so that 8 rows fill it. e4m3 codes are fp16 numbers exactly;
-//             block scales multiply the score and the weight. fp32 rows: q and
-//             the weight are two fp16 terms (22 bits), summed in one result.
+//             block scales multiply the score and the weight. The weight is
+//             two fp16 terms (22 bits), summed in one result; so is an fp32 q.
 //   Layout    the dims of a k step and of an output tile are permuted so that
 //             a lane's codes are 16 consecutive bytes of a key row (K) or of
 //             four key rows (V). A warp copies its tiles as they lie (cp.async,
@@ -116,7 +116,7 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
 template <typename T, int DP, int NB>
 struct K8Cfg {
     static constexpr int UNITS = NB == 1 ? 2 : 1;     // 16-key tiles whose scores are in registers at once
-    static constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;   // fp16 terms of a row
+    static constexpr int TERMS = sizeof(T) == 4 ? 2 : 1;   // fp16 terms of a row of q
     static constexpr int RT = 8 * NB;                 // rows of a tile
     static constexpr int KW = DP / 64;                // 16-byte pieces of a key row per lane
     static constexpr int VB = DP / 8;                 // bytes of a value row per lane
@@ -505,7 +505,9 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const float il = exp2_fast(-lv[u]);
-            uint32_t w[NB][TERMS][2];
+            // weights as two fp16 terms, for fp16 rows too: with one (11 bits) 41 % of the
+            // results of 64 fp16 sequences were not the exact ones' fp16 values (86 us), with two 0.2 % (88 us)
+            uint32_t w[NB][2][2];
 #pragma unroll
             for (int g = 0; g < NB; g++) {
                 float *q = p[g][u];
@@ -517,10 +519,8 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
                 for (int n = 0; n < 2; n++) {          // keys gid + 8 n: 8 x 8 weights, turned
                     const __half2 hi = __floats2half2_rn(q[2 * n], q[2 * n + 1]);
                     w[g][0][n] = transpose8(*reinterpret_cast<const uint32_t *>(&hi));
-                    if constexpr (TERMS == 2) {
-                        const float2 b = __half22float2(hi);
-                        w[g][TERMS - 1][n] = transpose8(pack_half2(q[2 * n] - b.x, q[2 * n + 1] - b.y));
-                    }
+                    const float2 b = __half22float2(hi);
+                    w[g][1][n] = transpose8(pack_half2(q[2 * n] - b.x, q[2 * n + 1] - b.y));
                 }
             }
 #pragma unroll
@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
 #pragma unroll
                 for (int g = 0; g < NB; g++)
 #pragma unroll
-                    for (int k = 0; k < TERMS; k++) mma16(O[g][mt], a, w[g][k][0], w[g][k][1]);
+                    for (int k = 0; k < 2; k++) mma16(O[g][mt], a, w[g][k][0], w[g][k][1]);
             }
         }
     };
