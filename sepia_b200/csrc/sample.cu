@@ -187,6 +187,9 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
     const int C = cl.num_blocks(), rank = cl.block_rank();
     const int row = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, V = P.vocab;
     SmShared *first = cl.map_shared_rank(&S, 0);
+    // A CTA's shared memory may be written by the others once it is known to
+    // have started: it arrives here, and they wait before their first store.
+    cl.barrier_arrive();
     griddep_wait();
     griddep_launch();
     const int i0 = min(V, rank * P.slice), n = min(V, i0 + P.slice) - i0;
@@ -243,6 +246,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
     if (lane == 0) reinterpret_cast<float *>(S.warp)[tid >> 5] = top;
     if (tid == 0) S.first_idx = INT32_MAX;
     __syncthreads();
+    cl.barrier_wait();                                 // every CTA has started; hidden behind the load
     if (tid < C) {
 #pragma unroll
         for (int w = 0; w < kSmThreads / 32; w++) top = fmaxf(top, reinterpret_cast<float *>(S.warp)[w]);
