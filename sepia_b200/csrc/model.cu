@@ -429,6 +429,21 @@ __global__ void k_state_new_call(ModelState *st) {
 using namespace sepia;
 
 // ============================================================== host side
+// A captured decode step and the caller's arrays baked into it: they are set
+// when the graph exists and cleared with it, so a call that fails in between
+// leaves no graph behind that answers for other arrays.
+struct StepGraph {
+    cudaGraph_t graph = nullptr;
+    cudaGraphExec_t exec = nullptr;
+    int32_t *out = nullptr;
+    const float *u = nullptr;
+    void drop() {
+        if (exec) cudaGraphExecDestroy(exec);
+        if (graph) cudaGraphDestroy(graph);
+        *this = StepGraph();
+    }
+};
+
 struct SepiaModel {
     SepiaModelDesc d;
     std::vector<SepiaModelLayer> layers;
@@ -448,9 +463,7 @@ struct SepiaModel {
     void *moe_ws_mem = nullptr;
     SepiaMoeWork ws{};
     int64_t max_q = 0, max_kv = 0, max_r = 0, max_rl = 0, max_ff = 0;
-    cudaGraph_t graph = nullptr;
-    cudaGraphExec_t exec = nullptr;
-    int32_t *graph_out = nullptr;    // out_ids array baked into the graph
+    StepGraph greedy;
     // expert sharding (world > 1)
     int rank = 0, world = 1;
     SepiaExchange *xchg = nullptr;   // the sharded MoE layers' exchange
@@ -465,10 +478,7 @@ struct SepiaModel {
     float *draw_f = nullptr;         // temperature, top_p, min_p
     int32_t *draw_k = nullptr;       // top_k
     bool draw_set = false;
-    cudaGraph_t graph_s = nullptr;
-    cudaGraphExec_t exec_s = nullptr;
-    int32_t *graph_s_out = nullptr;
-    const float *graph_s_u = nullptr;
+    StepGraph sampled;
 };
 
 namespace {
@@ -822,10 +832,8 @@ extern "C" int sepia_model_create_kv8(const SepiaModelDesc *d, int32_t block, Se
 
 extern "C" void sepia_model_destroy(SepiaModel *m) {
     if (!m) return;
-    if (m->exec) cudaGraphExecDestroy(m->exec);
-    if (m->graph) cudaGraphDestroy(m->graph);
-    if (m->exec_s) cudaGraphExecDestroy(m->exec_s);
-    if (m->graph_s) cudaGraphDestroy(m->graph_s);
+    m->greedy.drop();
+    m->sampled.drop();
     if (m->ws8) cudaFree(m->ws8);
     if (m->mem) cudaFree(m->mem);
     if (m->xchg) sepia_cuda_exchange_destroy(m->xchg);
@@ -876,20 +884,14 @@ extern "C" int sepia_model_prefill(SepiaModel *m, const int32_t *ids, int32_t n,
     return 1;
 }
 
-// n steps, replayed from a graph kept in (graph, exec) while its arrays are
-// the same; with u each step draws, without it takes the argmax.
-static int decode_steps(SepiaModel *m, int32_t n, int32_t *out_ids, const float *u, cudaGraph_t &graph,
-                        cudaGraphExec_t &exec, bool same, cudaStream_t st) {
+// n steps, replayed from the graph G, which is kept while its arrays are the
+// same; with u each step draws, without it takes the argmax.
+static int decode_steps(SepiaModel *m, int32_t n, int32_t *out_ids, const float *u, StepGraph &G, cudaStream_t st) {
+    if (G.out != out_ids || G.u != u) G.drop();
     k_state_new_call<<<1, 1, 0, st>>>(m->st);
     if (!check(cudaGetLastError(), "model: decode")) return 0;
-    if (exec && !same) {
-        cudaGraphExecDestroy(exec);
-        cudaGraphDestroy(graph);
-        exec = nullptr;
-        graph = nullptr;
-    }
     int32_t i0 = 0;
-    if (!exec) {
+    if (!G.exec) {
         // The first step runs eagerly (it sets every kernel's attributes
         // outside any capture), the rest replay its captured twin.
         if (!embed(m, 1, nullptr, out_ids, st) || !run_layers(m, true, st, u)) return 0;
@@ -906,19 +908,18 @@ static int decode_steps(SepiaModel *m, int32_t n, int32_t *out_ids, const float 
         cudaStreamDestroy(cs);
         if (!ok) { if (g) cudaGraphDestroy(g); return 0; }
         if (!check(e, "model: end capture")) return 0;
+        cudaGraphExec_t exec = nullptr;
         if (!check(cudaGraphInstantiate(&exec, g, 0), "model: graph instantiate")) { cudaGraphDestroy(g); return 0; }
-        graph = g;
+        G = StepGraph{g, exec, out_ids, u};
     }
     for (int32_t i = i0; i < n; i++)
-        if (!check(cudaGraphLaunch(exec, st), "model: graph launch")) return 0;
+        if (!check(cudaGraphLaunch(G.exec, st), "model: graph launch")) return 0;
     return 1;
 }
 
 extern "C" int sepia_model_decode(SepiaModel *m, int32_t n, int32_t *out_ids, void *stream) {
     if (!m || !out_ids || n <= 0) return fail("model: decode needs out_ids and n > 0");
-    const bool same = m->graph_out == out_ids;
-    m->graph_out = out_ids;
-    return decode_steps(m, n, out_ids, nullptr, m->graph, m->exec, same, as_stream(stream));
+    return decode_steps(m, n, out_ids, nullptr, m->greedy, as_stream(stream));
 }
 
 extern "C" int sepia_model_set_sampling(SepiaModel *m, float temperature, int32_t top_k, float top_p, float min_p,
@@ -941,10 +942,7 @@ extern "C" int sepia_model_draw(SepiaModel *m, const float *u, void *stream) {
 extern "C" int sepia_model_decode_sampled(SepiaModel *m, int32_t n, int32_t *out_ids, const float *u, void *stream) {
     if (!m || !out_ids || !u || n <= 0) return fail("model: decode_sampled needs out_ids, u and n > 0");
     if (!m->draw_set) return fail("model: decode_sampled before sepia_model_set_sampling");
-    const bool same = m->graph_s_out == out_ids && m->graph_s_u == u;
-    m->graph_s_out = out_ids;
-    m->graph_s_u = u;
-    return decode_steps(m, n, out_ids, u, m->graph_s, m->exec_s, same, as_stream(stream));
+    return decode_steps(m, n, out_ids, u, m->sampled, as_stream(stream));
 }
 
 extern "C" const float *sepia_model_logits(const SepiaModel *m) { return m ? m->logits : nullptr; }
