@@ -243,10 +243,12 @@ typedef struct {
  * (after append) sees kv_len[s] plus the new tokens. A sequence with
  * kv_len < 0 is idle: nothing is appended and its outputs are zero. A
  * sequence that breaks a bound (more than max_new new tokens, more than max_kv
- * in all, a slot out of range) is skipped the same way and sets the device
- * error word to 2. A block out of range sets it too, and is neither written nor
- * seen, as a position past the rotation table does, whose rows stay unrotated.
- * Two sequences of a step never share a block that the step writes, nor a slot. */
+ * in all, a slot out of range) is skipped the same way, its rows among the
+ * n_tokens zero however many there are, and sets the device error word to 2.
+ * start never falls; rows that it gives to no sequence are not written. A
+ * block out of range sets it too, and is neither written nor seen, as a
+ * position past the rotation table does, whose rows stay unrotated. Two
+ * sequences of a step never share a block that the step writes, nor a slot. */
 typedef struct {
     int32_t n_seqs, n_tokens;            /* n_tokens: new tokens of all sequences */
     int32_t max_new, max_kv;             /* per sequence: new tokens, tokens held after the step */

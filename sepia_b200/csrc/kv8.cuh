@@ -9,13 +9,19 @@ namespace sepia {
 
 constexpr int kKv8MaxDh = 128;
 
-// One sequence's part of a step. add < 0: idle or out of bounds (`rows` of
-// its token rows, from n0, still lie inside the step's n_tokens).
+// One sequence's part of a step. add < 0: idle or out of bounds; `rows` of
+// its token rows, from n0, still lie inside the step's n_tokens, and may be
+// more than max_new where that bound is the broken one.
 struct Kv8Seq {
     int n0, rows;        // first new token, token rows inside the step
     int held, add;       // tokens held before the step, new tokens
     int slot;
 };
+
+// Whether a sequence's token rows are within the step's bounds
+__device__ __forceinline__ bool kv8_rows_ok(const SepiaKv8Step &b, int n0, int add) {
+    return n0 >= 0 && add >= 0 && (int64_t)n0 + add <= b.n_tokens && add <= b.max_new;
+}
 
 __device__ __forceinline__ Kv8Seq kv8_seq(const SepiaKv8Cache &c, const SepiaKv8Step &b, int s, int *err) {
     Kv8Seq q;
@@ -23,8 +29,8 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const SepiaKv8Cache &c, const SepiaKv8
     q.slot = b.slot ? b.slot[s] : s;
     q.n0 = b.start ? b.start[s] : s;
     q.add = b.start ? b.start[s + 1] - q.n0 : 1;
-    const bool rows_ok = q.n0 >= 0 && q.add >= 0 && (int64_t)q.n0 + q.add <= b.n_tokens && q.add <= b.max_new;
-    q.rows = rows_ok ? q.add : 0;
+    const bool rows_ok = kv8_rows_ok(b, q.n0, q.add);
+    q.rows = rows_ok ? q.add : q.n0 >= 0 ? max(0, min(q.add, b.n_tokens - q.n0)) : 0;
     const int64_t total = (int64_t)q.held + q.add;
     const bool fits = total <= b.max_kv && total <= (int64_t)b.table_cols * c.block && q.slot >= 0 && q.slot < c.n_slots;
     if (q.held < 0 || !rows_ok || !fits) {
@@ -32,6 +38,15 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const SepiaKv8Cache &c, const SepiaKv8
         q.add = -1;
     }
     return q;
+}
+
+// Zeros for the step's rows of a sequence that is skipped, row elements `row`,
+// by the threads first, first + all, ...; out of line, for it is rare and
+// would cost the kernels around it registers.
+template <typename T>
+__device__ __noinline__ void kv8_zero_rows(T *out, int n0, int rows, int row, unsigned first, unsigned all) {
+    const int64_t n = (int64_t)rows * row;
+    for (int64_t e = first; e < n; e += all) out[(int64_t)n0 * row + e] = (T)0.0f;
 }
 
 // Pool block of column `col` of sequence s; -1 (and the error word) if the table's entry is out of range.

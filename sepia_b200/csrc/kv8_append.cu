@@ -149,13 +149,14 @@ __global__ void __launch_bounds__(kApThreads, MR == 2 ? 5 : 4) k_kv8_append(cons
         const int item = blockIdx.x - P.kv_ctas;
         const int s = item / P.q_items, H = P.a.n_heads;
         const Kv8Seq sq = kv8_seq(P.c, P.b, s, P.err);
-        const int rows = sq.rows * H, first = ((item - s * P.q_items) * kApWarps + warp) * kApQRows;
-        if (first >= rows) return;                     // the whole warp
-        if (sq.add < 0) {                              // idle or out of bounds: zeros
-            for (int r = first; r < min(rows, first + kApQRows); r++)
-                for (int e = lane; e < Dh; e += 32) ((T *)P.a.q_out)[((int64_t)sq.n0 * H + r) * Dh + e] = (T)0.0f;
+        const int first = ((item - s * P.q_items) * kApWarps + warp) * kApQRows;
+        if (sq.add < 0) {                              // idle or out of bounds: zeros, of more than max_new rows too
+            kv8_zero_rows((T *)P.a.q_out, sq.n0, sq.rows, H * Dh, (unsigned)(item - s * P.q_items) * kApThreads + tid,
+                          (unsigned)P.q_items * kApThreads);
             return;
         }
+        const int rows = sq.rows * H;
+        if (first >= rows) return;                     // the whole warp
         const int i0 = first / H, h0 = first - i0 * H; // rows are (token, head); the next row's by counting on
         float x[kApQRows][4], w[4] = {}, f[kApQRows];
         if (P.a.q_norm && d < Dh)

@@ -156,18 +156,15 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
     griddep_wait();
     griddep_launch();
     const Kv8Seq sq = kv8_seq(P.c, P.b, s, P.err);
-    const int rows = sq.rows * G - rt * RT;            // rows of this tile that exist (may exceed RT)
     const int64_t cell = ((int64_t)(s * gridDim.y + blockIdx.y) * P.splits + split) * RT;   // of this chunk's rows
     if (P.splits > 1 && tid < RT) P.part_ml[cell + tid] = make_float2(kLowest, 0.0f);       // empty until it is not
-    if (rows <= 0) return;
-    if (sq.add < 0) {                                  // idle or out of bounds: zeros
-        if (split == 0 && P.splits == 1)
-            for (int i = tid; i < min(rows, RT) * Dh; i += kK8Threads) {
-                const int R = rt * RT + i / Dh, t = R / G;
-                ((T *)P.a.out)[((int64_t)(sq.n0 + t) * H + hk * G + (R - t * G)) * Dh + i % Dh] = (T)0.0f;
-            }
+    if (sq.add < 0) {                                  // idle or out of bounds: zeros, of more than max_new rows too
+        if (split == 0)
+            kv8_zero_rows((T *)P.a.out, sq.n0, sq.rows, H * Dh, blockIdx.y * kK8Threads + tid, gridDim.y * kK8Threads);
         return;
     }
+    const int rows = sq.rows * G - rt * RT;            // rows of this tile that exist (may exceed RT)
+    if (rows <= 0) return;
     // tokens of the tile, the positions that any of them sees, this CTA's chunk
     const int ta = rt * RT / G, tb = min(sq.add - 1, (rt * RT + RT - 1) / G);
     const int pa = sq.held + ta, pb = sq.held + tb;
@@ -834,8 +831,8 @@ __global__ void __launch_bounds__(kK8Threads) k_kv8_merge(const K8Params P) {
                 for (int e = 0; e < 4; e++) A[e] += f * s_part[w][d + e];
         }
     }
-    // rows outside the step (a sequence out of bounds among them) do not exist
-    if (d < Dh && n0 >= 0 && n1 <= P.b.n_tokens && n1 - n0 <= P.b.max_new && t < n1 - n0)
+    // a sequence whose rows break a bound has none here (k_kv8_attn zeroed what lies inside the step)
+    if (d < Dh && kv8_rows_ok(P.b, n0, n1 - n0) && t < n1 - n0)
         put_row((T *)P.a.out + ((int64_t)(n0 + t) * H + h) * Dh + d, A, L);
 }
 
