@@ -71,10 +71,11 @@ class Kv8Step:
     """One step of a batch. table int32 [n_seqs, columns], kv_len int32
     [n_seqs] (tokens held before the step; < 0: idle), start int32
     [n_seqs + 1] (None: one new token each), slot int32 [n_seqs] (None: row s
-    of the tails). n_tokens, max_new and max_kv are host bounds; max_kv
-    defaults to what the table can hold."""
+    of the tails). n_tokens, max_new and max_kv are host bounds; max_new
+    defaults to n_tokens with start (a tighter bound is less work) and to 1
+    without, max_kv to what the table can hold."""
 
-    def __init__(self, table, kv_len, start=None, slot=None, n_tokens=None, max_new=1, max_kv=None):
+    def __init__(self, table, kv_len, start=None, slot=None, n_tokens=None, max_new=None, max_kv=None):
         n = kv_len.shape[0]
         if table.dim() != 2:
             _fail("table must have two dimensions")
@@ -83,8 +84,9 @@ class Kv8Step:
         st.kv_len = _check(kv_len, "kv_len", torch.int32, (n,))
         st.start = _check(start, "start", torch.int32, (n + 1,)) if start is not None else None
         st.slot = _check(slot, "slot", torch.int32, (n,)) if slot is not None else None
-        st.n_seqs, st.table_cols, st.max_new = n, table.shape[1], int(max_new)
+        st.n_seqs, st.table_cols = n, table.shape[1]
         st.n_tokens = n if n_tokens is None else int(n_tokens)
+        st.max_new = int(max_new) if max_new is not None else 1 if start is None else st.n_tokens
         st.max_kv = -1 if max_kv is None else int(max_kv)
         self.n_tokens, self.struct, self._keep = st.n_tokens, st, (table, kv_len, start, slot)
         self.device, self.index = kv_len.device, kv_len.device.index

@@ -81,3 +81,23 @@ def test_a_broken_bound_gives_zeros(lib, bad, max_kv, dtype):
     assert torch.all(runs[1][0] != 7) and torch.all(runs[1][1] != 7)
     assert torch.equal(runs[0][0], runs[1][0]) and torch.equal(runs[0][1], runs[1][1])
     assert same(runs[0][2], runs[1][2])             # the cache: only the neighbours' tokens went in
+
+
+def test_steps_with_start_need_no_max_new(lib):
+    """Left out, the bound is all the step's tokens: no sequence is skipped."""
+    from sepia_b200.kv8 import Kv8Step
+    new = [2, 0, 5]
+    start = torch.tensor([0, 2, 2, 7], dtype=torch.int32, device="cuda")
+    k, v, q = (torch.randn(7, heads, DIM, device="cuda") for heads in (HK, HK, H))
+    torch.cuda.synchronize()
+    lib.sepia_cuda_device_error(None)
+    results = []
+    for kw in (dict(max_new=max(new)), dict()):
+        B = Batch([31, 40, 9], HK, DIM, 16, seed=3)
+        step = Kv8Step(B.table, B.kv_len, start=start, slot=B.slot, n_tokens=7, **kw)
+        turned = B.cache.append(step, k, v, q=q)
+        results.append((turned, B.cache.attention(step, turned, 0.125)))
+    assert lib.sepia_cuda_device_error(None) == 0
+    assert torch.equal(results[0][0], results[1][0]) and torch.allclose(results[0][1], results[1][1], rtol=0, atol=1e-5)
+    assert torch.all(results[1][1] != 0)
+    assert Kv8Step(B.table, B.kv_len).struct.max_new == 1
