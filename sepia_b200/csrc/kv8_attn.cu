@@ -53,7 +53,11 @@ constexpr float kLowest = -3.402823466e38f;
 // The maximum is only moved (and the output rescaled) when a weight would
 // pass 2^15, so it may lag by two places. The smallest fp16 step, 2^-24, is
 // then 2^-37 of the greatest weight, and 2^-37 + the spread of the scales.
-constexpr float kPBits = 13.0f, kPMax = 15.0f;
+// Tiles without any value (hidden ones, zeros) count as of the exponent
+// kNoValue, below those of all scales (2^-32 for the least fp16 number): with
+// the scale of 1 that stands beside a block of zeros they would cost the others'
+// weights as many places as their values are small.
+constexpr float kPBits = 13.0f, kPMax = 15.0f, kNoValue = -60.0f;
 
 struct K8Params {
     SepiaKv8Cache c;
@@ -278,7 +282,7 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
                     cp_async_bytes<4>(st_u + to, P.c.k_scale + (int64_t)id_l * Hkv + hk);
                     cp_async_bytes<4>(st_u + to + 4, P.c.v_scale + (int64_t)id_l * Hkv + hk);
                 } else {
-                    *reinterpret_cast<float2 *>(st + to) = make_float2(-1.0f, 1.0f);
+                    *reinterpret_cast<float2 *>(st + to) = make_float2(-1.0f, __uint_as_float((uint32_t)(127 + (int)kNoValue) << 23));
                 }
             }
             copy(i, (const uint8_t *)P.c.k, 0, to_k);
@@ -398,14 +402,19 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
     // scale (negative: hidden) and the exponent of its value scale. kf(S):
     // the key products; entry i of S[g][u]: key gid + 8 (i / 2), row
     // 2 tig + i % 2. vf(u, mt, a): the values' operand. bias(g, i): the band's
-    // entry for key gid + 8 (i / 2), row i % 2. clean(u): values that are not
+    // entry for key gid + 8 (i / 2), row i % 2. some(u): whether any of this
+    // lane's values is not 0 (called after kf). clean(u): values that are not
     // numbers to 0, and which of the tile's 16 keys had any among this lane's.
-    auto step = [&](auto units, int t0, const float *ksc, const float *ev, auto kf, auto vf, auto bias, auto clean) {
+    auto step = [&](auto units, int t0, const float *ksc, float *ev, auto kf, auto vf, auto bias, auto some, auto clean) {
         constexpr int U = decltype(units)::value;
         float S[NB][U][4], f2[U], lv[U];
         kf(S);
-        const float top_ev = U == 2 ? fmaxf(ev[0], ev[U - 1]) : ev[0];
-        if (top_ev > eref) {                           // the whole warp
+        float top_ev = U == 2 ? fmaxf(ev[0], ev[U - 1]) : ev[0];
+        if (top_ev > eref) {                           // the whole warp; seldom
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (!__any_sync(0xffffffffu, some(u))) ev[u] = kNoValue;
+            top_ev = fmaxf(eref, U == 2 ? fmaxf(ev[0], ev[U - 1]) : ev[0]);
             const float f = exp2_fast(eref - top_ev);
 #pragma unroll
             for (int g = 0; g < NB; g++)
@@ -559,8 +568,9 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
 #pragma unroll
                 for (int e = 0; e < F::VB / 2; e++) most = __hmax2(most, __habs2(*reinterpret_cast<const __half2 *>(&v[k][e])));
             const float amax = warp_max(fmaxf(__low2float(most), __high2float(most)));
-            const int ex = amax > 0.0f ? (int)(__float_as_uint(amax) >> 23) - 127 - 8 : -60;
-            const float f = __uint_as_float((uint32_t)(127 - ex) << 23), one = 1.0f, ev_tail = (float)ex;
+            const int ex = amax > 0.0f ? (int)(__float_as_uint(amax) >> 23) - 127 - 8 : (int)kNoValue;
+            const float f = __uint_as_float((uint32_t)(127 - ex) << 23), one = 1.0f;
+            float ev_tail = (float)ex;
 #pragma unroll
             for (int k = 0; k < 4; k++)
 #pragma unroll
@@ -601,6 +611,7 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
                     const int far = pos[g][i & 1] - (t0 + gid + 8 * (i >> 1));
                     return far >= 0 && far < E ? rel[rel_at[g][i & 1] + far] : 0.0f;
                 },
+                [&](int) { return true; },             // ev_tail is of the values themselves
                 [&](int) {
                     uint32_t nan = 0;
 #pragma unroll
@@ -700,6 +711,16 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
             },
             [&](int g, int k) {
                 return *reinterpret_cast<const float *>(st + 2 * F::kTileB + F::kHeadB + (8 * g + 4 * u0 + k) * 128 + lane * 4);
+            },
+            [&](int u) {
+                uint32_t any = 0;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t *x = reinterpret_cast<const uint32_t *>(at + u * F::kTileB + F::kKeyB + (k >> 1) * 8 * DP + from_v[k & 1]);
+#pragma unroll
+                    for (int e = 0; e < F::VB / 4; e++) any |= x[e];
+                }
+                return (any & 0x7f7f7f7fu) != 0;
             },
             [&](int u) {                               // in the slots: no other lane reads these bytes
                 uint32_t nan = 0;
