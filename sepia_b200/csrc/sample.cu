@@ -63,10 +63,25 @@ __device__ __forceinline__ float sm_unkey(uint32_t k) {
 // (l - max)/T, at most 0, and e = exp of it; the best token's is 1 also where
 // max is infinite, or 1/T is (the least of NaN and 0 is 0)
 __device__ __forceinline__ float sm_exponent(float l, float best, float inv_t) {
-    return fminf((l - best) * inv_t, 0.0f);
+    return fminf(__fmul_rn(__fsub_rn(l, best), inv_t), 0.0f);
 }
 __device__ __forceinline__ float sm_exp(float l, float best, float inv_t) { return expf(sm_exponent(l, best, inv_t)); }
-__device__ __forceinline__ u64 sm_weight(float e) { return (u64)__float2uint_rn(e * kSmOne); }
+__device__ __forceinline__ u64 sm_weight(float e) { return (u64)__float2uint_rn(__fmul_rn(e, kSmOne)); }
+// A token's place among the bins, from its exponent, and among the parts of
+// a bin, from its place. The histogram, the gather and the sums have to put a
+// token into the same bin wherever they work it out, so every step is rounded
+// by itself here: the compiler must not join two of them at one site and not
+// at another. Each step keeps the order of places.
+__device__ __forceinline__ float sm_place(float exponent, float per) { return __fmul_rn(exponent, per); }
+__device__ __forceinline__ float sm_part_place(float place, int bin) {
+    return __fmul_rn(__fadd_rn(__fsub_rn(place, (float)bin), 0.5f), (float)kSmBins);
+}
+// The nearest whole number, by adding 2^23 (a conversion would hold up the
+// exponentials' unit); places may lie past the last bin by their rounding.
+__device__ __forceinline__ int sm_nearest(float place) {
+    return (int)min(kSmBins - 1u, __float_as_uint(__fadd_rn(place, 8388608.0f)) - 0x4b000000u);
+}
+__device__ __forceinline__ int sm_part(float part_place) { return sm_nearest(fmaxf(__fsub_rn(part_place, 0.5f), 0.0f)); }
 
 // The last token in
 struct SmCut {
@@ -321,7 +336,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
 #pragma unroll
         for (int e = 0; e < E; e++) {
             x[e] = sm_exponent(v[e], top, inv_t);
-            const uint32_t y = __float2uint_rn(expf(x[e]) * kSmOne);
+            const uint32_t y = (uint32_t)sm_weight(expf(x[e]));
             w[e] = v[e] >= cut.l ? y : 0u;
         }
         if (cut.idx != INT32_MAX) {                    // the whole cluster
@@ -433,13 +448,8 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
         if (tid == 0) S.bin = -1;
         __syncthreads();
         u64 beyond = 0;
-        auto place_of = [&](float l) { return sm_exponent(l, top, inv_t) * per; };
-        // The nearest whole number, by adding 2^23 (a conversion would hold up
-        // the exponentials' unit); `near` may be rounded past the range.
-        auto bin_at = [&](float place) {
-            return (int)min(kSmBins - 1u, __float_as_uint(place + 8388608.0f) - 0x4b000000u);
-        };
-        auto bin_of = [&](float l) { return bin_at(place_of(l)); };
+        auto place_of = [&](float l) { return sm_place(sm_exponent(l, top, inv_t), per); };
+        auto bin_of = [&](float l) { return sm_nearest(place_of(l)); };
         X.each([&](const float (&v)[E], int i) {
             if (!mass) {
 #pragma unroll
@@ -459,7 +469,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
 #pragma unroll
             for (int e = 0; e < E; e++)
                 if (v[e] >= near) {                    // some have weight 0: not in after all
-                    const int b = bin_at(x[e] * per);  // bin_of
+                    const int b = sm_nearest(sm_place(x[e], per));   // bin_of
                     atomicAdd(&S.hist[0][b], w[e] & 0xffffu);
                     atomicAdd(&S.hist[1][b], w[e] >> 16);
                 }
@@ -507,13 +517,12 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
         const int bin = S.bin;
         if (bin < 0) return false;                     // a count past all tokens of any weight: nothing to cut
         u64 above = S.found_before;
-        // A token's place within the bin, in parts of it (of part `sub`, where a part is in question)
+        // A token's part of the bin (of part `sub` of it, where that is in question)
         int sub = -1;
-        auto place_in_bin = [&](float l) {
-            const float at = (place_of(l) - (float)bin + 0.5f) * kSmBins;
-            return sub < 0 ? at : (at - (float)sub) * kSmBins;
+        auto part_of = [&](float l) { return sm_part(sm_part_place(place_of(l), bin)); };
+        auto part_of_sub = [&](float l) {
+            return sm_part(__fmul_rn(__fsub_rn(sm_part_place(place_of(l), bin), (float)sub), (float)kSmBins));
         };
-        auto part_at = [&](float place) { return bin_at(fmaxf(place - 0.5f, 0.0f)); };
         // Tokens of bins from .. bin (of part `sub` of the bin) into the lists of their CTAs, then
         // (if they fit) into the first CTA's; how many there are. Bounds a
         // little past the bins (half a bin to either side of whole numbers)
@@ -535,7 +544,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
                     if (fabsf(v[e] - mid) > half || !(v[e] >= near)) continue;
                     const int b = bin_of(v[e]);
                     if (b >= from && b <= bin && in(v[e], i + e) &&
-                        (sub < 0 || part_at((place_of(v[e]) - (float)bin + 0.5f) * kSmBins) == sub)) {
+                        (sub < 0 || part_of(v[e]) == sub)) {
                         const int at = atomicAdd(&S.n_list, 1);
                         if (at < kSmList) S.list[at] = ((u64)sm_key(v[e]) << 32) | (0xffffffffu - (uint32_t)(i + e));
                     }
@@ -580,7 +589,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
                 for (int e = 0; e < E; e++)
                     if (v[e] >= near && bin_of(v[e]) == bin && in(v[e], i + e)) {
                         const uint32_t w = mass ? sm_weight(sm_exp(v[e], top, inv_t)) : 1u;
-                        const int b = part_at(place_in_bin(v[e]));
+                        const int b = part_of(v[e]);   // sub is not set yet
                         atomicAdd(&S.hist[0][b], w & 0xffffu);
                         if (mass) atomicAdd(&S.hist[1][b], w >> 16);
                     }
@@ -603,7 +612,8 @@ __global__ void __launch_bounds__(kSmThreads, 2) k_sample(const SmParams P) {
                     const bool on = tid + e * kSmThreads < have;
                     y[e] = on ? S.list[tid + e * kSmThreads] : 0;
                     val[e] = on ? value(y[e]) : 0;
-                    part[e] = on ? part_at(place_in_bin(sm_unkey((uint32_t)(y[e] >> 32)))) : -1;
+                    const float l = sm_unkey((uint32_t)(y[e] >> 32));
+                    part[e] = !on ? -1 : sub < 0 ? part_of(l) : part_of_sub(l);
                 }
                 __syncthreads();                       // the list is read: its room becomes counters again
                 for (int i = tid; i < 2 * kSmBins; i += kSmThreads) (&S.hist[0][0])[i] = 0;
