@@ -15,6 +15,7 @@ replays a CUDA graph changes them in place.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import torch
 
@@ -90,7 +91,7 @@ class Kv8Step:
         st.max_kv = -1 if max_kv is None else int(max_kv)
         self.n_tokens, self.struct, self._keep = st.n_tokens, st, (table, kv_len, start, slot)
         self.device, self.index = kv_len.device, kv_len.device.index
-        self._max_kv, self._bound, self._ws = max_kv, {}, {}
+        self._max_kv, self._bound, self._ws, self._lock = max_kv, {}, {}, threading.Lock()
 
     def _for(self, cache):
         """The address of the step's struct for this cache's block size."""
@@ -104,7 +105,8 @@ class Kv8Step:
         return r[0]
 
     def workspace(self, cache, attn, key, stream):
-        """The attention workspace for one shape. One per stream: a workspace serves one call at a time."""
+        """The attention workspace for one shape and stream. It serves one call at a time, which takes
+        two launches in a row: callers hold the step's lock from here to the call's end."""
         ws = self._ws.get(key)
         if ws is None:
             nb = load().sepia_cuda_kv8_attn_ws_bytes(cache._ref, self._for(cache), C.addressof(attn))
@@ -213,7 +215,8 @@ class Kv8Cache:
         if tau is not None:
             a.tau = _check(tau, "tau", torch.float32, (n,))
         st = _stream(step.index, stream)
-        ws = step.workspace(self, a, (st, a.x_f16, h, self.n_kv_heads, d, self.block, window), stream)
-        if not self._attn(self._ref, step._for(self), C.addressof(a), ws[0], ws[1], st):
-            raise RuntimeError(f"sepia_b200: kv8_attn failed: {last_error()}")
+        with step._lock:                               # host threads that share a step take turns
+            ws = step.workspace(self, a, (st, a.x_f16, h, self.n_kv_heads, d, self.block, window), stream)
+            if not self._attn(self._ref, step._for(self), C.addressof(a), ws[0], ws[1], st):
+                raise RuntimeError(f"sepia_b200: kv8_attn failed: {last_error()}")
         return out
