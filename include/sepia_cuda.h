@@ -250,7 +250,7 @@ typedef struct {
  * position past the rotation table does, whose rows stay unrotated. Two
  * sequences of a step never share a block that the step writes, nor a slot. */
 typedef struct {
-    int32_t n_seqs, n_tokens;            /* n_tokens: new tokens of all sequences */
+    int32_t n_seqs, n_tokens;            /* at most 65535 sequences (attention); new tokens of all of them */
     int32_t max_new, max_kv;             /* per sequence: new tokens, tokens held after the step */
     int32_t table_cols;
     const int32_t *table;                /* [n_seqs, table_cols]: block of positions [c*block, (c+1)*block) */
@@ -287,7 +287,8 @@ int sepia_cuda_kv8_append(const SepiaKv8Cache *c, const SepiaKv8Step *b, const S
  * A row whose scores are all -infinity gives zeros. tau NULL means 1.
  * The workspace (16-byte aligned, never read before it is written) belongs
  * to one call at a time. A key or value that is not a number spoils the rows
- * that see its position, and no other. */
+ * that see its position, and no other. Refused: max_new * n_heads from 2^30,
+ * n_heads * rel_extent from 2^31 / 17. */
 typedef struct {
     int32_t x_f16;                       /* q and out: 1 fp16, 0 fp32; scores, weights' sums and outputs are summed in
                                             fp32, an fp32 q and the weights are held to 22 bits, an fp16 out is rounded once */

@@ -64,6 +64,7 @@ struct K8Params {
     SepiaKv8Step b;
     SepiaKv8Attn a;
     int G, row_tiles, splits, chunk;     // chunk: positions per split, a multiple of kK8Unit * kK8Warps
+    int tile0;                           // the launch's first row tile (0 where tiles are cut into chunks)
     int q_vec;                           // four elements of q in one load
     float *part;                         // [n_seqs, n_kv_heads * row_tiles, splits, rows of a tile, Dh]
     float2 *part_ml;                     // [n_seqs, n_kv_heads * row_tiles, splits, rows of a tile]: maximum, sum
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
     extern __shared__ __align__(16) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
     const int split = blockIdx.x, s = blockIdx.z;
-    const int hk = blockIdx.y / P.row_tiles, rt = blockIdx.y - hk * P.row_tiles;
+    const int tile = P.tile0 + blockIdx.y, hk = tile / P.row_tiles, rt = tile - hk * P.row_tiles;
     const int Dh = FULL ? DP : P.c.head_dim, B = P.c.block, H = P.a.n_heads, Hkv = P.c.n_kv_heads, G = P.G;
     griddep_wait();
     griddep_launch();
@@ -891,13 +892,19 @@ static K8Plan k8_plan(const SepiaKv8Cache &c, const SepiaKv8Step &b, const Sepia
 }
 
 template <typename T, int DP, int NB, bool FULL>
-static int k8_launch(const K8Params &P, cudaStream_t st) {
+static int k8_launch(K8Params &P, cudaStream_t st) {
     using F = K8Cfg<T, DP, NB>;
     const int64_t rows = (int64_t)P.b.max_new * P.a.n_heads;
     const int smem = std::max(F::kQB + kK8Warps * F::stage(P.a.rel_extent > 0), F::kMergeB);
     if (!ensure_smem((const void *)k_kv8_attn<T, DP, NB, FULL>, smem)) return 0;
-    const dim3 grid((unsigned)P.splits, (unsigned)(P.c.n_kv_heads * P.row_tiles), (unsigned)P.b.n_seqs);
-    if (!check(launch_pdl(k_kv8_attn<T, DP, NB, FULL>, grid, dim3(kK8Threads), smem, st, P), "kv8_attn launch")) return 0;
+    // The tiles of a long piece of a prompt (16384 tokens of 64 heads) may be
+    // more than a grid's y holds; k8_plan cuts tiles only where they are few.
+    constexpr int kMaxY = 65535;
+    const int tiles = P.c.n_kv_heads * P.row_tiles;
+    for (P.tile0 = 0; P.tile0 < tiles; P.tile0 += kMaxY) {
+        const dim3 grid((unsigned)P.splits, (unsigned)std::min(kMaxY, tiles - P.tile0), (unsigned)P.b.n_seqs);
+        if (!check(launch_pdl(k_kv8_attn<T, DP, NB, FULL>, grid, dim3(kK8Threads), smem, st, P), "kv8_attn launch")) return 0;
+    }
     if (P.splits == 1) return 1;
     // One warp per row while a row has few chunks, four beyond: 64 sequences of
     // 4 chunks 86 us (four warps: 98), one of 65 chunks 21 us (one warp: 25).
@@ -908,12 +915,12 @@ static int k8_launch(const K8Params &P, cudaStream_t st) {
 }
 
 template <typename T, int DP, bool FULL>
-static int k8_launch_rows(const K8Params &P, int rt, cudaStream_t st) {
+static int k8_launch_rows(K8Params &P, int rt, cudaStream_t st) {
     return rt == 8 ? k8_launch<T, DP, 1, FULL>(P, st) : k8_launch<T, DP, 2, FULL>(P, st);
 }
 
 template <typename T>
-static int k8_launch_dim(const K8Params &P, int rt, cudaStream_t st) {
+static int k8_launch_dim(K8Params &P, int rt, cudaStream_t st) {
     const int Dh = P.c.head_dim;
     if (Dh <= 64) return Dh == 64 ? k8_launch_rows<T, 64, true>(P, rt, st) : k8_launch_rows<T, 64, false>(P, rt, st);
     return Dh == 128 ? k8_launch_rows<T, 128, true>(P, rt, st) : k8_launch_rows<T, 128, false>(P, rt, st);
@@ -952,7 +959,7 @@ extern "C" int sepia_cuda_kv8_attn(const SepiaKv8Cache *c, const SepiaKv8Step *b
     if (a->q_stride < (int64_t)a->n_heads * c->head_dim) return fail("%s: q_stride is shorter than a token", what);
     if (a->rel_extent && !a->rel_logits) return fail("%s: rel_extent without rel_logits", what);
     const K8Plan p = k8_plan(*c, *b, *a);
-    if ((int64_t)c->n_kv_heads * p.row_tiles > 65535) return fail("%s: step too large", what);
+    if (p.splits > 1 && (int64_t)c->n_kv_heads * p.row_tiles > 65535) return fail("%s: step too large", what);
     if (!ws || ws_bytes < std::max<size_t>(16, p.bytes)) return fail("%s: workspace of %zu bytes < %zu needed", what, ws_bytes, p.bytes);
     if (reinterpret_cast<uintptr_t>(ws) & 15) return fail("%s: workspace must be 16-byte aligned", what);
     K8Params P;

@@ -101,3 +101,22 @@ def test_steps_with_start_need_no_max_new(lib):
     assert torch.equal(results[0][0], results[1][0]) and torch.allclose(results[0][1], results[1][1], rtol=0, atol=1e-5)
     assert torch.all(results[1][1] != 0)
     assert Kv8Step(B.table, B.kv_len).struct.max_new == 1
+
+
+def test_a_prompt_of_many_row_tiles(lib):
+    """16384 new tokens of 64 heads at once: what the append takes, the attention takes."""
+    hk, h, dim, n, window = 8, 64, 16, 16384, 24
+    B = Batch([0], hk, dim, 64, seed=13, room=n)
+    B.append([n], advance=False)
+    q = torch.randn(n, h, dim, device="cuda")
+    out = B.cache.attention(B.step([n]), q, 1.0 / dim, window=window)
+    B.kv_len += n
+    keys, vals = (torch.tensor(B.held(0, w)[0]).repeat_interleave(h // hk, dim=1) for w in (0, 1))
+    for t in [0, 1, 23, 24, n // 2, n - 1, *B.rng.integers(0, n, 200).tolist()]:
+        at = slice(max(0, t - window + 1), t + 1)
+        w = torch.softmax(torch.einsum("hd,jhd->hj", q[t].cpu().double(), keys[at]) / dim, dim=1)
+        want = torch.einsum("hj,jhd->hd", w, vals[at])
+        # an fp32 sum of exact products, twice, and 2^-19 for exponentials and sums (test_gpu_kv8.py)
+        top = torch.einsum("hd,jhd->hj", q[t].abs().cpu().double(), keys[at].abs()).max() / dim
+        tol = (2 * dim * 2.0 ** -24 * float(top) + 2.0 ** -19) * float(vals[at].abs().max())
+        assert float((out[t].cpu().double() - want).abs().max()) <= tol, t
