@@ -67,7 +67,7 @@ typedef struct {
     int32_t n_layers;
     int32_t vocab, unpadded_vocab;
     int32_t d_rel, conv_k, window;
-    int32_t max_positions;                  /* KV cache capacity */
+    int32_t max_positions;                  /* KV cache capacity; a token past it sets the device error word to 2 */
     float eps;                              /* (float)rms_norm_eps */
     float mup;                              /* (float)logits_mup_width_multiplier */
     int32_t has_log_scaling;

@@ -201,7 +201,9 @@ struct PrepArgs {
     int64_t kv_dim;
     float eps;
     int is_sliding, window;
-    const double *tau_table;    // per position (global layers)
+    const double *tau_table;    // per position (global layers), `cap` of them
+    int64_t cap;                // positions that the caches hold
+    int *err;
     ModelState *st;
     // relative-position band: rel_logits[h, r] = sum_d r_vec[h, d] rel_proj[d, r]
     const float *r_vec, *rel_proj;
@@ -250,7 +252,13 @@ __global__ void __launch_bounds__(128) k_attn_prep(const PrepArgs A) {
         A.rel_logits[i] = (float)acc;
         return;
     }
-    const int64_t pos = A.st->pos;
+    // A token past the caches' end sets the error word; it takes the last
+    // position's place (fp32 cache) or no part in attention (8-bit cache).
+    int64_t pos = A.st->pos;
+    if (pos >= A.cap) {
+        pos = A.cap - 1;
+        if (blockIdx.x == 0 && d == 0) set_error(A.err, kErrBadArgs);
+    }
     const double tau = (A.is_sliding || !A.tau_table) ? 1.0 : A.tau_table[pos];
     if ((int)blockIdx.x < A.H) {
         const int h = blockIdx.x;
@@ -577,7 +585,7 @@ int run_layers(SepiaModel *m, bool want_logits, cudaStream_t st, const float *u 
         P.q_norm = L.q_norm; P.k_norm = L.k_norm; P.k_sconv = L.k_sconv; P.v_sconv = L.v_sconv;
         P.H = H; P.Hkv = Hkv; P.Dh = Dh; P.K = K; P.kv_dim = kv_dim; P.eps = d.eps;
         P.is_sliding = L.is_sliding; P.window = d.window; P.tau_table = d.has_log_scaling ? m->tau : nullptr;
-        P.st = m->st;
+        P.st = m->st; P.cap = d.max_positions; P.err = dev_info().err;
         P.r_vec = m->r; P.rel_proj = L.rel_proj; P.rel_logits = m->rl; P.d_rel = (int)d.d_rel;
         P.E = L.rel_extent;
         P.k_conv = m->kv_block ? m->k : nullptr;

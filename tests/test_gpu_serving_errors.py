@@ -72,3 +72,29 @@ def test_a_call_after_a_failed_one_writes_its_own_arrays(model, sampled):
     run(new, u_new)
     torch.cuda.synchronize()
     assert torch.equal(new, want) and torch.equal(old, kept)
+
+
+@pytest.mark.parametrize("kv_block", [0, 16])
+def test_tokens_past_the_capacity(model, lib, tmp_path, kv_block):
+    """They set the error word and touch nothing outside the caches: the tokens
+    before them and a sequence after a reset are as ever."""
+    from sepia_b200.model import DeviceModel
+    d, _, _ = G.build("baseline_types", tmp_path / "m")
+    ids = torch.as_tensor(np.random.default_rng(1).integers(0, 400, 48).astype(np.int32), device="cuda")
+    m = DeviceModel.from_container(d, max_positions=40, kv_block=kv_block)
+    torch.cuda.synchronize()
+    lib.sepia_cuda_device_error(None)
+
+    def upto(n):
+        m.reset()
+        m.prefill(ids[:n], True)
+        return m.logits()
+    want = upto(40)
+    out = torch.empty(6, dtype=torch.int32, device="cuda")
+    assert lib.sepia_cuda_device_error(None) == 0
+    upto(48)
+    assert lib.sepia_cuda_device_error(None) == 2
+    upto(37)
+    m.decode(out)                                       # three of the six fit
+    assert lib.sepia_cuda_device_error(None) == 2
+    assert torch.equal(upto(40), want) and lib.sepia_cuda_device_error(None) == 0
