@@ -266,7 +266,8 @@ typedef struct {
  * elements from one token to the next, so q, k and v may be slices of one
  * projection's rows. */
 typedef struct {
-    int32_t x_f16;                       /* q, k, v and q_out: 1 fp16, 0 fp32 (arithmetic in fp32 either way) */
+    int32_t x_f16;                       /* q, k, v and q_out: 1 fp16, 0 fp32; either way queries are worked out in
+                                            fp32 and keys in fp64, before they are rounded to fp16 and 8 bits */
     int32_t n_heads;                     /* query heads; read only with q */
     const void *k, *v;                   /* [n_tokens, n_kv_heads, head_dim] */
     int64_t k_stride, v_stride;

@@ -12,7 +12,7 @@
 //
 // A prompt is bound by HBM and, close behind, by instructions (a norm is a
 // warp reduction for 4 values a lane): 8192 tokens, 64 heads over 8, fp32, 120
-// us, 5.2 TB/s with 69 % of the issue slots busy. One token is latency, 4.1 us:
+// us, 5.2 TB/s with 69 % of the issue slots busy. One token is latency, 4.0 us:
 // launch, lengths, rows (one round of loads for a whole block), norm, store.
 // 128-thread CTAs lost on every size (one token 7.8 us, 8192 tokens 144).
 #include "kv8.cuh"
@@ -135,7 +135,8 @@ __device__ __forceinline__ const float2 *rotation_row(const SepiaKv8Append &a, i
 
 // MR: rows of a block per warp. A kernel for each block size: with one for
 // blocks of 64 the shorter ones ran through rows that they do not have (48
-// tokens, blocks of 32: 10.0 us, 7.8 now; ragged pieces, blocks of 16: 21.5, 16.3).
+// tokens, blocks of 32: 10.0 us, 7.8 now; ragged pieces, blocks of 16: 21.5, 16.2).
+// Blocks of 64 keep 8 rows in flight at 64 registers a thread and spill 16 to 23 words.
 template <typename T, int MR>
 __global__ void __launch_bounds__(kApThreads, MR == 2 ? 5 : 4) k_kv8_append(const ApParams P) {
     __shared__ float s_amax[kApWarps];

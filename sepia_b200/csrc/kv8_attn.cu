@@ -26,10 +26,10 @@
 //             slots hold one step: keys are fetched again as soon as their
 //             scores are done, values when their output is, each behind the
 //             other half of the step and three more warps of the scheduler.
-//   Measured  1 x 32768, 64 heads over 8, fp32: 21 us, of which 12 (5.6 TB/s)
+//   Measured  1 x 32768, 64 heads over 8, fp32: 20.5 us, of which 12 (5.6 TB/s)
 //             are key steps and the rest start and merge; 64 ragged sequences
-//             of 2048 to 4096, fp16: 86 us, 4.8 TB/s; a window of 4096: 10.6 us.
-//             With more rows (12 x 6001, 4 new tokens: 78 us) the chains of
+//             of 2048 to 4096, fp16: 89 us, 4.6 TB/s; a window of 4096: 9.7 us.
+//             With more rows (12 x 6001, 4 new tokens: 79 us) the chains of
 //             conversions and products bind, 25 us at the product's full rate.
 #include "kv8.cuh"
 #include "runtime.h"
@@ -147,8 +147,9 @@ __device__ __forceinline__ void put_row(T *to, const float (&A)[4], float L) {
 }
 
 // FULL: head_dim is DP (64 or 128), every offset a constant; otherwise the
-// dims past head_dim are read as zeros (128 dims that way: 1 x 32768 23.3 us,
-// constant 21.3; 64 sequences 90 and 86).
+// dims past head_dim are read as zeros (128 dims that way: 1 x 32768 22.0 us,
+// constant 20.5; 64 sequences 93.5 and 89). Four CTAs an SM leave 128 registers,
+// and the forms for 128 dims spill 8 to 40 bytes (those with FULL 8 and 12).
 template <typename T, int DP, int NB, bool FULL>
 __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Params P) {
     using F = K8Cfg<T, DP, NB>;
@@ -513,7 +514,7 @@ __global__ void __launch_bounds__(kK8Threads, k8_ctas(NB)) k_kv8_attn(const K8Pa
         for (int u = 0; u < U; u++) {
             const float il = exp2_fast(-lv[u]);
             // weights as two fp16 terms, for fp16 rows too: with one (11 bits) 41 % of the
-            // results of 64 fp16 sequences were not the exact ones' fp16 values (86 us), with two 0.2 % (88 us)
+            // results of 64 fp16 sequences were not the exact ones' fp16 values (86 us), with two 0.2 % (88.5)
             uint32_t w[NB][2][2];
 #pragma unroll
             for (int g = 0; g < NB; g++) {
@@ -865,18 +866,21 @@ struct K8Plan {
 
 // Chunks: one wave of equal chunks over all CTA slots while that leaves a
 // chunk at most kMaxChunk positions; longer work runs in several waves of
-// kMaxChunk, so that ragged sequences even out (64 ragged sequences: 85 us
-// with 1024, 90 with 512). Where rows alone make four waves (long pieces of
-// prompts) nothing is cut: 512 new tokens on 4096 take 485 us, cut 569, and no
+// kMaxChunk, so that ragged sequences even out (64 ragged sequences: 89 us
+// with 1024, 95 with 512). Where rows alone make four waves (long pieces of
+// prompts) nothing is cut: 512 new tokens on 4096 take 497 us, cut 582, and no
 // workspace.
 static K8Plan k8_plan(const SepiaKv8Cache &c, const SepiaKv8Step &b, const SepiaKv8Attn &a) {
     constexpr int64_t kUnit = kK8Unit * kK8Warps, kMaxChunk = 1024;
     K8Plan p;
     p.G = a.n_heads / c.n_kv_heads;
     // Two groups of 8 rows a tile convert half the codes, but take 168
-    // registers a thread where one takes 128: 4 new tokens of 8 heads a KV head
-    // (32 rows) 85 us, with one group 79; 16 tokens (128 rows) 196 and 210, 512
-    // tokens 485 and 547.
+    // registers a thread where one takes 128. Measured as one group / two (us,
+    // fp32, 8 heads a KV head): 12 sequences of 6001 with 32 rows 79 / 86, 48
+    // rows 115 / 115, 64 rows 151 / 147, 72 rows 169 / 164, 128 rows 295 / 274;
+    // 1 x 32768 with 40 rows 62 / 69, 64 rows 90 / 85; 6 x 300 with 48 rows 18.1 /
+    // 17.9, 64 rows 19.8 / 24.4. From 48 to 64 rows neither side wins; the rule
+    // keeps the one that small calls need.
     const int rt = p.rt = (int64_t)b.max_new * p.G <= 64 ? 8 : 16;
     p.row_tiles = (int)(((int64_t)b.max_new * p.G + rt - 1) / rt);
     const int64_t span = a.window ? std::min<int64_t>(b.max_kv, (int64_t)a.window + b.max_new + kK8Tile) : b.max_kv;
@@ -907,7 +911,7 @@ static int k8_launch(K8Params &P, cudaStream_t st) {
     }
     if (P.splits == 1) return 1;
     // One warp per row while a row has few chunks, four beyond: 64 sequences of
-    // 4 chunks 86 us (four warps: 98), one of 65 chunks 21 us (one warp: 25).
+    // 4 chunks 89 us (four warps: 101), one of 64 chunks 20.5 us (one warp: 25).
     const dim3 g1((unsigned)((rows + kK8Warps - 1) / kK8Warps), (unsigned)P.b.n_seqs), g4((unsigned)rows, (unsigned)P.b.n_seqs);
     const cudaError_t e = P.splits <= 8 ? launch_pdl(k_kv8_merge<T, NB, 1>, g1, dim3(kK8Threads), 0, st, P)
                                         : launch_pdl(k_kv8_merge<T, NB, 4>, g4, dim3(kK8Threads), 0, st, P);
